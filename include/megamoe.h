@@ -368,6 +368,125 @@ int mm_moe_backward(const uint16_t* dy, const uint16_t* x, const uint16_t* w1,
                     uint16_t* grad_hidden, float* grad_rw,
                     uint16_t* grad_gate_up, mm_stream_t stream);
 
+/* ------------------------------------------- a few tokens, whole layer */
+
+/* Most tokens of mm_moe_few and mm_moe_few_int8. */
+#define MM_FEW_MAX_TOKENS 64
+/* Columns of the activation that share a scale in mm_moe_few_int8. */
+#define MM_FEW_ACT_GROUP 32
+
+/*
+ * The forward of the layer for 0 <= tokens <= MM_FEW_MAX_TOKENS in two
+ * launches, without routing tables: for route r = t * top_k + j of expert
+ * e = selected[r] (ids outside [0, E) carry no expert),
+ *   act[r] = bf16(act_fn(x[t] w1[e] gate, up) * routing_weights[r]),
+ *   out[t] = bf16(sum_j act[t * top_k + j] w2[e]^T),
+ * sums in fp32, the slots in slot order; unlike mm_moe_forward it rounds
+ * neither gate and up nor the expert outputs to bf16. Operands as in
+ * mm_moe_forward; hidden and inter multiples of 128, top_k <= 64, E <= 32768.
+ * Scratch of mm_moe_few_scratch_bytes (int8 = 0; 0 for sizes out of range),
+ * free again when the stream has passed the call. No counterpart in the
+ * reference.
+ */
+size_t mm_moe_few_scratch_bytes(int64_t tokens, int32_t top_k, int32_t hidden,
+                                int32_t inter, int32_t int8);
+
+int mm_moe_few(const uint16_t* x, const int32_t* selected,
+               const float* routing_weights, const uint16_t* w1,
+               const uint16_t* w2, int64_t w2_se, int64_t w2_sh, int64_t w2_sf,
+               int64_t tokens, int32_t top_k, int32_t num_experts,
+               int32_t hidden, int32_t inter, int32_t act_kind,
+               float situ_beta, float situ_linear_beta, float clamp_limit,
+               uint16_t* out, void* scratch, size_t scratch_bytes,
+               mm_stream_t stream);
+
+/*
+ * mm_moe_few on int8 rows and int8 experts: x [tokens, hidden] with x_scale
+ * [tokens], w1 [E, 2 inter, hidden] (gate rows, then up rows) with w1_scale
+ * [E, 2 inter], w2 [E, hidden, inter] with w2_scale [E, hidden], all
+ * contiguous. Products are summed in int32. The activation (fp32, times the
+ * routing weight) is rounded to int8 in groups of MM_FEW_ACT_GROUP columns
+ * with scale = max |act| / 127 of the group; FC2 sums a group in int32 and the
+ * groups in fp32. Scratch of mm_moe_few_scratch_bytes with int8 = 1.
+ */
+int mm_moe_few_int8(const int8_t* x, const float* x_scale,
+                    const int32_t* selected, const float* routing_weights,
+                    const int8_t* w1, const float* w1_scale, const int8_t* w2,
+                    const float* w2_scale, int64_t tokens, int32_t top_k,
+                    int32_t num_experts, int32_t hidden, int32_t inter,
+                    int32_t act_kind, float situ_beta, float situ_linear_beta,
+                    float clamp_limit, uint16_t* out, void* scratch,
+                    size_t scratch_bytes, mm_stream_t stream);
+
+/* -------------------------------------------------- norm and 8-bit rows */
+
+/* Element types of the entries below. */
+#define MM_T_BF16 0
+#define MM_T_FP16 1
+#define MM_T_FP32 2
+#define MM_T_INT8 3
+#define MM_T_E4M3 4 /* OCP "fn": max 448 */
+
+/*
+ * Root-mean-square norm of `rows` rows of 1 <= hidden <= 32768 columns, with
+ * the residual's addition in front:
+ *   h = x + residual rounded to h_type (h = x with residual == NULL),
+ *   y = h / sqrt(mean(h^2) + eps) * weight   (weight NULL: all ones)
+ * in fp32, rounded once. x and residual have unit column strides and row
+ * strides ldx, ldr in elements, at any alignment of their type; h_out
+ * (required with residual), y, scale and rstd are contiguous. x_type is BF16,
+ * FP16 or FP32; h_type, the type of residual and h_out, is x_type or FP32;
+ * weight_type is any of the three. y_type is x_type, or INT8 / E4M3 with one
+ * scale [rows] a row: a = max |y| of the row, scale = max(a, 1e-30) / Q (Q =
+ * 127 or 448; 1 where a = 0), y = round(y / scale). A row that holds a NaN or
+ * an infinity gets scale NaN and bytes 0. rstd ([rows], or NULL) receives
+ * 1 / sqrt(mean(h^2) + eps) for the backward. No counterpart in the reference,
+ * whose layer begins behind the norm.
+ */
+int mm_rms_norm(const void* x, int64_t ldx, int32_t x_type, const void* residual,
+                int64_t ldr, int32_t h_type, const void* weight,
+                int32_t weight_type, int64_t rows, int32_t hidden, float eps,
+                void* h_out, void* y, int32_t y_type, float* scale, float* rstd,
+                mm_stream_t stream);
+
+/*
+ * Backward of mm_rms_norm with y_type == x_type:
+ *   g = dh + rstd * weight * dy - h * rstd^3 * mean(weight * dy * h),
+ *   dx = g in x_type, dresidual = g in h_type (NULL: not wanted),
+ *   dweight = sum over rows of dy * h * rstd in weight_type (NULL: not wanted)
+ * dy [rows, hidden] in x_type; dh (gradient of h_out, or NULL) and h in
+ * h_type; dx and dresidual contiguous. The rows' sums have a fixed order.
+ * The workspace is needed with dweight only.
+ */
+size_t mm_rms_norm_bwd_workspace_bytes(int64_t rows, int32_t hidden);
+
+int mm_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh,
+                    const void* h, int64_t ldh, const void* weight,
+                    int32_t weight_type, const float* rstd, int32_t x_type,
+                    int32_t h_type, int64_t rows, int32_t hidden, void* dx,
+                    void* dresidual, void* dweight, void* workspace,
+                    size_t workspace_bytes, mm_stream_t stream);
+
+/* The 8-bit output of mm_rms_norm for y = x: rows of x with one scale each. */
+int mm_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int64_t rows,
+                     int32_t cols, void* q, int32_t q_type, float* scale,
+                     mm_stream_t stream);
+
+/* ---------------------------------------------------------- int8 product */
+
+/*
+ * out[i, j] = a_scale[i] * b_scale[j] * sum_k a[i, k] * b[j, k] + bias[j]
+ * for int8 a [m, k] and b [n, k], unit column strides, row strides lda and ldb
+ * at any alignment. The sum is exact in int32 (k < 2^17); scales and bias
+ * (NULL: none; BF16, FP16 or FP32) are applied in fp32 and the result is
+ * rounded once to out_type (BF16, FP16 or FP32; row stride ldo). No
+ * counterpart in the reference.
+ */
+int mm_int8_matmul(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb,
+                   const float* a_scale, const float* b_scale, const void* bias,
+                   int32_t bias_type, int64_t m, int64_t n, int64_t k, void* out,
+                   int64_t ldo, int32_t out_type, mm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,11 @@ ACT_KINDS = {"swiglu": 0, "situglu": 1, "clamp_swiglu": 2}
 # saved FC1 output formats (MM_FC1_* in include/megamoe.h) and the FP8 scale group
 FC1_FORMATS = {"bf16": 0, "fp16": 1, "fp8": 2}
 FC1_SCALE_GROUP = 128
+# element types of the norm and the int8 product (MM_T_*)
+ELEMENT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.int8: 3, torch.float8_e4m3fn: 4}
+# the few-token layer (MM_FEW_MAX_TOKENS, MM_FEW_ACT_GROUP)
+FEW_MAX_TOKENS = 64
+FEW_ACT_GROUP = 32
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -65,6 +70,18 @@ SIGNATURES = {
                                        _P, _P, _P, _P, _P]),
     "mm_swiglu_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _P, _P, _P, _I32, _I64, _I32, _I32, _F32,
                                      _F32, _F32, _P, _P, _P]),
+    "mm_moe_few_scratch_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32]),
+    "mm_moe_few": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _F32, _F32,
+                                  _F32, _P, _P, _SZ, _P]),
+    "mm_moe_few_int8": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F32, _F32,
+                                       _F32, _P, _P, _SZ, _P]),
+    "mm_rms_norm": (ctypes.c_int, [_P, _I64, _I32, _P, _I64, _I32, _P, _I32, _I64, _I32, _F32, _P, _P, _I32, _P, _P,
+                                   _P]),
+    "mm_rms_norm_bwd_workspace_bytes": (_SZ, [_I64, _I32]),
+    "mm_rms_norm_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I32, _P, _I32, _I32, _I64, _I32, _P, _P, _P,
+                                       _P, _SZ, _P]),
+    "mm_quantize_rows": (ctypes.c_int, [_P, _I64, _I32, _I64, _I32, _P, _I32, _P, _P]),
+    "mm_int8_matmul": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _I32, _I64, _I64, _I64, _P, _I64, _I32, _P]),
 }
 
 _lib = None

@@ -326,3 +326,146 @@ def layer_backward(dy, x, w1, w2, tokens: int, top_k: int, offsets, send_token, 
               dab.data_ptr(), dscale.data_ptr(), grad_fc2.data_ptr(), dx.data_ptr(), gh.data_ptr(), grw.data_ptr(),
               ggu.data_ptr(), torch.cuda.current_stream(dy.device).cuda_stream)
     return grad_act, dab, dscale, grad_fc2, dx, gh, grw, ggu
+
+
+def _launch(device: torch.device, name: str, *args):
+    """Call an entry point on torch's current stream of ``device``, which need
+    not be the current device (kernels launch on the current one)."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream)
+
+
+def _rows(name: str, t: torch.Tensor):
+    """(address, row stride, rows) of ``t`` [..., columns] as evenly spaced rows."""
+    columns = t.shape[-1]
+    if columns > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have unit column stride")
+    if t.dim() == 2:
+        return t.data_ptr(), t.stride(0), t.shape[0]
+    if t.dim() == 1:
+        return t.data_ptr(), columns, 1
+    try:
+        flat = t.view(-1, columns)
+    except RuntimeError:
+        raise ValueError(f"the rows of {name} must be evenly spaced in memory") from None
+    return flat.data_ptr(), flat.stride(0), flat.shape[0]
+
+
+_TYPES = _lib.ELEMENT_TYPES
+
+
+def rms_norm(x, weight, residual, eps: float, out_dtype, keep_rstd: bool = False):
+    """(y, scale | None, h | None, rstd | None) for operands ``ops.norm`` has checked."""
+    dev, hidden = x.device, x.shape[-1]
+    xp, ldx, rows = _rows("x", x)
+    rp = ldr = 0
+    h = None
+    xt = ht = _TYPES[x.dtype]
+    if residual is not None:
+        rp, ldr, _ = _rows("residual", residual)
+        ht = _TYPES[residual.dtype]
+        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+    y = torch.empty(x.shape, dtype=out_dtype, device=dev)
+    scale = None if out_dtype == x.dtype else torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if keep_rstd else None
+    if rows:
+        _launch(dev, "mm_rms_norm", xp, ldx, xt, rp, ldr, ht, None if weight is None else weight.data_ptr(),
+                0 if weight is None else _TYPES[weight.dtype], rows, hidden, eps, None if h is None else h.data_ptr(),
+                y.data_ptr(), _TYPES[out_dtype], None if scale is None else scale.data_ptr(),
+                None if rstd is None else rstd.data_ptr())
+    return y, scale, h, rstd
+
+
+def rms_norm_bwd(dy, dh, h, weight, rstd, x_dtype, want_residual: bool, want_weight: bool):
+    """(dx, dresidual | None, dweight | None); dresidual is dx itself where the types agree."""
+    dev, hidden = h.device, h.shape[-1]
+
+    def rows_of(name, t):
+        try:
+            return t, _rows(name, t)
+        except ValueError:  # a gradient comes in any layout (an expanded scalar, a transposed view)
+            t = t.contiguous()
+            return t, _rows(name, t)
+
+    dy, (dyp, lddy, _) = rows_of("dy", dy)
+    dhp = lddh = 0
+    if dh is not None:
+        dh, (dhp, lddh, _) = rows_of("dh", dh)
+    hp, ldh, rows = _rows("h", h)
+    dx = torch.empty(h.shape, dtype=x_dtype, device=dev)
+    dres = None
+    if want_residual:
+        dres = dx if h.dtype == x_dtype else torch.empty(h.shape, dtype=h.dtype, device=dev)
+    dw = ws = None
+    nbytes = 0
+    if want_weight:
+        dw = torch.empty(hidden, dtype=weight.dtype, device=dev)
+        nbytes = _lib.load().mm_rms_norm_bwd_workspace_bytes(rows, hidden)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    if rows or want_weight:
+        _launch(dev, "mm_rms_norm_bwd", dyp, lddy, dhp, lddh, hp, ldh, None if weight is None else weight.data_ptr(),
+                0 if weight is None else _TYPES[weight.dtype], rstd.data_ptr(), _TYPES[x_dtype], _TYPES[h.dtype], rows,
+                hidden, dx.data_ptr(), None if dres is None or dres is dx else dres.data_ptr(),
+                None if dw is None else dw.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
+    return dx, dres, dw
+
+
+def quantize_rows(x, dtype):
+    """(q, scale) of the rows of ``x``."""
+    xp, ldx, rows = _rows("x", x)
+    q = torch.empty(x.shape, dtype=dtype, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if rows:
+        _launch(x.device, "mm_quantize_rows", xp, ldx, _TYPES[x.dtype], rows, x.shape[-1], q.data_ptr(), _TYPES[dtype],
+                scale.data_ptr())
+    return q, scale
+
+
+def int8_matmul(a, b, a_scale, b_scale, bias, out_dtype):
+    """[..., N] product of operands ``ops.int8`` has checked."""
+    ap, lda, m = _rows("a", a)
+    n, k = b.shape
+    out = torch.empty(*a.shape[:-1], n, dtype=out_dtype, device=a.device)
+    if m:
+        if m > 1 and lda < k:
+            raise ValueError("the rows of a must not overlap")
+        _launch(a.device, "mm_int8_matmul", ap, lda, b.data_ptr(), b.stride(0), a_scale.data_ptr(), b_scale.data_ptr(),
+                None if bias is None else bias.data_ptr(), 0 if bias is None else _TYPES[bias.dtype], m, n, k,
+                out.data_ptr(), n, _TYPES[out_dtype])
+    return out
+
+
+def few_forward(x, selected, routing_weights, w1, w2, num_experts: int, activation: str, situ_beta: float,
+                situ_linear_beta, clamp_limit: float):
+    """The layer for a few tokens (``mm_moe_few``), for operands the operator has validated."""
+    tokens, top_k = selected.shape
+    hidden, inter = x.shape[1], w1.shape[2] // 2
+    out = torch.empty(tokens, hidden, dtype=torch.bfloat16, device=x.device)
+    nbytes = _lib.load().mm_moe_few_scratch_bytes(tokens, top_k, hidden, inter, 0)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    se, sh, sf = w2.stride()
+    _launch(x.device, "mm_moe_few", x.data_ptr(), selected.data_ptr(), routing_weights.data_ptr(), w1.data_ptr(),
+            w2.data_ptr(), se, sh, sf, tokens, top_k, num_experts, hidden, inter, _lib.ACT_KINDS[activation],
+            situ_beta, situ_linear_beta if situ_linear_beta is not None else 0.0, clamp_limit, out.data_ptr(),
+            scratch.data_ptr(), nbytes)
+    return out
+
+
+def few_forward_int8(x, x_scale, selected, routing_weights, experts, num_experts: int, activation: str,
+                     situ_beta: float, situ_linear_beta, clamp_limit: float):
+    """The int8 layer for a few tokens (``mm_moe_few_int8``), for operands the operator has validated."""
+    tokens, top_k = selected.shape
+    hidden, inter = x.shape[1], experts.down.shape[2]
+    out = torch.empty(tokens, hidden, dtype=torch.bfloat16, device=x.device)
+    nbytes = _lib.load().mm_moe_few_scratch_bytes(tokens, top_k, hidden, inter, 1)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _launch(x.device, "mm_moe_few_int8", x.data_ptr(), x_scale.data_ptr(), selected.data_ptr(),
+            routing_weights.data_ptr(), experts.gate_up.data_ptr(), experts.gate_up_scale.data_ptr(),
+            experts.down.data_ptr(), experts.down_scale.data_ptr(), tokens, top_k, num_experts, hidden, inter,
+            _lib.ACT_KINDS[activation], situ_beta, situ_linear_beta if situ_linear_beta is not None else 0.0,
+            clamp_limit, out.data_ptr(), scratch.data_ptr(), nbytes)
+    return out

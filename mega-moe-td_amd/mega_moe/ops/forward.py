@@ -33,11 +33,14 @@ from ..config import MoEForwardConfig
 from ..runtime.routing import MoERoutingPlan, RouteTables, plan_from_tables, route
 from ._saved import MoESaved
 from ..runtime.timing import StageTimer
+from .. import _lib
 from . import _kernels as K
+from .int8 import Int8Experts
 
 # Device-kernel limits (csrc/routing.hip kMaxExperts, csrc/rowops.hip combine slots).
 MAX_EXPERTS = 32768
 MAX_TOP_K = 64
+MAX_FEW_TOKENS = _lib.FEW_MAX_TOKENS
 
 
 @dataclass
@@ -370,6 +373,76 @@ class FusedMoEForward(torch.nn.Module):
             received_routing_weights=received_w,
             send_route_indices=routing_plan.send_route_indices,
         )
+
+    # ------------------------------------------------------------ a few tokens
+    def _validate_few(self, selected_experts):
+        if selected_experts.shape[0] > MAX_FEW_TOKENS:
+            raise ValueError(f"at most {MAX_FEW_TOKENS} tokens, got {selected_experts.shape[0]}; "
+                             "use forward for more")
+
+    def _validate_few_sizes(self, two_inter):
+        if self.hidden_size % 128 or two_inter % 256:
+            raise ValueError("hidden_size and ffn size must be multiples of 128 for the MFMA tiles")
+
+    def forward_few(self, hidden_states, selected_experts, gate_up_weight, down_weight, routing_weights):
+        """The forward for at most 64 tokens in two launches (serving: one token
+        of each sequence at a time).
+
+        Arguments and result as ``forward``; sums are fp32 and only the
+        activation and the output are rounded to bf16 (``forward`` also rounds
+        gate, up and the expert outputs), so the last bits differ from
+        ``forward``'s. Nothing is saved for a backward, no workspace of the
+        operator is used and its routing generation does not move: calls may run
+        on any stream, between a forward and its backward, and captured.
+        No counterpart in the reference.
+        """
+        self._validate_dispatch_inputs(hidden_states, selected_experts)
+        self._validate_few(selected_experts)
+        self._validate_gate_up_weight(gate_up_weight, hidden_states.device)
+        self._validate_routing_weights(routing_weights, selected_experts)
+        self._validate_down_weight(down_weight, gate_up_weight, hidden_states.device)
+        self._validate_few_sizes(gate_up_weight.shape[2])
+        if not hidden_states.shape[0]:
+            return torch.empty_like(hidden_states)
+        return K.few_forward(hidden_states, selected_experts, routing_weights, gate_up_weight, down_weight,
+                             self.experts_per_rank, self.activation, self.situ_beta, self.situ_linear_beta,
+                             self.clamp_limit)
+
+    def forward_few_int8(self, tokens, token_scale, selected_experts, experts: Int8Experts, routing_weights):
+        """``forward_few`` on int8 rows and int8 experts.
+
+        ``tokens`` int8 [T, H] with fp32 ``token_scale`` [T], as ``rms_norm`` and
+        ``quantize_rows`` make them; returns bf16 [T, H]. The products are summed
+        in int32; between them the activation (times the routing weight) is
+        rounded to int8 in groups of 32 columns with the group's largest value
+        at 127. A NaN or infinite scale makes its own token's output NaN.
+        """
+        self._validate_topk_indices(selected_experts)
+        self._validate_few(selected_experts)
+        if not isinstance(experts, Int8Experts):
+            raise TypeError("experts must be an Int8Experts")
+        expected = (selected_experts.shape[0], self.hidden_size)
+        if tokens.dtype != torch.int8:
+            raise TypeError(f"tokens must use torch.int8, got {tokens.dtype}")
+        if tuple(tokens.shape) != expected or not tokens.is_contiguous():
+            raise ValueError(f"tokens must be contiguous with shape {expected}, got {tuple(tokens.shape)}")
+        if (token_scale.dtype != torch.float32 or tuple(token_scale.shape) != expected[:1]
+                or not token_scale.is_contiguous()):
+            raise ValueError(f"token_scale must be contiguous FP32 with shape {expected[:1]}")
+        self._validate_routing_weights(routing_weights, selected_experts)
+        num_experts, two_inter, hidden = experts.gate_up.shape
+        if num_experts != self.experts_per_rank or hidden != self.hidden_size:
+            raise ValueError(f"experts hold {num_experts} experts of hidden size {hidden}, expected "
+                             f"{self.experts_per_rank} of {self.hidden_size}")
+        self._validate_few_sizes(two_inter)
+        device = selected_experts.device
+        if tokens.device != device or token_scale.device != device or experts.gate_up.device != device:
+            raise ValueError("tokens, token_scale, selected_experts and experts must be on the same device")
+        if not expected[0]:
+            return torch.empty(expected, dtype=torch.bfloat16, device=device)
+        return K.few_forward_int8(tokens, token_scale, selected_experts, routing_weights, experts,
+                                  self.experts_per_rank, self.activation, self.situ_beta, self.situ_linear_beta,
+                                  self.clamp_limit)
 
     # ------------------------------------------------------------ full forward
     def _forward_staged(self, hidden_states, selected_experts, gate_up_weight, down_weight, routing_weights,
