@@ -9,10 +9,11 @@
 // itself, and reads its weights once, straight into matrix-instruction
 // operands. Weights are the instruction's rows and tokens its 16 columns, so 1
 // to 16 rows of an expert cost the same and absent ones need no masking: a
-// result column depends on its own token only. The 8 waves of a workgroup
-// share the sum's axis and join through LDS in wave order. The second launch
-// leaves fp32 rows in scratch; the workgroup that finishes a range of columns
-// last adds the tokens' slots in slot order. Every sum has a fixed order.
+// result column depends on its own token only. An expert of more rows takes
+// them 16 at a time, its weights from L2 from the second time on. The waves of
+// a workgroup share the sum's axis and join through LDS in wave order. The
+// second launch leaves fp32 rows in scratch; the workgroup that finishes a
+// tile of columns last adds the tokens' slots in slot order. Every sum has a fixed order.
 #include "common.h"
 
 namespace {
@@ -20,10 +21,13 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 512, kWaves = 8;
-constexpr int kMaxRoutes = 4096;  // 64 tokens of 64 slots
+constexpr int kTokens = 16;       // columns of the matrix instructions
 constexpr int kGroup = MM_FEW_ACT_GROUP;
 constexpr float kScaleFloor = 1e-30f;
+// 32-bit byte offsets of a lane: 24 rows of w1 (4 I bytes each), 64 tokens of x
+// (2 H), and the activation's routes (checked with the sizes)
+constexpr int kMaxDim = 1 << 20;
+constexpr int64_t kMaxStride = int64_t(1) << 25;  // and 24 rows of w2
 
 struct FewArgs {
   const void* x;              // [T, H] bf16 or int8
@@ -40,42 +44,71 @@ struct FewArgs {
   void* act;                  // [R, I] bf16 or int8
   float* act_scale;           // [R, I / 32], int8
   float* y;                   // [R, H]
-  int32_t* done;              // [column tiles + 1]: arrivals, then the number of distinct experts
+  int32_t* done;              // [fc2_tiles + 1]: arrivals at each tile, then the distinct experts
   bf16* out;                  // [T, H]
   int32_t tiles, fc2_tiles;   // column tiles of this launch, and of the second
 };
 
-// A slot of the grid is an expert where the experts are no more than the
-// routes, else a route, of which the first with its expert does the work.
-// Fills `list` with the routes of the slot's expert in ascending order and
-// returns their number, 0 if the slot has no work. Every wave scans for itself
-// and writes the same values: no barrier.
-__device__ __forceinline__ int find_routes(const FewArgs& p, int slot, uint16_t* list, int& expert) {
-  const int lane = threadIdx.x & 63;
-  const bool by_expert = p.E <= p.R;
-  const int e = by_expert ? slot : __builtin_amdgcn_readfirstlane(p.selected[slot]);
-  expert = e;
-  if (static_cast<uint32_t>(e) >= static_cast<uint32_t>(p.E)) return 0;
-  int count = 0;
-  for (int base = 0; base < p.R; base += 64) {
-    const int r = base + lane;
-    const bool hit = r < p.R && p.selected[r] == e;
-    const uint64_t mask = __ballot(hit);
-    if (!by_expert && count == 0 && mask && base + __ffsll(static_cast<unsigned long long>(mask)) - 1 != slot) return 0;
-    if (hit) list[count + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(r);
-    count += __popcll(mask);
-  }
-  return count;
+// Workgroup ids go round the 8 XCDs. Eight neighbouring tiles run on one XCD,
+// at about the same time: narrow ones share lines, and an expert's rows are
+// read in runs of a kilobyte.
+constexpr int kNear = 8;
+__device__ __forceinline__ int near_block() {
+  constexpr int G = 8 * kNear;
+  const int b = blockIdx.x, base = b / G * G;
+  if (base + G > static_cast<int>(gridDim.x)) return b;
+  return base + (b & 7) * kNear + (b - base) / 8;
 }
 
+// What a workgroup works on. A slot of the grid is an expert where the experts
+// are no more than the routes, else a route, of which the first with its expert
+// does the work. `list` (R entries) gets the routes of the slot's expert in
+// ascending order, `valid` a bit for every route with an expert; count is 0 if
+// the slot has no work. Every wave scans for itself and writes the same values
+// to LDS: no barrier.
+struct Work {
+  int slot, tile, expert, count;
+  __device__ __forceinline__ Work(const FewArgs& p, uint16_t* list, uint64_t* valid) {
+    const int block = near_block(), lane = threadIdx.x & 63;
+    slot = block / p.tiles;
+    tile = block % p.tiles;
+    count = 0;
+    const bool by_expert = p.E <= p.R;
+    expert = by_expert ? slot : __builtin_amdgcn_readfirstlane(p.selected[slot]);
+    if (static_cast<uint32_t>(expert) >= static_cast<uint32_t>(p.E)) return;
+    int n = 0, first = slot;
+    for (int base = 0; base < p.R; base += 256) {
+      int e[4];  // loaded together
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int r = base + u * 64 + lane;
+        e[u] = r < p.R ? p.selected[r] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int r0 = base + u * 64;
+        if (r0 >= p.R) break;
+        const uint64_t mask = __ballot(e[u] == expert);
+        const uint64_t live = __ballot(static_cast<uint32_t>(e[u]) < static_cast<uint32_t>(p.E));
+        if (n == 0 && mask) first = r0 + __ffsll(static_cast<unsigned long long>(mask)) - 1;
+        if (e[u] == expert) list[n + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(r0 + lane);
+        if (lane == 0) valid[r0 >> 6] = live;
+        n += __popcll(mask);
+      }
+    }
+    if (by_expert || first == slot) count = n;
+  }
+};
+
 // Clears the second launch's arrival counters and counts the distinct experts,
-// each of which arrives once at every range of columns.
+// each of which arrives once at every tile.
+template <int THREADS>
 __device__ void prepare_done(const FewArgs& p, uint32_t* bits) {
-  for (int i = threadIdx.x; i < p.fc2_tiles; i += kThreads) p.done[i] = 0;
+  for (int i = threadIdx.x; i < p.fc2_tiles; i += THREADS) p.done[i] = 0;
   const int words = (p.E + 31) / 32;
-  for (int i = threadIdx.x; i < words; i += kThreads) bits[i] = 0;
+  for (int i = threadIdx.x; i < words; i += THREADS) bits[i] = 0;
   __syncthreads();
-  for (int r = threadIdx.x; r < p.R; r += kThreads) {
+  for (int r = threadIdx.x; r < p.R; r += THREADS) {
     const uint32_t e = static_cast<uint32_t>(p.selected[r]);
     if (e < static_cast<uint32_t>(p.E)) atomicOr(&bits[e >> 5], 1u << (e & 31));
   }
@@ -90,441 +123,389 @@ __device__ void prepare_done(const FewArgs& p, uint32_t* bits) {
 }
 
 // ------------------------------------------------------------------ products
+// Every operand is addressed as a uniform base and a 32-bit offset of the lane.
+// A step's loads are issued together and awaited by its own multiplication:
+// what keeps the memory busy is that two to five workgroups fit a CU. A second
+// and a third step in registers cost that and were slower (8 experts' weights
+// are 10% faster with them, 112 experts' 10 to 20% slower).
+
 // Weights with their columns contiguous, CL columns a lane: 8 rows of CL
 // columns are transposed in registers (4 v_perm for each 16 bytes) into CL
 // operands of 16 columns x 32 rows. Column of operand c, row i: CL * i + c.
-template <int CL>
-struct ColumnWeights {
-  static constexpr int DW = CL / 2;
-  uint32_t raw[8][DW];
-  __device__ __forceinline__ void load(const bf16* p, int64_t ld) {
+// w_off: the lane's columns in row 8 * (lane / 16). Lines that a wave reads
+// whole carry the non-temporal hint (7168 x 4096, 64-column tiles: 373 us
+// against 411 for 41 experts); halves of lines do not, as the hint drops the
+// half that the neighbour comes for (640 against 503).
+template <int CL, bool STREAM>
+struct ColumnStep {
+  typedef uint32_t Raw __attribute__((ext_vector_type(CL / 2)));
+  Raw w[8];
+  bf16x8 x;
+  __device__ __forceinline__ void load(const char* wp, uint32_t w_off, int64_t row_bytes, const char* xp, uint32_t x_off) {
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      if constexpr (CL == 8) {
-        const uint4 v = load_stream16(p + r * ld);
-        raw[r][0] = v.x, raw[r][1] = v.y, raw[r][2] = v.z, raw[r][3] = v.w;
-      } else {
-        const uint2 v = load_stream8(p + r * ld);
-        raw[r][0] = v.x, raw[r][1] = v.y;
-      }
+      const Raw* p = reinterpret_cast<const Raw*>(wp + r * row_bytes + w_off);
+      w[r] = STREAM ? __builtin_nontemporal_load(p) : *p;
     }
+    __builtin_memcpy(&x, xp + x_off, 16);
   }
-  __device__ __forceinline__ bf16x8 operand(int c) const {
-    const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;
-    u32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_perm(raw[2 * i + 1][c >> 1], raw[2 * i][c >> 1], sel);
-    return __builtin_bit_cast(bf16x8, v);
-  }
-};
-
-// acc[c][n] += W^T x over this wave's steps of 32 rows (wave, wave + 8, ...).
-// w: the lane's columns in row 8 * (lane / 16); x[n]: its token's values there.
-template <int CL, int NT>
-__device__ __forceinline__ void columns_product(f32x4 (&acc)[CL][NT], const bf16* w, int64_t ld,
-                                                const bf16* const (&x)[NT], int steps, int wave) {
-  ColumnWeights<CL> cw[2];
-  bf16x8 xv[2][NT];
-  auto load = [&](int buf, int s) {
-    cw[buf].load(w + static_cast<int64_t>(s) * 32 * ld, ld);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) __builtin_memcpy(&xv[buf][n], x[n] + s * 32, 16);
-  };
-  auto multiply = [&](int buf) {
+  __device__ __forceinline__ void multiply(f32x4 (&acc)[CL]) const {
 #pragma unroll
     for (int c = 0; c < CL; ++c) {
-      const bf16x8 a = cw[buf].operand(c);
+      const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;
+      u32x4 v;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) acc[c][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, xv[buf][n], acc[c][n], 0, 0, 0);
-    }
-  };
-  if (wave >= steps) return;
-  load(0, wave);
-  for (int s = wave; s < steps; s += 2 * kWaves) {
-    if (s + kWaves < steps) load(1, s + kWaves);
-    multiply(0);
-    if (s + kWaves >= steps) break;
-    if (s + 2 * kWaves < steps) load(0, s + 2 * kWaves);
-    multiply(1);
-  }
-}
-
-// Weights with the sum's axis contiguous: 16 bytes a lane are an operand as
-// they are. G groups of 16 rows; steps of 64 elements take two instructions,
-// so that both halves of a 128-byte line are asked for together.
-template <int G, int NT>
-__device__ __forceinline__ void rows_product(f32x4 (&acc)[G][NT], const bf16* w, int64_t ld,
-                                             const bf16* const (&x)[NT], int steps, int wave) {
-  bf16x8 wv[2][2][G], xv[2][2][NT];
-  auto load = [&](int buf, int s) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-        wv[buf][h][g] = __builtin_bit_cast(bf16x8, load_stream16(w + g * 16 * ld + s * 64 + h * 32));
-#pragma unroll
-      for (int n = 0; n < NT; ++n) __builtin_memcpy(&xv[buf][h][n], x[n] + s * 64 + h * 32, 16);
-    }
-  };
-  auto multiply = [&](int buf) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          acc[g][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[buf][h][g], xv[buf][h][n], acc[g][n], 0, 0, 0);
-  };
-  if (wave >= steps) return;
-  load(0, wave);
-  for (int s = wave; s < steps; s += 2 * kWaves) {
-    if (s + kWaves < steps) load(1, s + kWaves);
-    multiply(0);
-    if (s + kWaves >= steps) break;
-    if (s + 2 * kWaves < steps) load(0, s + 2 * kWaves);
-    multiply(1);
-  }
-}
-
-// The same on int8 (steps of 128 bytes, instructions of 64). w[g]: the lane's
-// row of group g at byte 16 * (lane / 16).
-template <int G, int NT>
-struct Int8Step {
-  i32x4 w[2][G], x[2][NT];
-  __device__ __forceinline__ void load(const int8_t* const (&wp)[G], const int8_t* const (&xp)[NT], int s) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int g = 0; g < G; ++g) w[h][g] = __builtin_bit_cast(i32x4, load_stream16(wp[g] + s * 128 + h * 64));
-#pragma unroll
-      for (int n = 0; n < NT; ++n) __builtin_memcpy(&x[h][n], xp[n] + s * 128 + h * 64, 16);
+      for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_perm(w[2 * i + 1][c >> 1], w[2 * i][c >> 1], sel);
+      acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), x, acc[c], 0, 0, 0);
     }
   }
 };
 
-// Sums of the waves' partial results in wave order; item = operand * 64 + lane.
-template <int N, class V>
-__device__ __forceinline__ void leave_partials(V* red, const V* acc, int wave, int lane) {
+// Weights with the sum's axis contiguous: 16 bytes a lane are an operand as
+// they are, 16 weight rows and 64 bytes of the sum's axis an instruction. The
+// other half of each line is the next wave's or step's, so no non-temporal hint
+// here (int8, 3072 x 2048 of 112 experts: 141 us against 173). w[g]: group g.
+template <int G>
+struct RowWeights {
+  i32x4 w[G];
+  __device__ __forceinline__ void load(const char* wp, int64_t group_bytes, uint32_t w_off) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) red[(wave * N + i) * 64 + lane] = acc[i];
-}
+    for (int g = 0; g < G; ++g) __builtin_memcpy(&w[g], wp + g * group_bytes + w_off, 16);
+  }
+};
+
 template <int N, class V>
-__device__ __forceinline__ V join_partials(const V* red, int item) {
-  V s = red[item];
+__device__ __forceinline__ void clear(V (&acc)[N]) {
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) s += red[w * N * 64 + item];
-  return s;
+  for (int a = 0; a < N; ++a) acc[a] = V{0, 0, 0, 0};
 }
+
+// The W waves of a workgroup share the sum's axis: of n pieces, wave w takes w,
+// w + W, ... Their partial sums are joined through LDS in the order of the waves.
+template <int W>
+struct Waves {
+  int wave;
+  __device__ __forceinline__ Waves() : wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {}
+  template <int N, class V>
+  __device__ __forceinline__ void leave(V* red, const V (&acc)[N]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[(wave * N + i) * 64 + (threadIdx.x & 63)] = acc[i];
+  }
+  // operand `op` of the lane
+  template <int N, class V>
+  __device__ __forceinline__ V join(const V* red, int op) const {
+    const V* r = red + op * 64 + (threadIdx.x & 63);
+    V s = r[0];
+#pragma unroll
+    for (int k = 1; k < W; ++k) s += r[k * N * 64];
+    return s;
+  }
+};
+
+// LDS of a launch beside its fixed arrays: `valid`, then `list`.
+extern __shared__ uint64_t route_lds[];
+__device__ __forceinline__ uint16_t* list_of(const FewArgs& p) {
+  return reinterpret_cast<uint16_t*>(route_lds + (p.R + 63) / 64);
+}
+size_t route_lds_bytes(int R) { return static_cast<size_t>((R + 63) / 64) * 8 + static_cast<size_t>(R) * 2; }
 
 // ------------------------------------------------------------------ first launch, bf16
 // Tile of C = 8 * CL columns: operand rows 0..7 are gate, 8..15 up columns.
-template <int CL, int NT>
-__global__ __launch_bounds__(kThreads) void few_fc1_kernel(FewArgs p) {
+template <int CL, int W>
+__global__ __launch_bounds__(W * 64) void few_fc1_kernel(FewArgs p) {
   constexpr int C = 8 * CL;
-  __shared__ f32x4 red[kWaves * CL * NT * 64];
-  __shared__ uint16_t list[kMaxRoutes];
-  __shared__ __attribute__((aligned(16))) bf16 stage[NT * 16][C + 8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = lane & 15, q = lane >> 4;
-  if (blockIdx.x == 0) prepare_done(p, reinterpret_cast<uint32_t*>(red));
-  const int slot = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
-  int e;
-  const int count = find_routes(p, slot, list, e);
-  if (!count) return;
-  const int64_t ld = 2 * static_cast<int64_t>(p.I);
-  const bf16* w = static_cast<const bf16*>(p.w1) + static_cast<int64_t>(e) * p.H * ld + static_cast<int64_t>(8 * q) * ld +
-                  (j < 8 ? 0 : p.I) + tile * C + CL * (j & 7);
-  for (int c0 = 0; c0 < count; c0 += 16 * NT) {
-    const bf16* x[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-      x[n] = static_cast<const bf16*>(p.x) +
-             static_cast<int64_t>(list[min(c0 + n * 16 + j, count - 1)] / p.top_k) * p.H + 8 * q;
-    f32x4 acc[CL][NT];
-#pragma unroll
-    for (int c = 0; c < CL; ++c)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) acc[c][n] = f32x4{0, 0, 0, 0};
-    columns_product<CL, NT>(acc, w, ld, x, p.H / 32, wave);
-    leave_partials<CL * NT>(red, &acc[0][0], wave, lane);
+  __shared__ f32x4 red[W * CL * 64];
+  __shared__ __attribute__((aligned(16))) bf16 stage[kTokens][C + 8];
+  const Waves<W> ws;
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
+  uint16_t* list = list_of(p);
+  if (blockIdx.x == 0) prepare_done<W * 64>(p, reinterpret_cast<uint32_t*>(red));
+  const Work wk(p, list, route_lds);
+  if (!wk.count) return;
+  const int64_t row_bytes = 4 * static_cast<int64_t>(p.I);
+  const char* w = static_cast<const char*>(p.w1) + static_cast<int64_t>(wk.expert) * p.H * row_bytes + wk.tile * C * 2;
+  const uint32_t w_off = static_cast<uint32_t>(8 * q * row_bytes) + (j < 8 ? 0 : 2 * p.I) + CL * 2 * (j & 7);
+  for (int c0 = 0; c0 < wk.count; c0 += kTokens) {
+    const int route = list[min(c0 + j, wk.count - 1)];
+    const uint32_t x_off = (static_cast<uint32_t>(route / p.top_k) * p.H + 8 * q) * 2;
+    const float wt = p.w[route];
+    f32x4 acc[CL];
+    clear(acc);
+    for (int s = ws.wave; s < p.H / 32; s += W) {
+      ColumnStep<CL, C * 2 >= 128> st;
+      st.load(w + s * 32 * row_bytes, w_off, row_bytes, static_cast<const char*>(p.x) + s * 64, x_off);
+      st.multiply(acc);
+    }
+    ws.leave(red, acc);
     __syncthreads();
-    for (int item = tid; item < CL * NT * 64; item += kThreads) {
-      const int c = (item >> 6) / NT, n = (item >> 6) % NT;
-      const f32x4 v = join_partials<CL * NT>(red, item);
-      const int at = c0 + n * 16 + j;
-      const float wt = p.w[list[min(at, count - 1)]];
+    for (int c = ws.wave; c < CL; c += W) {
+      const f32x4 v = ws.template join<CL>(red, c);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float up = __shfl(v[r], (lane + 32) & 63);
         if (lane < 32)
-          stage[n * 16 + j][CL * (4 * q + r) + c] =
+          stage[j][CL * (4 * q + r) + c] =
               static_cast<bf16>(gated_act(p.act_kind, v[r], up, p.beta, p.lbeta, p.limit) * wt);
       }
     }
     __syncthreads();
-    for (int item = tid; item < NT * 16 * (C / 8); item += kThreads) {
+    for (int item = tid; item < kTokens * (C / 8); item += W * 64) {
       const int row = item / (C / 8), vec = item % (C / 8);
-      if (c0 + row < count)
-        *reinterpret_cast<uint4*>(static_cast<bf16*>(p.act) + static_cast<int64_t>(list[c0 + row]) * p.I + tile * C +
+      if (c0 + row < wk.count)
+        *reinterpret_cast<uint4*>(static_cast<bf16*>(p.act) + static_cast<int64_t>(list[c0 + row]) * p.I + wk.tile * C +
                                   vec * 8) = *reinterpret_cast<const uint4*>(&stage[row][vec * 8]);
     }
   }
 }
 
 // ------------------------------------------------------------------ second launch
+// y crosses the XCDs' L2 caches inside the launch: it is written and read with
+// agent-scope accesses, which go past them. A release fence would write back
+// the whole L2 of the XCD for every workgroup (8 experts, 2048 columns: 41 us
+// against 10).
+__device__ __forceinline__ void put_y(float* p, const f32x4& v) {
+  const uint64_t* w = reinterpret_cast<const uint64_t*>(&v);
+  uint64_t* d = reinterpret_cast<uint64_t*>(p);
+  __hip_atomic_store(d, w[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store(d + 1, w[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // Called by every workgroup with work once its part of y is written; the last
-// of its range of columns adds the slots. C columns, column c of a row at
-// place(c) of the range.
-template <int C, class Place>
-__device__ __forceinline__ void finish(const FewArgs& p, int tile, int live, Place place) {
+// of the tile adds the tokens' slots. y holds the tile's C columns in the order
+// that column_of gives. A thread adds 4 columns of ITEMS tokens with all loads
+// of 8 slots in flight.
+template <int C, int THREADS, class ColumnOf>
+__device__ __forceinline__ void finish(const FewArgs& p, const Work& wk, int live, ColumnOf column_of) {
+  constexpr int ITEMS = 2, Q = C / 4;
   __shared__ int last;
-  __threadfence();  // y of every thread is out before the workgroup arrives
+  // each wave's stores have reached memory before its workgroup arrives
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(&p.done[tile], 1) == live - 1;
+  if (threadIdx.x == 0)
+    last = __hip_atomic_fetch_add(&p.done[wk.tile], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == live - 1;
   __syncthreads();
   if (!last) return;
-  __threadfence();  // and the other workgroups' y is read behind their arrivals
-  for (int i = threadIdx.x; i < p.tokens * C; i += kThreads) {
-    const int t = i / C, c = i % C;
-    const float* y = p.y + static_cast<int64_t>(t) * p.top_k * p.H + tile * C + place(c);
-    float s = 0.0f;
-    for (int k0 = 0; k0 < p.top_k; k0 += 8) {
-      float v[8];
+  const int col0 = wk.tile * C, items = p.tokens * Q;
+  for (int i0 = threadIdx.x; i0 < items; i0 += ITEMS * THREADS) {
+    f32x4 s[ITEMS];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const bool in = k0 + k < p.top_k &&
-                        static_cast<uint32_t>(p.selected[t * p.top_k + k0 + k]) < static_cast<uint32_t>(p.E);
-        v[k] = in ? y[static_cast<int64_t>(k0 + k) * p.H] : 0.0f;
+    for (int u = 0; u < ITEMS; ++u) s[u] = f32x4{0, 0, 0, 0};
+    for (int k0 = 0; k0 < p.top_k; k0 += 8) {
+      uint64_t v[ITEMS][8][2];
+#pragma unroll
+      for (int u = 0; u < ITEMS; ++u) {
+        const int i = i0 + u * THREADS;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int r = i / Q * p.top_k + k0 + k;
+          v[u][k][0] = v[u][k][1] = 0;
+          if (i < items && k0 + k < p.top_k && ((route_lds[r >> 6] >> (r & 63)) & 1)) {
+            const uint64_t* y = reinterpret_cast<const uint64_t*>(p.y + static_cast<int64_t>(r) * p.H + col0 + i % Q * 4);
+            v[u][k][0] = __hip_atomic_load(y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            v[u][k][1] = __hip_atomic_load(y + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
+        }
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s += v[k];
+      for (int u = 0; u < ITEMS; ++u)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[u][r] += __uint_as_float(static_cast<uint32_t>(v[u][k][r >> 1] >> (32 * (r & 1))));
     }
-    p.out[static_cast<int64_t>(t) * p.H + tile * C + c] = static_cast<bf16>(s);
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const int i = i0 + u * THREADS;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (i < items) p.out[static_cast<int64_t>(i / Q) * p.H + col0 + column_of(i % Q * 4 + r)] = static_cast<bf16>(s[u][r]);
+    }
   }
 }
 
 // No route has an expert: the first slot's workgroups write the empty sums.
-template <int C>
-__device__ __forceinline__ void finish_empty(const FewArgs& p, int tile) {
-  for (int i = threadIdx.x; i < p.tokens * C; i += kThreads)
-    p.out[static_cast<int64_t>(i / C) * p.H + tile * C + i % C] = static_cast<bf16>(0.0f);
+template <int C, int THREADS>
+__device__ __forceinline__ void finish_empty(const FewArgs& p, const Work& wk) {
+  for (int i = threadIdx.x; i < p.tokens * C; i += THREADS)
+    p.out[static_cast<int64_t>(i / C) * p.H + wk.tile * C + i % C] = static_cast<bf16>(0.0f);
 }
 
-// ROWS: w2's sum axis is contiguous (N = 4 groups of 16 columns), else its
-// columns are (N = CL columns a lane).
-template <bool ROWS, int N, int NT>
-__global__ __launch_bounds__(kThreads) void few_fc2_kernel(FewArgs p) {
+// ROWS: w2's sum axis is contiguous (N groups of 16 columns), else its columns
+// are (N = CL columns a lane).
+template <bool ROWS, int N, int W>
+__global__ __launch_bounds__(W * 64) void few_fc2_kernel(FewArgs p) {
   constexpr int C = 16 * N;
-  __shared__ f32x4 red[kWaves * N * NT * 64];
-  __shared__ uint16_t list[kMaxRoutes];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = lane & 15, q = lane >> 4;
-  const int slot = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
+  __shared__ f32x4 red[W * N * 64];
+  const Waves<W> ws;
+  const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
+  uint16_t* list = list_of(p);
+  const Work wk(p, list, route_lds);
   const int live = p.done[p.tiles];
-  if (live == 0 && slot == 0) finish_empty<C>(p, tile);
-  int e;
-  const int count = find_routes(p, slot, list, e);
-  if (!count) return;
-  const bf16* w = static_cast<const bf16*>(p.w2) + static_cast<int64_t>(e) * p.w2_se +
-                  (ROWS ? static_cast<int64_t>(tile * C + j) * p.w2_ld + 8 * q
-                        : static_cast<int64_t>(8 * q) * p.w2_ld + tile * C + N * j);
-  for (int c0 = 0; c0 < count; c0 += 16 * NT) {
-    const bf16* x[NT];
+  if (live == 0 && wk.slot == 0) finish_empty<C, W * 64>(p, wk);
+  if (!wk.count) return;
+  const int col = wk.tile * C;
+  const int64_t row_bytes = 2 * p.w2_ld;
+  const char* w = static_cast<const char*>(p.w2) + 2 * static_cast<int64_t>(wk.expert) * p.w2_se +
+                  (ROWS ? col * row_bytes : col * 2);
+  const uint32_t w_off = ROWS ? static_cast<uint32_t>(j * row_bytes) + 16 * q
+                              : static_cast<uint32_t>(8 * q * row_bytes) + N * 2 * j;
+  const char* x = static_cast<const char*>(p.act);
+  for (int c0 = 0; c0 < wk.count; c0 += kTokens) {
+    const int64_t route = list[min(c0 + j, wk.count - 1)];
+    const uint32_t x_off = (static_cast<uint32_t>(route) * p.I + 8 * q) * 2;
+    f32x4 acc[N];
+    clear(acc);
+    for (int s = ws.wave; s < p.I / 32; s += W) {
+      if constexpr (ROWS) {
+        RowWeights<N> st;
+        bf16x8 xv;
+        st.load(w + s * 64, 16 * row_bytes, w_off);
+        __builtin_memcpy(&xv, x + s * 64 + x_off, 16);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      x[n] = static_cast<const bf16*>(p.act) + static_cast<int64_t>(list[min(c0 + n * 16 + j, count - 1)]) * p.I + 8 * q;
-    f32x4 acc[N][NT];
-#pragma unroll
-    for (int c = 0; c < N; ++c)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) acc[c][n] = f32x4{0, 0, 0, 0};
-    if constexpr (ROWS)
-      rows_product<N, NT>(acc, w, p.w2_ld, x, p.I / 64, wave);
-    else
-      columns_product<N, NT>(acc, w, p.w2_ld, x, p.I / 32, wave);
-    if (c0) __syncthreads();
-    leave_partials<N * NT>(red, &acc[0][0], wave, lane);
+        for (int g = 0; g < N; ++g)
+          acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, st.w[g]), xv, acc[g], 0, 0, 0);
+      } else {
+        ColumnStep<N, true> st;
+        st.load(w + s * 32 * row_bytes, w_off, row_bytes, x + s * 64, x_off);
+        st.multiply(acc);
+      }
+    }
+    if (c0) __syncthreads();  // the 16 tokens before have been joined
+    ws.leave(red, acc);
     __syncthreads();
-    // operand c, rows 4q..4q + 3 of token j are kept side by side in y
-    for (int item = tid; item < N * NT * 64; item += kThreads) {
-      const int c = (item >> 6) / NT, n = (item >> 6) % NT, at = c0 + n * 16 + j;
-      const f32x4 v = join_partials<N * NT>(red, item);
-      if (at < count)
-        *reinterpret_cast<f32x4*>(p.y + static_cast<int64_t>(list[at]) * p.H + tile * C + c * 16 + 4 * q) = v;
+    // rows 4q..4q + 3 of an operand and token j are kept side by side in y
+    for (int op = ws.wave; op < N; op += W) {
+      const f32x4 v = ws.template join<N>(red, op);
+      if (c0 + j < wk.count) put_y(p.y + route * p.H + col + op * 16 + 4 * q, v);
     }
   }
-  finish<C>(p, tile, live, [](int c) { return ROWS ? c : (c % N) * 16 + c / N; });
+  finish<C, W * 64>(p, wk, live, [](int at) { return ROWS ? at : at % 16 * N + at / 16; });
 }
 
 // ------------------------------------------------------------------ int8
-// Tile of 32 columns: operands 0, 1 are gate columns, 2, 3 up columns.
-template <int NT>
-__global__ __launch_bounds__(kThreads) void few_fc1_int8_kernel(FewArgs p) {
-  constexpr int C = kGroup, G = 4;
-  __shared__ i32x4 red[kWaves * G * NT * 64];
-  __shared__ uint16_t list[kMaxRoutes];
-  __shared__ float stage[NT * 16][C + 1];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = lane & 15, q = lane >> 4;
-  if (blockIdx.x == 0) prepare_done(p, reinterpret_cast<uint32_t*>(red));
-  const int slot = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
-  int e;
-  const int count = find_routes(p, slot, list, e);
-  if (!count) return;
-  const int8_t* w[G];
+// Tile of 32 columns: operands 0, 1 are gate rows of w1, 2, 3 up rows. The
+// first wave joins them and has the 32 columns of 16 tokens in its registers,
+// 8 of a token in a lane, the others 16, 32 and 48 lanes on.
+template <int W>
+__global__ __launch_bounds__(W * 64) void few_fc1_int8_kernel(FewArgs p) {
+  constexpr int C = kGroup, G = 2;
+  __shared__ i32x4 red[W * 2 * G * 64];
+  const Waves<W> ws;
+  const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
+  uint16_t* list = list_of(p);
+  if (blockIdx.x == 0) prepare_done<W * 64>(p, reinterpret_cast<uint32_t*>(red));
+  const Work wk(p, list, route_lds);
+  if (!wk.count) return;
+  const int col = wk.tile * C;
+  const int64_t up_bytes = static_cast<int64_t>(p.I) * p.H;
+  const char* w = static_cast<const char*>(p.w1) + 2 * wk.expert * up_bytes + static_cast<int64_t>(col) * p.H;
+  const uint32_t w_off = j * p.H + 16 * q;
+  for (int c0 = 0; c0 < wk.count; c0 += kTokens) {
+    const int64_t route = list[min(c0 + j, wk.count - 1)];
+    const int token = static_cast<int>(route) / p.top_k;
+    const uint32_t x_off = static_cast<uint32_t>(token) * p.H + 16 * q;
+    i32x4 acc[2 * G];
+    clear(acc);
+    for (int s = ws.wave; s < p.H / 64; s += W) {
+      RowWeights<G> gate, up;
+      i32x4 xv;
+      gate.load(w + s * 64, 16 * p.H, w_off);
+      up.load(w + up_bytes + s * 64, 16 * p.H, w_off);
+      __builtin_memcpy(&xv, static_cast<const char*>(p.x) + s * 64 + x_off, 16);
 #pragma unroll
-  for (int g = 0; g < G; ++g)
-    w[g] = static_cast<const int8_t*>(p.w1) +
-           (static_cast<int64_t>(e) * 2 * p.I + (g >> 1) * p.I + tile * C + (g & 1) * 16 + j) * p.H + 16 * q;
-  const int steps = p.H / 128;
-  for (int c0 = 0; c0 < count; c0 += 16 * NT) {
-    const int8_t* x[NT];
+      for (int g = 0; g < G; ++g) {
+        acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(gate.w[g], xv, acc[g], 0, 0, 0);
+        acc[G + g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(up.w[g], xv, acc[G + g], 0, 0, 0);
+      }
+    }
+    if (c0) __syncthreads();  // the 16 tokens before have been joined
+    ws.leave(red, acc);
+    __syncthreads();
+    if (ws.wave) continue;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      x[n] = static_cast<const int8_t*>(p.x) +
-             static_cast<int64_t>(list[min(c0 + n * 16 + j, count - 1)] / p.top_k) * p.H + 16 * q;
-    i32x4 acc[G][NT];
+    for (int g = 0; g < 2 * G; ++g) acc[g] = ws.template join<2 * G>(red, g);
+    const float sx = p.x_scale[token], wt = p.w[route];
+    const float* sc = p.w1_scale + static_cast<int64_t>(wk.expert) * 2 * p.I + col + 4 * q;
+    float a[G][4];
+    uint32_t top = 0;  // of the bit patterns, where NaN lies above infinity
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) acc[g][n] = i32x4{0, 0, 0, 0};
-    Int8Step<G, NT> st[2];
-    auto multiply = [&](const Int8Step<G, NT>& s) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) acc[g][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.w[h][g], s.x[h][n], acc[g][n], 0, 0, 0);
-    };
-    if (wave < steps) {
-      st[0].load(w, x, wave);
-      for (int s = wave; s < steps; s += 2 * kWaves) {
-        if (s + kWaves < steps) st[1].load(w, x, s + kWaves);
-        multiply(st[0]);
-        if (s + kWaves >= steps) break;
-        if (s + 2 * kWaves < steps) st[0].load(w, x, s + 2 * kWaves);
-        multiply(st[1]);
+      for (int r = 0; r < 4; ++r) {
+        a[g][r] = gated_act(p.act_kind, static_cast<float>(acc[g][r]) * (sx * sc[g * 16 + r]),
+                            static_cast<float>(acc[G + g][r]) * (sx * sc[p.I + g * 16 + r]), p.beta, p.lbeta, p.limit) * wt;
+        top = max(top, __float_as_uint(a[g][r]) & 0x7fffffffu);
       }
-    }
-    leave_partials<G * NT>(red, &acc[0][0], wave, lane);
-    __syncthreads();
-    for (int item = tid; item < 2 * NT * 64; item += kThreads) {
-      const int g = (item >> 6) / NT, n = (item >> 6) % NT;
-      const i32x4 gate = join_partials<G * NT>(red, (g * NT + n) * 64 + lane);
-      const i32x4 up = join_partials<G * NT>(red, ((g + 2) * NT + n) * 64 + lane);
-      const int route = list[min(c0 + n * 16 + j, count - 1)];
-      const float sx = p.x_scale[route / p.top_k], wt = p.w[route];
-      const float* ws = p.w1_scale + static_cast<int64_t>(e) * 2 * p.I + tile * C + g * 16 + 4 * q;
+    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+    if (c0 + j >= wk.count) continue;
+    const bool finite = top < 0x7f800000u;
+    const float most = fmaxf(__uint_as_float(top), kScaleFloor), inv = finite ? 127.0f / most : 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      uint32_t b = 0;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        stage[n * 16 + j][g * 16 + 4 * q + r] =
-            gated_act(p.act_kind, static_cast<float>(gate[r]) * (sx * ws[r]),
-                      static_cast<float>(up[r]) * (sx * ws[p.I + r]), p.beta, p.lbeta, p.limit) * wt;
+        b |= static_cast<uint32_t>(finite ? static_cast<int>(__builtin_rintf(a[g][r] * inv)) & 0xff : 0) << (8 * r);
+      *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(p.act) + route * p.I + col + g * 16 + 4 * q) = b;
     }
-    __syncthreads();
-    // 32 lanes a row: its largest value (of the bit patterns, so that NaN shows), scale and bytes
-    for (int item = tid; item < NT * 16 * C; item += kThreads) {
-      const int row = item / C, col = item % C;
-      const float v = stage[row][col];
-      uint32_t top = __float_as_uint(v) & 0x7fffffffu;
-#pragma unroll
-      for (int m = 16; m > 0; m >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), m)));
-      if (c0 + row >= count) continue;
-      const bool finite = top < 0x7f800000u;
-      const float a = fmaxf(__uint_as_float(top), kScaleFloor);
-      const int route = list[c0 + row];
-      static_cast<int8_t*>(p.act)[static_cast<int64_t>(route) * p.I + tile * C + col] =
-          finite ? static_cast<int8_t>(static_cast<int>(__builtin_rintf(v * (127.0f / a)))) : 0;
-      if (col == 0)
-        p.act_scale[static_cast<int64_t>(route) * (p.I / C) + tile] = finite ? a / 127.0f : __uint_as_float(0x7fc00000u);
-    }
+    if (q == 0) p.act_scale[route * (p.I / C) + col / C] = finite ? most / 127.0f : __uint_as_float(0x7fc00000u);
   }
 }
 
 // Tile of 64 columns. An instruction's 64 elements span two scale groups (the
-// operand's lanes 0..31 and 32..63), so each group is multiplied with the
-// other's activations zeroed and joins the fp32 sum under its own scale.
-template <int NT>
-__global__ __launch_bounds__(kThreads) void few_fc2_int8_kernel(FewArgs p) {
+// operand's lanes 0..31 and 32..63), so each is multiplied with the other's
+// activations zeroed and joins the fp32 sum under its own scale.
+template <int W>
+__global__ __launch_bounds__(W * 64) void few_fc2_int8_kernel(FewArgs p) {
   constexpr int G = 4, C = 16 * G;
-  __shared__ f32x4 red[kWaves * G * NT * 64];
-  __shared__ uint16_t list[kMaxRoutes];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = lane & 15, q = lane >> 4;
-  const int slot = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
+  __shared__ f32x4 red[W * G * 64];
+  const Waves<W> ws;
+  const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
+  uint16_t* list = list_of(p);
+  const Work wk(p, list, route_lds);
   const int live = p.done[p.tiles];
-  if (live == 0 && slot == 0) finish_empty<C>(p, tile);
-  int e;
-  const int count = find_routes(p, slot, list, e);
-  if (!count) return;
-  const int8_t* w[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g)
-    w[g] = static_cast<const int8_t*>(p.w2) + (static_cast<int64_t>(e) * p.H + tile * C + g * 16 + j) * p.I + 16 * q;
-  const int steps = p.I / 128, groups = p.I / kGroup;
-  for (int c0 = 0; c0 < count; c0 += 16 * NT) {
-    const int8_t* x[NT];
-    const float* sc[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int64_t route = list[min(c0 + n * 16 + j, count - 1)];
-      x[n] = static_cast<const int8_t*>(p.act) + route * p.I + 16 * q;
-      sc[n] = p.act_scale + route * groups;
-    }
-    f32x4 acc[G][NT];
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) acc[g][n] = f32x4{0, 0, 0, 0};
-    Int8Step<G, NT> st[2];
-    float sv[2][NT][4];
-    auto load = [&](int buf, int s) {
-      st[buf].load(w, x, s);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) __builtin_memcpy(sv[buf][n], sc[n] + s * 4, 16);
-    };
-    auto multiply = [&](int buf) {
+  if (live == 0 && wk.slot == 0) finish_empty<C, W * 64>(p, wk);
+  if (!wk.count) return;
+  const int col = wk.tile * C;
+  const char* w = static_cast<const char*>(p.w2) + (static_cast<int64_t>(wk.expert) * p.H + col) * p.I;
+  const uint32_t w_off = j * p.I + 16 * q;
+  for (int c0 = 0; c0 < wk.count; c0 += kTokens) {
+    const int64_t route = list[min(c0 + j, wk.count - 1)];
+    const uint32_t x_off = static_cast<uint32_t>(route) * p.I + 16 * q;
+    const uint32_t sc_off = static_cast<uint32_t>(route) * (p.I / kGroup) * 4;
+    f32x4 acc[G];
+    clear(acc);
+    for (int s = ws.wave; s < p.I / 64; s += W) {
+      RowWeights<G> st;
+      i32x4 xv;
+      float sv[2];
+      st.load(w + s * 64, 16 * p.I, w_off);
+      __builtin_memcpy(&xv, static_cast<const char*>(p.act) + s * 64 + x_off, 16);
+      __builtin_memcpy(sv, reinterpret_cast<const char*>(p.act_scale) + s * (64 / kGroup * 4) + sc_off, 8);
       const i32x4 zero = {0, 0, 0, 0};
+      const i32x4 lo = lane < 32 ? xv : zero, hi = lane < 32 ? zero : xv;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int g = 0; g < G; ++g) {
+        const i32x4 a = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.w[g], lo, zero, 0, 0, 0);
+        const i32x4 b = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.w[g], hi, zero, 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const i32x4 lo = lane < 32 ? st[buf].x[h][n] : zero, hi = lane < 32 ? zero : st[buf].x[h][n];
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-            const i32x4 a = __builtin_amdgcn_mfma_i32_16x16x64_i8(st[buf].w[h][g], lo, zero, 0, 0, 0);
-            const i32x4 b = __builtin_amdgcn_mfma_i32_16x16x64_i8(st[buf].w[h][g], hi, zero, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              acc[g][n][r] += static_cast<float>(a[r]) * sv[buf][n][2 * h] + static_cast<float>(b[r]) * sv[buf][n][2 * h + 1];
-          }
-        }
-    };
-    if (wave < steps) {
-      load(0, wave);
-      for (int s = wave; s < steps; s += 2 * kWaves) {
-        if (s + kWaves < steps) load(1, s + kWaves);
-        multiply(0);
-        if (s + kWaves >= steps) break;
-        if (s + 2 * kWaves < steps) load(0, s + 2 * kWaves);
-        multiply(1);
+        for (int r = 0; r < 4; ++r) acc[g][r] += static_cast<float>(a[r]) * sv[0] + static_cast<float>(b[r]) * sv[1];
       }
     }
-    if (c0) __syncthreads();
-    leave_partials<G * NT>(red, &acc[0][0], wave, lane);
+    if (c0) __syncthreads();  // the 16 tokens before have been joined
+    ws.leave(red, acc);
     __syncthreads();
-    for (int item = tid; item < G * NT * 64; item += kThreads) {
-      const int g = (item >> 6) / NT, n = (item >> 6) % NT, at = c0 + n * 16 + j;
-      f32x4 v = join_partials<G * NT>(red, item);
-      const float* ws = p.w2_scale + static_cast<int64_t>(e) * p.H + tile * C + g * 16 + 4 * q;
+    for (int op = ws.wave; op < G; op += W) {
+      f32x4 v = ws.template join<G>(red, op);
+      const int at = col + op * 16 + 4 * q;
+      const float* sc = p.w2_scale + static_cast<int64_t>(wk.expert) * p.H + at;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] *= ws[r];
-      if (at < count)
-        *reinterpret_cast<f32x4*>(p.y + static_cast<int64_t>(list[at]) * p.H + tile * C + g * 16 + 4 * q) = v;
+      for (int k = 0; k < 4; ++k) v[k] *= sc[k];
+      if (c0 + j < wk.count) put_y(p.y + route * p.H + at, v);
     }
   }
-  finish<C>(p, tile, live, [](int c) { return c; });
+  finish<C, W * 64>(p, wk, live, [](int at) { return at; });
 }
 
 // ------------------------------------------------------------------ host
@@ -547,24 +528,30 @@ struct FewScratch {
 
 bool few_sizes_ok(int64_t tokens, int32_t top_k, int32_t E, int32_t H, int32_t I) {
   return tokens >= 0 && tokens <= MM_FEW_MAX_TOKENS && top_k > 0 && top_k <= 64 && E > 0 && E <= 32768 && H > 0 &&
-         H % 128 == 0 && I > 0 && I % 128 == 0 && H <= (1 << 20) && I <= (1 << 20);
+         H % 128 == 0 && I > 0 && I % 128 == 0 && H <= kMaxDim && I <= kMaxDim &&
+         tokens * top_k * I < (int64_t(1) << 31);
 }
 
 int slots_of(const FewArgs& p) { return p.E <= p.R ? p.E : p.R; }
 
-// Two launches of (slots x column tiles) workgroups each.
-template <class K1, class K2>
-int launch_both(FewArgs p, int c1, K1 k1, int c2, K2 k2, hipStream_t s) {
-  const int slots = slots_of(p), tiles1 = p.I / c1, tiles2 = p.H / c2;
+// One launch: its waves and its tiles of `width` columns.
+struct Launch {
+  void (*kernel)(FewArgs);
+  int waves, width;
+};
+
+int launch_both(FewArgs p, const Launch& a, const Launch& b, hipStream_t s) {
+  const int slots = slots_of(p), tiles1 = p.I / a.width, tiles2 = p.H / b.width;
   MM_CHECK_ARG(static_cast<int64_t>(slots) * (tiles1 > tiles2 ? tiles1 : tiles2) < (int64_t(1) << 23),
                "mm_moe_few: too many tiles");
+  const size_t lds = route_lds_bytes(p.R);
   p.fc2_tiles = tiles2;
   p.tiles = tiles1;
-  k1<<<slots * tiles1, kThreads, 0, s>>>(p);
+  a.kernel<<<slots * tiles1, a.waves * 64, lds, s>>>(p);
   const int rc = mm_check_launch("few_fc1_kernel");
   if (rc) return rc;
   p.tiles = tiles2;
-  k2<<<slots * tiles2, kThreads, 0, s>>>(p);
+  b.kernel<<<slots * tiles2, b.waves * 64, lds, s>>>(p);
   return mm_check_launch("few_fc2_kernel");
 }
 
@@ -582,6 +569,8 @@ extern "C" int mm_moe_few(const uint16_t* x, const int32_t* selected, const floa
                           size_t scratch_bytes, mm_stream_t stream) {
   MM_CHECK_ARG(few_sizes_ok(tokens, top_k, num_experts, hidden, inter), "mm_moe_few: bad sizes");
   MM_CHECK_ARG(w2_sh == 1 || w2_sf == 1, "mm_moe_few: w2 needs a unit stride along hidden or inter");
+  MM_CHECK_ARG(w2_sh >= 0 && w2_sh <= kMaxStride && w2_sf >= 0 && w2_sf <= kMaxStride,
+               "mm_moe_few: w2 rows more than 2^25 elements apart");
   MM_CHECK_ARG(act_kind >= MM_ACT_SWIGLU && act_kind <= MM_ACT_CLAMP_SWIGLU, "mm_moe_few: bad activation");
   if (tokens == 0) return MM_OK;
   const FewScratch f(tokens * top_k, hidden, inter, false);
@@ -598,12 +587,12 @@ extern "C" int mm_moe_few(const uint16_t* x, const int32_t* selected, const floa
             reinterpret_cast<float*>(base + f.y), reinterpret_cast<int32_t*>(base + f.done),
             reinterpret_cast<bf16*>(out), 0, 0};
   const hipStream_t s = mm_hip_stream(stream);
-  if (tokens <= 16) {
-    if (rows) return launch_both(p, 32, few_fc1_kernel<4, 1>, 64, few_fc2_kernel<true, 4, 1>, s);
-    return launch_both(p, 32, few_fc1_kernel<4, 1>, 64, few_fc2_kernel<false, 4, 1>, s);
-  }
-  if (rows) return launch_both(p, 64, few_fc1_kernel<8, 2>, 64, few_fc2_kernel<true, 4, 2>, s);
-  return launch_both(p, 64, few_fc1_kernel<8, 2>, 128, few_fc2_kernel<false, 8, 2>, s);
+  // 64 columns a tile read whole lines; with fewer workgroups than two to a CU
+  // 32 columns, twice as many, win (8 experts of 1024 columns: 25 us against 40;
+  // of 768, one token: 12.3 against 17.8; 112 experts of 768: 156 against 117)
+  const bool wide = static_cast<int64_t>(slots_of(p)) * (inter / 64) >= 512;
+  return launch_both(p, wide ? Launch{few_fc1_kernel<8, 8>, 8, 64} : Launch{few_fc1_kernel<4, 8>, 8, 32},
+                     rows ? Launch{few_fc2_kernel<true, 4, 8>, 8, 64} : Launch{few_fc2_kernel<false, 4, 8>, 8, 64}, s);
 }
 
 extern "C" int mm_moe_few_int8(const int8_t* x, const float* x_scale, const int32_t* selected,
@@ -629,6 +618,5 @@ extern "C" int mm_moe_few_int8(const int8_t* x, const float* x_scale, const int3
             reinterpret_cast<float*>(base + f.act_scale), reinterpret_cast<float*>(base + f.y),
             reinterpret_cast<int32_t*>(base + f.done), reinterpret_cast<bf16*>(out), 0, 0};
   const hipStream_t s = mm_hip_stream(stream);
-  if (tokens <= 16) return launch_both(p, 32, few_fc1_int8_kernel<1>, 64, few_fc2_int8_kernel<1>, s);
-  return launch_both(p, 32, few_fc1_int8_kernel<2>, 64, few_fc2_int8_kernel<2>, s);
+  return launch_both(p, {few_fc1_int8_kernel<4>, 4, kGroup}, {few_fc2_int8_kernel<4>, 4, 64}, s);
 }
