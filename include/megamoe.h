@@ -477,7 +477,7 @@ int mm_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int64_t rows,
 /*
  * out[i, j] = a_scale[i] * b_scale[j] * sum_k a[i, k] * b[j, k] + bias[j]
  * for int8 a [m, k] and b [n, k], unit column strides, row strides lda and ldb
- * at any alignment. The sum is exact in int32 (k < 2^17); scales and bias
+ * from k to 2^23 at any alignment. The sum is exact in int32 (k < 2^17); scales and bias
  * (NULL: none; BF16, FP16 or FP32) are applied in fp32 and the result is
  * rounded once to out_type (BF16, FP16 or FP32; row stride ldo). No
  * counterpart in the reference.

@@ -5,6 +5,8 @@
 // a [M, K] and b [N, K] are int8 with K contiguous. The sum is exact in int32
 // (|sum| <= 2^14 K < 2^31 for K < 2^17), the scales and the bias are applied
 // in fp32 and the result is rounded once to the output's type.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -13,6 +15,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMaxK = (1 << 17) - 1;
+constexpr int64_t kMaxStride = int64_t(1) << 23;  // 256 rows of a tile in 32-bit offsets
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 512;  // a tile's last row stays in 32 bits
 
 struct I8Args {
@@ -26,114 +29,477 @@ struct I8Args {
   int32_t m, n, k, out_type, bias_type;
 };
 
-// 16 bytes of a row from byte k on, from any address (gfx950 loads 16 bytes
-// at any alignment); bytes at or past K read as zero and are not touched.
-__device__ __forceinline__ i32x4 load16(const int8_t* row, int k, int K) {
-  i32x4 v = {0, 0, 0, 0};
-  const int n = K - k;
-  if (n >= 16) {
-    __builtin_memcpy(&v, row + k, 16);
-  } else if (n > 0) {
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 15; ++i)
-      if (i < n) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + i])) << (8 * (i & 3));
-    v = i32x4{static_cast<int>(w[0]), static_cast<int>(w[1]), static_cast<int>(w[2]), static_cast<int>(w[3])};
-  }
-  return v;
+// Workgroup id -> tile: the ids of an XCD (congruent mod 8) take a run of tiles,
+// 8 rows of tiles deep, so that rows and channels are reused from its L2.
+__device__ __forceinline__ void tile_of(int num_m, int num_n, int& mt, int& nt) {
+  const int total = num_m * num_n, per = total / 8, rest = total % 8, x = blockIdx.x & 7;
+  const int l = x * per + min(x, rest) + (blockIdx.x >> 3);
+  constexpr int DEEP = 8;
+  const int group = l / (DEEP * num_n), first = group * DEEP, rows = min(DEEP, num_m - first), in = l - group * DEEP * num_n;
+  mt = first + in % rows;
+  nt = in / rows;
 }
 
+// Four consecutive columns of a row, from their whole sums.
 __device__ __forceinline__ float load_any(const void* p, int type, int64_t at) {
   if (type == MM_T_FP32) return static_cast<const float*>(p)[at];
   if (type == MM_T_FP16) return static_cast<float>(static_cast<const _Float16*>(p)[at]);
   return static_cast<float>(static_cast<const bf16*>(p)[at]);
 }
 
-__device__ __forceinline__ void store_any(void* p, int type, int64_t at, float v) {
-  if (type == MM_T_FP32)
-    static_cast<float*>(p)[at] = v;
-  else if (type == MM_T_FP16)
-    static_cast<_Float16*>(p)[at] = static_cast<_Float16>(v);
-  else
-    static_cast<bf16*>(p)[at] = static_cast<bf16>(v);
+// The scales and the bias of four consecutive columns, loaded once for all of a
+// lane's rows: fetched row by row, each store waited for them (256 x 256 tiles:
+// 41 us an epilogue, 6 so).
+struct Columns4 {
+  float sb[4], bias[4];
+  int col, left;  // columns left from col on
+  __device__ __forceinline__ Columns4(const I8Args& p, int c) : col(c), left(p.n - c) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int at = min(c + r, p.n - 1);
+      sb[r] = p.sb[at];
+      bias[r] = p.bias ? load_any(p.bias, p.bias_type, at) : 0.0f;
+    }
+  }
+  __device__ __forceinline__ void store(const I8Args& p, int row, float sa, const i32x4& v) const {
+    float f[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = static_cast<float>(v[r]) * sa * sb[r] + bias[r];
+    const int64_t at = row * p.ldo + col;
+    if (p.out_type == MM_T_FP32) {
+      float* out = static_cast<float*>(p.out) + at;
+      if (left >= 4) {
+        __builtin_memcpy(out, f, 16);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 3; ++r)
+          if (r < left) out[r] = f[r];
+      }
+      return;
+    }
+    const uint2 h = p.out_type == MM_T_FP16 ? make_uint2(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]))
+                                            : make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+    uint16_t* out = static_cast<uint16_t*>(p.out) + at;
+    if (left >= 4) {
+      __builtin_memcpy(out, &h, 8);
+    } else {
+      if (left > 0) out[0] = static_cast<uint16_t>(h.x);
+      if (left > 1) out[1] = static_cast<uint16_t>(h.x >> 16);
+      if (left > 2) out[2] = static_cast<uint16_t>(h.y);
+    }
+  }
+};
+
+// Sixteen bytes of a row as an operand. Rows that do not begin on 4-byte
+// borders (SHIFT) are read as the five aligned words around them and shifted:
+// 16-byte loads from odd addresses take the memory pipe twice as long (1021 x
+// 2305 x 1793: 25 us that way, YY this). A word is read only if it holds a byte
+// of the sixteen. `base` is aligned to 4 and the same for the wave.
+__device__ __forceinline__ i32x4 join16(const uint32_t (&d)[5], uint32_t sh) {
+  i32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = static_cast<int>(__builtin_amdgcn_alignbyte(d[i + 1], d[i], sh));
+  return v;
 }
 
-// LDS tile [ROWS][128 bytes]: 16-byte slot s of row r sits at s ^ ((r >> 1) & 7),
-// which gives the 16 rows of one pass of a fragment read distinct banks.
+template <bool SHIFT>
+__device__ __forceinline__ i32x4 load16(const char* base, uint32_t off) {
+  if constexpr (!SHIFT) {
+    i32x4 v;
+    __builtin_memcpy(&v, base + off, 16);
+    return v;
+  } else {
+    const uint32_t sh = off & 3;
+    const char* p = base + (off - sh);
+    uint32_t d[5];
+    __builtin_memcpy(d, __builtin_assume_aligned(p, 4), 16);
+    __builtin_memcpy(d + 4, __builtin_assume_aligned(p + (sh ? 16 : 12), 4), 4);
+    return join16(d, sh);
+  }
+}
+
+// The same of a row with n bytes left: bytes past them read as zero and are
+// not touched.
+__device__ __forceinline__ i32x4 load16_cut(const char* base, uint32_t off, int n) {
+  const int sh = off & 3;
+  const uint32_t* p = reinterpret_cast<const uint32_t*>(base + (off - sh));
+  uint32_t d[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) d[i] = n > 0 && 4 * i < n + sh && 4 * i < 16 + sh ? p[i] : 0;
+  i32x4 v = join16(d, sh);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int keep = n - 4 * i;
+    v[i] &= keep >= 4 ? -1 : keep <= 0 ? 0 : (1 << (8 * keep)) - 1;
+  }
+  return v;
+}
+
+// Address of a row as an aligned base and what is left of it.
+__device__ __forceinline__ const char* aligned_base(const int8_t* p, uint32_t& rest) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  rest = a & 3;
+  return reinterpret_cast<const char*>(a - rest);
+}
+
+// ------------------------------------------------------------------ operands from memory
+// Tile of 16 G channels x 16 NT tokens for products that a grid of large tiles
+// would not fill the chip with. Channels are the rows of v_mfma_i32_16x16x64_i8
+// and tokens its columns; 16 bytes of a row are a lane's operand as they lie in
+// memory. The W waves share the sum's axis in pieces of 128 bytes (wave w takes
+// w, w + W, ...), U of them in flight, and join through LDS.
+template <int G, int NT, int W, int U, bool SHIFT>
+__global__ __launch_bounds__(W * 64) void int8_direct_kernel(I8Args p) {
+  __shared__ i32x4 red[W * G * NT * 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, q = lane >> 4;
+  // every XCD gets a run of channels with all their tokens
+  const int total = gridDim.x, per = (total + 7) / 8, tiles_m = (p.m + NT * 16 - 1) / (NT * 16);
+  int tile = blockIdx.x;
+  if (total % 8 == 0) tile = (tile & 7) * per + (tile >> 3);
+  const int n0 = tile / tiles_m * (G * 16), m0 = tile % tiles_m * (NT * 16);
+  uint32_t b_off[G], a_off[NT], rest_a, rest_b;
+  const char* a = aligned_base(p.a + m0 * p.lda, rest_a);
+  const char* b = aligned_base(p.b + n0 * p.ldb, rest_b);
+#pragma unroll
+  for (int g = 0; g < G; ++g) b_off[g] = static_cast<uint32_t>(min(g * 16 + j, p.n - 1 - n0)) * static_cast<uint32_t>(p.ldb) + rest_b + 16 * q;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) a_off[n] = static_cast<uint32_t>(min(n * 16 + j, p.m - 1 - m0)) * static_cast<uint32_t>(p.lda) + rest_a + 16 * q;
+  i32x4 acc[G][NT];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[g][n] = i32x4{0, 0, 0, 0};
+  const int full = p.k / 128;
+  auto steps = [&](auto count, int s) {
+    constexpr int C = decltype(count)::value;
+    i32x4 bv[C][G][2], av[C][NT][2];
+#pragma unroll
+    for (int u = 0; u < C; ++u) {
+      const int at = (s + u * W) * 128;
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) bv[u][g][h] = load16<SHIFT>(b + at + h * 64, b_off[g]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) av[u][n][h] = load16<SHIFT>(a + at + h * 64, a_off[n]);
+    }
+#pragma unroll
+    for (int u = 0; u < C; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            acc[g][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bv[u][g][h], av[u][n][h], acc[g][n], 0, 0, 0);
+  };
+  int s = wave;
+  for (; s + (U - 1) * W < full; s += U * W) steps(std::integral_constant<int, U>{}, s);
+  for (; s < full; s += W) steps(std::integral_constant<int, 1>{}, s);
+  if (p.k % 128 && s == full) {  // the last piece of the sum, cut at K
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = full * 128 + h * 64;
+      i32x4 bv[G], av[NT];
+#pragma unroll
+      for (int g = 0; g < G; ++g) bv[g] = load16_cut(b + at, b_off[g], p.k - at - 16 * q);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) av[n] = load16_cut(a + at, a_off[n], p.k - at - 16 * q);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[g][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bv[g], av[n], acc[g][n], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) red[(wave * G * NT + n * G + g) * 64 + lane] = acc[g][n];
+  __syncthreads();
+  for (int op = wave; op < G * NT; op += W) {
+    i32x4 v = red[op * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v += red[(w * G * NT + op) * 64 + lane];
+    const int row = m0 + op / G * 16 + j;
+    if (row < p.m) Columns4(p, n0 + op % G * 16 + 4 * q).store(p, row, p.sa[row], v);
+  }
+}
+
+// ------------------------------------------------------------------ tiles through LDS
+// BM x BN tile, WM x WN waves of (BM / WM) x (BN / WN) in v_mfma_i32_32x32x32_i8
+// blocks. Stages of 128 bytes of the sum's axis go through registers, PRE
+// stages ahead, into a ring of two LDS buffers; one barrier a stage. The
+// operands are swapped, so a lane holds 4 consecutive columns of one row.
+//
+// A sum in int32 has no order: the stage that K cuts comes first, with its
+// missing bytes zeroed, and every other stage is whole.
+//
+// With KS > 1 a stage is KS pieces of 128 bytes, one for each of KS groups of
+// WM x WN waves; the groups' sums are joined at the end. Products of few tiles
+// then have KS times fewer stages, one after the other, and KS times the bytes
+// in flight.
 constexpr int BK = 128;
+
+// LDS rows of 128 bytes: 16-byte slot s of row r sits at s ^ ((r >> 1) & 7),
+// which gives the 16 rows of one pass of a fragment read distinct banks.
 __device__ __forceinline__ int slot_of(int r, int s) { return r * BK + ((s ^ ((r >> 1) & 7)) << 4); }
 
-// 128 x 128 tile, 4 waves of 64 x 64 in v_mfma_i32_32x32x32_i8 blocks. The
-// operands are swapped, so a lane holds 4 consecutive columns of one row.
-__global__ __launch_bounds__(256) void int8_tile_kernel(I8Args p) {
-  constexpr int BM = 128, BN = 128;
-  __shared__ __attribute__((aligned(16))) int8_t As[BM * BK], Bs[BN * BK];
-  const int num_n = (p.n + BN - 1) / BN;
-  const int m0 = blockIdx.x / num_n * BM, n0 = blockIdx.x % num_n * BN;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
-  const int8_t *pa[4], *pb[4];
+// ROWS rows of a stage: KS sub-panels of [ROWS][128], filled by NT threads.
+template <int ROWS, int NT, int KS, bool SHIFT>
+struct Panel {
+  static constexpr int VPR = 8 * KS, PER = ROWS * VPR / NT;  // 16-byte vectors a row, a thread
+  static_assert(PER * NT == ROWS * VPR && NT % VPR == 0, "whole vectors");
+  const char* base;
+  uint32_t off[PER];
+  __device__ __forceinline__ void init(const int8_t* p, int64_t ld, int r0, int rows) {
+    uint32_t rest;
+    base = aligned_base(p + r0 * ld, rest);
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    const int r = (v * 256 + tid) >> 3;
-    pa[v] = p.a + static_cast<int64_t>(min(m0 + r, p.m - 1)) * p.lda;
-    pb[v] = p.b + static_cast<int64_t>(min(n0 + r, p.n - 1)) * p.ldb;
-  }
-  const int s = tid & 7;
-  i32x4 ra[4], rb[4];
-  auto load = [&](int k0) {
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      ra[v] = load16(pa[v], k0 + s * 16, p.k);
-      rb[v] = load16(pb[v], k0 + s * 16, p.k);
+    for (int v = 0; v < PER; ++v) {
+      const int c = v * NT + threadIdx.x;
+      off[v] = static_cast<uint32_t>(min(c / VPR, rows - 1 - r0)) * static_cast<uint32_t>(ld) + rest + c % VPR * 16;
     }
-  };
-  i32x16 acc[2][2];
+  }
+  __device__ __forceinline__ void load(i32x4 (&r)[PER], int k) const {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int v = 0; v < PER; ++v) r[v] = load16<SHIFT>(base + k, off[v]);
+  }
+  __device__ __forceinline__ void load_cut(i32x4 (&r)[PER], int k, int K) const {
+    const int in = threadIdx.x % VPR * 16;  // the same for all of a thread's vectors
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int v = 0; v < PER; ++v) r[v] = load16_cut(base + k, off[v], K - k - in);
+  }
+  __device__ __forceinline__ static void put(int8_t* lds, const i32x4 (&r)[PER]) {
+#pragma unroll
+    for (int v = 0; v < PER; ++v) {
+      const int c = v * NT + threadIdx.x, s = c % VPR;
+      *reinterpret_cast<i32x4*>(lds + s / 8 * ROWS * BK + slot_of(c / VPR, s % 8)) = r[v];
+    }
+  }
+};
+
+template <int BM, int BN, int WM, int WN, int KS, int PRE, bool SHIFT>
+__global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) {
+  constexpr int NT = WM * WN * KS * 64, STEP = KS * BK, MI = BM / WM / 32, NI = BN / WN / 32;
+  __shared__ __attribute__((aligned(1024))) int8_t smem[2][(BM + BN) * STEP];
+  const int num_m = (p.m + BM - 1) / BM, num_n = (p.n + BN - 1) / BN;
+  int mt, nt;
+  tile_of(num_m, num_n, mt, nt);
+  const int m0 = mt * BM, n0 = nt * BN;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ks = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
+  Panel<BM, NT, KS, SHIFT> pa;
+  Panel<BN, NT, KS, SHIFT> pb;
+  pa.init(p.a, p.lda, m0, p.m);
+  pb.init(p.b, p.ldb, n0, p.n);
+  i32x16 acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
-  load(0);
-  for (int k0 = 0; k0 < p.k; k0 += BK) {
-    __syncthreads();
+
+  const int cut = p.k % STEP, stages = (p.k + STEP - 1) / STEP;
+  i32x4 ra[PRE][Panel<BM, NT, KS, SHIFT>::PER], rb[PRE][Panel<BN, NT, KS, SHIFT>::PER];
+  // stage s > 0 begins at byte (s - 1) * STEP, or s * STEP where K cuts none
+  const int shift = cut ? STEP : 0;
+  if (cut) {
+    pa.load_cut(ra[0], p.k - cut, p.k);
+    pb.load_cut(rb[0], p.k - cut, p.k);
+  } else {
+    pa.load(ra[0], 0);
+    pb.load(rb[0], 0);
+  }
+  Panel<BM, NT, KS, SHIFT>::put(smem[0], ra[0]);
+  Panel<BN, NT, KS, SHIFT>::put(smem[0] + BM * STEP, rb[0]);
+  // loads past the last stage repeat it (K >= STEP: there is a whole one)
+  auto at = [&](int s) { return max(min(s, stages - 1) * STEP - shift, 0); };
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int r = (v * 256 + tid) >> 3;
-      *reinterpret_cast<i32x4*>(As + slot_of(r, s)) = ra[v];
-      *reinterpret_cast<i32x4*>(Bs + slot_of(r, s)) = rb[v];
-    }
-    __syncthreads();
-    if (k0 + BK < p.k) load(k0 + BK);
+  for (int u = 0; u < PRE; ++u) {
+    pa.load(ra[u], at(u + 1));
+    pb.load(rb[u], at(u + 1));
+  }
+  __syncthreads();
+  i32x4 fa[2][MI], fb[2][NI];
+  auto frags = [&](int set, const int8_t* buf, int kk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+      fa[set][i] = *reinterpret_cast<const i32x4*>(buf + ks * BM * BK + slot_of(wm * (BM / WM) + i * 32 + (lane & 31), kk * 2 + (lane >> 5)));
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+      fb[set][j] = *reinterpret_cast<const i32x4*>(buf + BM * STEP + ks * BN * BK + slot_of(wn * (BN / WN) + j * 32 + (lane & 31), kk * 2 + (lane >> 5)));
+  };
+  auto mfmas = [&](int set) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[set][j], fa[set][i], acc[i][j], 0, 0, 0);
+  };
+  frags(0, smem[0], 0);
+  // Sub-steps of 32 bytes: the next one's fragments are read while this one
+  // multiplies. Stage s + 1 goes from its registers to LDS in sub-steps 0 (a)
+  // and 1 (b) and its registers take stage s + 1 + PRE; the barrier after
+  // sub-step 2 publishes it, and its first fragments are read in sub-step 3.
+  // Past the last stage the writes land where nobody reads any more.
+  auto stage = [&](int s, auto reg) __attribute__((always_inline)) {
+    constexpr int R = decltype(reg)::value;
+    const int8_t* cur = smem[s & 1];
+    int8_t* nxt = smem[(s + 1) & 1];
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      i32x4 fa[2], fb[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fa[i] = *reinterpret_cast<const i32x4*>(As + slot_of(wm * 64 + i * 32 + (lane & 31), kk * 2 + (lane >> 5)));
-        fb[i] = *reinterpret_cast<const i32x4*>(Bs + slot_of(wn * 64 + i * 32 + (lane & 31), kk * 2 + (lane >> 5)));
+      frags((kk + 1) & 1, kk < 3 ? cur : nxt, (kk + 1) & 3);
+      mfmas(kk & 1);
+      if (kk == 0) {
+        Panel<BM, NT, KS, SHIFT>::put(nxt, ra[R]);
+        pa.load(ra[R], at(s + 1 + PRE));
+      }
+      if (kk == 1) {
+        Panel<BN, NT, KS, SHIFT>::put(nxt + BM * STEP, rb[R]);
+        pb.load(rb[R], at(s + 1 + PRE));
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[j], fa[i], acc[i][j], 0, 0, 0);
+      for (int g = 0; g < MI * NI; ++g) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+        __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // LDS write
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // global load
+      }
+      if (kk == 2) __syncthreads();
+    }
+  };
+  for (int s = 0; s < stages; s += PRE) {
+    stage(s, std::integral_constant<int, 0>{});
+    if constexpr (PRE > 1) {
+      if (s + 1 < stages) stage(s + 1, std::integral_constant<int, 1>{});
     }
   }
+
+  // Epilogue, 32 rows of a wave at a time: through its own LDS (the padding
+  // keeps 16-byte writes of consecutive rows on different banks), so that
+  // neighbouring lanes store neighbouring columns.
+  constexpr int COLS = BN / WN, PITCH = COLS + 4, LANES = COLS / 4;
+  static_assert(WM * WN * 32 * PITCH * 4 <= sizeof(smem), "epilogue staging");
+  __syncthreads();
+  if constexpr (KS > 1) {  // group 0 adds the others' sums, one group at a time
+    static_assert(BM * BN * 4 <= sizeof(smem), "a group's sums");
+    i32x4* red = reinterpret_cast<i32x4*>(&smem[0][0]) + (wm * WN + wn) * (MI * NI * 4 * 64) + lane;
+    for (int k = 1; k < KS; ++k) {
+      if (ks == k) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = m0 + wm * 64 + i * 32 + (lane & 31);
-    if (row >= p.m) continue;
-    const float sa = p.sa[row];
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < NI; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int col = n0 + wn * 64 + j * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
-        if (col >= p.n) continue;
-        float v = static_cast<float>(acc[i][j][r]) * sa * p.sb[col];
-        if (p.bias) v += load_any(p.bias, p.bias_type, col);
-        store_any(p.out, p.out_type, static_cast<int64_t>(row) * p.ldo + col, v);
+            for (int g = 0; g < 4; ++g)
+              red[((i * NI + j) * 4 + g) * 64] =
+                  i32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
       }
+      __syncthreads();
+      if (ks == 0) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const i32x4 v = red[((i * NI + j) * 4 + g) * 64];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[i][j][4 * g + r] += v[r];
+            }
+      }
+      __syncthreads();
+    }
+    if (ks) return;
+  }
+  i32x4* out = reinterpret_cast<i32x4*>(&smem[0][0]) + wave * (32 * PITCH / 4);
+  const int c = lane % LANES * 4;
+  const Columns4 columns(p, n0 + wn * COLS + c);
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int r0 = m0 + wm * (BM / WM) + i * 32;
+    const float sa = p.sa[min(r0 + (lane & 31), p.m - 1)];
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        out[((lane & 31) * PITCH + j * 32 + g * 8 + (lane >> 5) * 4) / 4] =
+            i32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+#pragma unroll 4
+    for (int k = 0; k < 32 * LANES / 64; ++k) {
+      const int r = k * (64 / LANES) + lane / LANES;
+      const float s = __shfl(sa, r);
+      if (r0 + r < p.m) columns.store(p, r0 + r, s, out[(r * PITCH + c) / 4]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ choice
+int launch(void (*kernel)(I8Args), int64_t tiles, int threads, const I8Args& p, hipStream_t s) {
+  MM_CHECK_ARG(tiles * threads < (int64_t(1) << 32), "mm_int8_matmul: too many tiles");
+  kernel<<<static_cast<uint32_t>(tiles), threads, 0, s>>>(p);
+  return mm_check_launch("int8_matmul");
+}
+
+int64_t tiles_of(const I8Args& p, int bm, int bn) {
+  return ((static_cast<int64_t>(p.m) + bm - 1) / bm) * ((static_cast<int64_t>(p.n) + bn - 1) / bn);
+}
+
+template <int G, int NT, int W, int U>
+int launch_direct(const I8Args& p, bool shift, hipStream_t s) {
+  return launch(shift ? int8_direct_kernel<G, NT, W, U, true> : int8_direct_kernel<G, NT, W, U, false>,
+                tiles_of(p, NT * 16, G * 16), W * 64, p, s);
+}
+
+template <int BM, int BN, int WM, int WN, int KS, int PRE, bool SHIFT>
+int launch_tiles(const I8Args& p, hipStream_t s) {
+  return launch(int8_tile_kernel<BM, BN, WM, WN, KS, PRE, SHIFT>, tiles_of(p, BM, BN), WM * WN * KS * 64, p, s);
+}
+
+// Time of a product in us by its tiles: every 256 of them take `round` + `byte`
+// a byte of K, as measured on full rounds (and about 4 us in all). Tiles below
+// 64 x 64 gain from the bytes they have in flight while the chip is not full.
+struct TileCost {
+  int bm, bn, step;  // step: K has to reach one whole stage
+  double round, byte;
+};
+constexpr TileCost kTileCosts[] = {
+    {256, 256, 128, 17.0, 13.3e-3}, {128, 128, 128, 4.0, 5.0e-3}, {64, 64, 128, 1.5, 1.75e-3},
+    {32, 64, 512, 2.0, 1.4e-3},     {32, 32, 1024, 2.0, 1.15e-3},
+};
+
+int best_tile(const I8Args& p) {
+  int best = 0;
+  double least = 1e300;
+  for (int i = 0; i < 5; ++i) {
+    const TileCost& c = kTileCosts[i];
+    const double t = static_cast<double>((tiles_of(p, c.bm, c.bn) + 255) / 256) * (c.round + c.byte * p.k);
+    if (p.k >= c.step && t < least) best = i, least = t;
+  }
+  return best;
+}
+
+int launch_best(const I8Args& p, hipStream_t s) {
+  // rows on 4-byte borders need no shifting; the two largest tiles leave odd
+  // addresses to the memory pipe, which their longer stages hide (2048 x 4097 x
+  // 4096: 80 us in 128 x 128 tiles against 90 with shifts)
+  const bool shift = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.lda | p.ldb) & 3) != 0;
+  // 16 rows: 7168 x 4096 in 8 us, the smallest tiles 11
+  if (p.m <= 16) return launch_direct<1, 1, 16, 4>(p, shift, s);
+  if (p.k < BK) return launch_direct<4, 4, 1, 1>(p, shift, s);  // not one whole stage
+  switch (best_tile(p)) {
+    case 0: return launch_tiles<256, 256, 2, 2, 1, 1, false>(p, s);
+    case 1: return launch_tiles<128, 128, 2, 2, 1, 2, false>(p, s);
+    case 2:
+      // the sum shared by two groups of waves until the chip is full (256 x
+      // 7168 x 4096, 256 tiles: 19 us against 24; 464 tiles of 2309: 23 against 20)
+      if (p.k >= 2 * BK && tiles_of(p, 64, 64) <= 256)
+        return shift ? launch_tiles<64, 64, 2, 2, 2, 2, true>(p, s) : launch_tiles<64, 64, 2, 2, 2, 2, false>(p, s);
+      return shift ? launch_tiles<64, 64, 2, 2, 1, 2, true>(p, s) : launch_tiles<64, 64, 2, 2, 1, 2, false>(p, s);
+    case 3: return shift ? launch_tiles<32, 64, 1, 2, 4, 2, true>(p, s) : launch_tiles<32, 64, 1, 2, 4, 2, false>(p, s);
+    default: return shift ? launch_tiles<32, 32, 1, 1, 8, 1, true>(p, s) : launch_tiles<32, 32, 1, 1, 8, 1, false>(p, s);
   }
 }
 
@@ -148,13 +514,16 @@ extern "C" int mm_int8_matmul(const int8_t* a, int64_t lda, const int8_t* b, int
                "mm_int8_matmul: bad sizes (%lld x %lld x %lld; K at most %d)", static_cast<long long>(m),
                static_cast<long long>(n), static_cast<long long>(k), kMaxK);
   MM_CHECK_ARG(is_float_type(out_type) && (!bias || is_float_type(bias_type)), "mm_int8_matmul: bad types");
-  MM_CHECK_ARG((m <= 1 || lda >= k) && (n <= 1 || ldb >= k) && (m <= 1 || ldo >= n), "mm_int8_matmul: bad strides");
-  const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128);
-  MM_CHECK_ARG(tiles < (int64_t(1) << 24), "mm_int8_matmul: too many tiles");  // 2^32 threads in a launch
+  MM_CHECK_ARG((m <= 1 || (lda >= k && lda <= kMaxStride)) && (n <= 1 || (ldb >= k && ldb <= kMaxStride)) &&
+                   (m <= 1 || ldo >= n),
+               "mm_int8_matmul: bad strides (rows of a and b at least K and at most %lld apart)",
+               static_cast<long long>(kMaxStride));
   if (m == 0) return MM_OK;
   MM_CHECK_ARG(a && b && a_scale && b_scale && out, "mm_int8_matmul: null pointer");
+  // a single row's stride is never stepped over
+  if (m == 1) lda = k;
+  if (n == 1) ldb = k;
   const I8Args p{a, b, a_scale, b_scale, bias, out, lda, ldb, ldo, static_cast<int32_t>(m), static_cast<int32_t>(n),
                  static_cast<int32_t>(k), out_type, bias_type};
-  int8_tile_kernel<<<static_cast<uint32_t>(tiles), 256, 0, mm_hip_stream(stream)>>>(p);
-  return mm_check_launch("int8_tile_kernel");
+  return launch_best(p, mm_hip_stream(stream));
 }

@@ -328,15 +328,29 @@ def layer_backward(dy, x, w1, w2, tokens: int, top_k: int, offsets, send_token, 
     return grad_act, dab, dscale, grad_fc2, dx, gh, grw, ggu
 
 
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the handle without the Stream object around it, where this torch has it (2 us less a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
 def _launch(device: torch.device, name: str, *args):
     """Call an entry point on torch's current stream of ``device``, which need
     not be the current device (kernels launch on the current one)."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
+    index = device.index
+    stream = _raw_stream(index)
+    if index == torch.cuda.current_device():
         _lib.call(name, *args, stream)
     else:
         with torch.cuda.device(device):
             _lib.call(name, *args, stream)
+
+
+def _empty(like: torch.Tensor, dtype=None) -> torch.Tensor:
+    """A contiguous tensor of ``like``'s shape and device."""
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def _rows(name: str, t: torch.Tensor):
@@ -368,8 +382,8 @@ def rms_norm(x, weight, residual, eps: float, out_dtype, keep_rstd: bool = False
     if residual is not None:
         rp, ldr, _ = _rows("residual", residual)
         ht = _TYPES[residual.dtype]
-        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
-    y = torch.empty(x.shape, dtype=out_dtype, device=dev)
+        h = _empty(residual)
+    y = _empty(x, out_dtype)
     scale = None if out_dtype == x.dtype else torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     rstd = torch.empty(rows, dtype=torch.float32, device=dev) if keep_rstd else None
     if rows:
@@ -383,23 +397,16 @@ def rms_norm(x, weight, residual, eps: float, out_dtype, keep_rstd: bool = False
 def rms_norm_bwd(dy, dh, h, weight, rstd, x_dtype, want_residual: bool, want_weight: bool):
     """(dx, dresidual | None, dweight | None); dresidual is dx itself where the types agree."""
     dev, hidden = h.device, h.shape[-1]
-
-    def rows_of(name, t):
-        try:
-            return t, _rows(name, t)
-        except ValueError:  # a gradient comes in any layout (an expanded scalar, a transposed view)
-            t = t.contiguous()
-            return t, _rows(name, t)
-
-    dy, (dyp, lddy, _) = rows_of("dy", dy)
-    dhp = lddh = 0
+    dy = dy.contiguous()  # a gradient comes in any layout (an expanded scalar, a transposed view)
+    dhp = 0
     if dh is not None:
-        dh, (dhp, lddh, _) = rows_of("dh", dh)
+        dh = dh.contiguous()
+        dhp = dh.data_ptr()
     hp, ldh, rows = _rows("h", h)
-    dx = torch.empty(h.shape, dtype=x_dtype, device=dev)
+    dx = _empty(h, x_dtype)
     dres = None
     if want_residual:
-        dres = dx if h.dtype == x_dtype else torch.empty(h.shape, dtype=h.dtype, device=dev)
+        dres = dx if h.dtype == x_dtype else _empty(h)
     dw = ws = None
     nbytes = 0
     if want_weight:
@@ -407,7 +414,7 @@ def rms_norm_bwd(dy, dh, h, weight, rstd, x_dtype, want_residual: bool, want_wei
         nbytes = _lib.load().mm_rms_norm_bwd_workspace_bytes(rows, hidden)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     if rows or want_weight:
-        _launch(dev, "mm_rms_norm_bwd", dyp, lddy, dhp, lddh, hp, ldh, None if weight is None else weight.data_ptr(),
+        _launch(dev, "mm_rms_norm_bwd", dy.data_ptr(), hidden, dhp, hidden, hp, ldh, None if weight is None else weight.data_ptr(),
                 0 if weight is None else _TYPES[weight.dtype], rstd.data_ptr(), _TYPES[x_dtype], _TYPES[h.dtype], rows,
                 hidden, dx.data_ptr(), None if dres is None or dres is dx else dres.data_ptr(),
                 None if dw is None else dw.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
@@ -417,7 +424,7 @@ def rms_norm_bwd(dy, dh, h, weight, rstd, x_dtype, want_residual: bool, want_wei
 def quantize_rows(x, dtype):
     """(q, scale) of the rows of ``x``."""
     xp, ldx, rows = _rows("x", x)
-    q = torch.empty(x.shape, dtype=dtype, device=x.device)
+    q = _empty(x, dtype)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     if rows:
         _launch(x.device, "mm_quantize_rows", xp, ldx, _TYPES[x.dtype], rows, x.shape[-1], q.data_ptr(), _TYPES[dtype],
@@ -431,8 +438,8 @@ def int8_matmul(a, b, a_scale, b_scale, bias, out_dtype):
     n, k = b.shape
     out = torch.empty(*a.shape[:-1], n, dtype=out_dtype, device=a.device)
     if m:
-        if m > 1 and lda < k:
-            raise ValueError("the rows of a must not overlap")
+        if m > 1 and not k <= lda <= 1 << 23:
+            raise ValueError(f"the rows of a must be {k} to {1 << 23} elements apart (no overlap), got {lda}")
         _launch(a.device, "mm_int8_matmul", ap, lda, b.data_ptr(), b.stride(0), a_scale.data_ptr(), b_scale.data_ptr(),
                 None if bias is None else bias.data_ptr(), 0 if bias is None else _TYPES[bias.dtype], m, n, k,
                 out.data_ptr(), n, _TYPES[out_dtype])

@@ -16,6 +16,7 @@ import torch
 from . import _kernels as K
 from .norm import MAX_HIDDEN, quantize_rows
 
+MAX_STRIDE = 1 << 23  # of a row, 256 of which a kernel's offsets have to span
 MAX_K = (1 << 17) - 1  # the int32 sum is exact below 2^17 products of two int8 values
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -26,7 +27,7 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
 
     ``a`` int8 [..., K] (rows evenly spaced in memory, unit column stride) with
     fp32 ``a_scale`` of ``a``'s leading shape, one a token; ``b`` int8 [N, K]
-    (unit column stride, any row stride) with fp32 ``b_scale`` [N], one a
+    (unit column stride, rows up to 2^23 elements apart, as ``a``'s) with fp32 ``b_scale`` [N], one a
     channel; ``bias`` [N] in bf16, fp16 or fp32. 1 <= K < 2^17: the sum is exact
     in int32; scales and bias are applied in fp32 and the result is rounded
     once to bf16, fp16 or fp32. No gradient.
@@ -44,8 +45,8 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
         raise ValueError(f"b must have shape [N, K] with N >= 1 and 1 <= K <= {MAX_K}, got {tuple(b.shape)}")
     if k > 1 and b.stride(1) != 1:
         raise ValueError("b must have unit column stride ([N, K], K contiguous)")
-    if n > 1 and b.stride(0) < k:
-        raise ValueError("the rows of b must not overlap")
+    if n > 1 and not k <= b.stride(0) <= MAX_STRIDE:
+        raise ValueError(f"the rows of b must be {k} to {MAX_STRIDE} elements apart (no overlap), got {b.stride(0)}")
     for name, t, shape in (("a_scale", a_scale, a.shape[:-1]), ("b_scale", b_scale, (n,))):
         if t.dtype != torch.float32:
             raise TypeError(f"{name} must be torch.float32, got {t.dtype}")

@@ -46,16 +46,23 @@ class _RMSNorm(torch.autograd.Function):
         return y if residual is None else (y, h)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
-        if dy is None and dh is None:
-            return None, None, None, None
-        if dy is None:
-            dy = torch.zeros(h.shape, dtype=ctx.x_dtype, device=h.device)
-        dx, dres, dw = K.rms_norm_bwd(dy, dh, h, weight, rstd, ctx.x_dtype, ctx.has_residual and ctx.needs_input_grad[2],
-                                      weight is not None and ctx.needs_input_grad[1])
-        return dx, dw, dres, None
+        # grad mode is on here only under create_graph, whose second backward must raise
+        return _rms_norm_grads_once(ctx, dy, dh) if torch.is_grad_enabled() else _rms_norm_grads(ctx, dy, dh)
+
+
+def _rms_norm_grads(ctx, dy, dh):
+    h, weight, rstd = ctx.saved_tensors
+    if dy is None and dh is None:
+        return None, None, None, None
+    if dy is None:
+        dy = torch.zeros(h.shape, dtype=ctx.x_dtype, device=h.device)
+    dx, dres, dw = K.rms_norm_bwd(dy, dh, h, weight, rstd, ctx.x_dtype, ctx.has_residual and ctx.needs_input_grad[2],
+                                  weight is not None and ctx.needs_input_grad[1])
+    return dx, dw, dres, None
+
+
+_rms_norm_grads_once = torch.autograd.function.once_differentiable(_rms_norm_grads)
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
