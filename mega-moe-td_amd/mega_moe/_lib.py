@@ -116,10 +116,9 @@ class MegaMoEError(RuntimeError):
 
 def call(name: str, *args):
     """Call a status-returning entry point and raise on a non-zero status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    rc = getattr(_lib or load(), name)(*args)
     if rc != 0:
-        msg = lib.mm_last_error().decode(errors="replace")
+        msg = load().mm_last_error().decode(errors="replace")
         raise MegaMoEError(f"{name} failed ({rc}): {msg}")
 
 

@@ -334,18 +334,18 @@ def _raw_stream(index: int) -> int:
 
 # the handle without the Stream object around it, where this torch has it (2 us less a call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _launch(device: torch.device, name: str, *args):
     """Call an entry point on torch's current stream of ``device``, which need
     not be the current device (kernels launch on the current one)."""
     index = device.index
-    stream = _raw_stream(index)
-    if index == torch.cuda.current_device():
-        _lib.call(name, *args, stream)
+    if index == _current_device():
+        _lib.call(name, *args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, stream)
+            _lib.call(name, *args, _raw_stream(index))
 
 
 def _empty(like: torch.Tensor, dtype=None) -> torch.Tensor:
@@ -355,11 +355,14 @@ def _empty(like: torch.Tensor, dtype=None) -> torch.Tensor:
 
 def _rows(name: str, t: torch.Tensor):
     """(address, row stride, rows) of ``t`` [..., columns] as evenly spaced rows."""
+    if t.dim() == 2:
+        rows, columns = t.shape
+        ld, step = t.stride()
+        if step == 1 or columns <= 1:
+            return t.data_ptr(), ld, rows
     columns = t.shape[-1]
     if columns > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have unit column stride")
-    if t.dim() == 2:
-        return t.data_ptr(), t.stride(0), t.shape[0]
     if t.dim() == 1:
         return t.data_ptr(), columns, 1
     try:
@@ -436,14 +439,14 @@ def int8_matmul(a, b, a_scale, b_scale, bias, out_dtype):
     """[..., N] product of operands ``ops.int8`` has checked."""
     ap, lda, m = _rows("a", a)
     n, k = b.shape
-    out = torch.empty(*a.shape[:-1], n, dtype=out_dtype, device=a.device)
+    out = torch.empty(m, n, dtype=out_dtype, device=a.device)
     if m:
         if m > 1 and not k <= lda <= 1 << 23:
             raise ValueError(f"the rows of a must be {k} to {1 << 23} elements apart (no overlap), got {lda}")
         _launch(a.device, "mm_int8_matmul", ap, lda, b.data_ptr(), b.stride(0), a_scale.data_ptr(), b_scale.data_ptr(),
                 None if bias is None else bias.data_ptr(), 0 if bias is None else _TYPES[bias.dtype], m, n, k,
                 out.data_ptr(), n, _TYPES[out_dtype])
-    return out
+    return out if a.dim() == 2 else out.view(*a.shape[:-1], n)
 
 
 def few_forward(x, selected, routing_weights, w1, w2, num_experts: int, activation: str, situ_beta: float,

@@ -27,7 +27,7 @@ def _check_float(name: str, t: torch.Tensor):
 
 
 def _check_device(name: str, t: torch.Tensor):
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be a HIP device tensor")
 
 
@@ -86,6 +86,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
     is floating; 8-bit outputs carry no gradient and refuse inputs that ask for
     one.
     """
+    dtype = x.dtype
     _check_float("x", x)
     if x.dim() == 0:
         raise ValueError("x must have shape [..., hidden]")
@@ -93,14 +94,13 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
     _check_columns("x", hidden)
     if weight is not None:
         _check_float("weight", weight)
-        if tuple(weight.shape) != (hidden,) or not weight.is_contiguous():
+        if weight.dim() != 1 or weight.shape[0] != hidden or not weight.is_contiguous():
             raise ValueError(f"weight must be contiguous with shape ({hidden},), got {tuple(weight.shape)}")
         if weight.device != x.device:
             raise ValueError("weight and x must be on the same device")
     if residual is not None:
-        _check_float("residual", residual)
-        if residual.dtype != x.dtype and residual.dtype != torch.float32:
-            raise TypeError(f"residual must use {x.dtype} or torch.float32, got {residual.dtype}")
+        if residual.dtype != dtype and residual.dtype != torch.float32:
+            raise TypeError(f"residual must use {dtype} or torch.float32, got {residual.dtype}")
         if residual.shape != x.shape:
             raise ValueError(f"residual must have shape {tuple(x.shape)}, got {tuple(residual.shape)}")
         if residual.device != x.device:
@@ -108,16 +108,17 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
     if out_dtype is None:
-        out_dtype = x.dtype
-    elif out_dtype != x.dtype and out_dtype not in _EIGHT_BITS:
-        raise TypeError(f"out_dtype must be {x.dtype}, torch.int8 or torch.float8_e4m3fn, got {out_dtype}")
-    needs_grad = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                              or (residual is not None and residual.requires_grad))
-    if out_dtype in _EIGHT_BITS:
+        out_dtype = dtype
+    elif out_dtype != dtype and out_dtype not in _EIGHT_BITS:
+        raise TypeError(f"out_dtype must be {dtype}, torch.int8 or torch.float8_e4m3fn, got {out_dtype}")
+    needs_grad = (x.requires_grad or (weight is not None and weight.requires_grad)
+                  or (residual is not None and residual.requires_grad)) and torch.is_grad_enabled()
+    eight_bits = out_dtype != dtype
+    if eight_bits:
         if needs_grad:
             raise ValueError("an 8-bit output carries no gradient; call under torch.no_grad() or on detached inputs")
     _check_device("x", x)
-    if out_dtype in _EIGHT_BITS:
+    if eight_bits:
         q, scale, h, _ = K.rms_norm(x, weight, residual, eps, out_dtype)
         return (q, scale) if residual is None else (q, scale, h)
     if needs_grad:

@@ -54,6 +54,14 @@ def test_product(m, n, k, dtype, bias):
     _check(mega_moe.int8_matmul(a, b, sa, sb, bias=bias, out_dtype=dtype), a, b, sa, sb, bias, dtype)
 
 
+@pytest.mark.parametrize("m,n,k", [  # tiles of 256, 128, 64 and 32 rows, K whole and cut, rows on odd addresses
+    (4096, 4096, 640), (4090, 4090, 3001), (2048, 3000, 517), (1500, 2000, 300), (700, 5000, 2050), (128, 4096, 4099),
+    (128, 4096, 2048), (200, 2000, 260), (40, 4000, 4101), (48, 4096, 2048)])
+def test_every_tile(m, n, k):
+    a, b, sa, sb = _operands(m, n, k, seed=7)
+    _check(mega_moe.int8_matmul(a, b, sa, sb), a, b, sa, sb, None, BF)
+
+
 @pytest.mark.parametrize("m", [1, 5, 40, 130, 300])
 @pytest.mark.parametrize("k", [1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 257, 1023, 1025])
 def test_ends_of_the_sum(m, k):
