@@ -46,6 +46,7 @@ struct FewArgs {
   float* y;                   // [R, H]
   int32_t* done;              // [fc2_tiles + 1]: arrivals at each tile, then the distinct experts
   bf16* out;                  // [T, H]
+  int32_t slots;              // experts or routes, each with all column tiles
   int32_t tiles, fc2_tiles;   // column tiles of this launch, and of the second
 };
 
@@ -53,10 +54,10 @@ struct FewArgs {
 // at about the same time: narrow ones share lines, and an expert's rows are
 // read in runs of a kilobyte.
 constexpr int kNear = 8;
-__device__ __forceinline__ int near_block() {
+__device__ __forceinline__ int near_block(int blocks) {
   constexpr int G = 8 * kNear;
   const int b = blockIdx.x, base = b / G * G;
-  if (base + G > static_cast<int>(gridDim.x)) return b;
+  if (base + G > blocks) return b;
   return base + (b & 7) * kNear + (b - base) / 8;
 }
 
@@ -69,7 +70,7 @@ __device__ __forceinline__ int near_block() {
 struct Work {
   int slot, tile, expert, count;
   __device__ __forceinline__ Work(const FewArgs& p, uint16_t* list, uint64_t* valid) {
-    const int block = near_block(), lane = threadIdx.x & 63;
+    const int block = near_block(p.slots * p.tiles), lane = threadIdx.x & 63;
     slot = block / p.tiles;
     tile = block % p.tiles;
     count = 0;
@@ -119,7 +120,6 @@ __device__ void prepare_done(const FewArgs& p, uint32_t* bits) {
     for (int m = 32; m > 0; m >>= 1) n += __shfl_xor(n, m);
     if (threadIdx.x == 0) p.done[p.fc2_tiles] = n;
   }
-  __syncthreads();
 }
 
 // ------------------------------------------------------------------ products
@@ -162,15 +162,27 @@ struct ColumnStep {
 };
 
 // Weights with the sum's axis contiguous: 16 bytes a lane are an operand as
-// they are, 16 weight rows and 64 bytes of the sum's axis an instruction. The
-// other half of each line is the next wave's or step's, so no non-temporal hint
-// here (int8, 3072 x 2048 of 112 experts: 141 us against 173). w[g]: group g.
+// they are, 16 weight rows and 64 bytes of the sum's axis an instruction. A
+// piece is 128 bytes, so that a wave asks for both halves of a line, one after
+// the other (41 experts of 4096 x 7168 in int8: 205 us, in pieces of 64 bytes
+// 236), without the non-temporal hint, which drops the second half (244).
+// w[g][h]: half h of group g.
 template <int G>
-struct RowWeights {
-  i32x4 w[G];
+struct RowStep {
+  i32x4 w[G][2];
   __device__ __forceinline__ void load(const char* wp, int64_t group_bytes, uint32_t w_off) {
 #pragma unroll
-    for (int g = 0; g < G; ++g) __builtin_memcpy(&w[g], wp + g * group_bytes + w_off, 16);
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) __builtin_memcpy(&w[g][h], wp + g * group_bytes + h * 64 + w_off, 16);
+  }
+};
+// The tokens' two operands of a piece.
+struct TokenStep {
+  i32x4 x[2];
+  __device__ __forceinline__ void load(const char* xp, uint32_t x_off) {
+    __builtin_memcpy(&x[0], xp + x_off, 16);
+    __builtin_memcpy(&x[1], xp + 64 + x_off, 16);
   }
 };
 
@@ -219,7 +231,10 @@ __global__ __launch_bounds__(W * 64) void few_fc1_kernel(FewArgs p) {
   const Waves<W> ws;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
   uint16_t* list = list_of(p);
-  if (blockIdx.x == 0) prepare_done<W * 64>(p, reinterpret_cast<uint32_t*>(red));
+  if (static_cast<int>(blockIdx.x) == p.slots * p.tiles) {  // the workgroup behind the tiles
+    prepare_done<W * 64>(p, reinterpret_cast<uint32_t*>(red));
+    return;
+  }
   const Work wk(p, list, route_lds);
   if (!wk.count) return;
   const int64_t row_bytes = 4 * static_cast<int64_t>(p.I);
@@ -355,16 +370,21 @@ __global__ __launch_bounds__(W * 64) void few_fc2_kernel(FewArgs p) {
     const uint32_t x_off = (static_cast<uint32_t>(route) * p.I + 8 * q) * 2;
     f32x4 acc[N];
     clear(acc);
-    for (int s = ws.wave; s < p.I / 32; s += W) {
-      if constexpr (ROWS) {
-        RowWeights<N> st;
-        bf16x8 xv;
-        st.load(w + s * 64, 16 * row_bytes, w_off);
-        __builtin_memcpy(&xv, x + s * 64 + x_off, 16);
+    if constexpr (ROWS) {
+      for (int s = ws.wave; s < p.I / 64; s += W) {
+        RowStep<N> st;
+        TokenStep tok;
+        st.load(w + s * 128, 16 * row_bytes, w_off);
+        tok.load(x + s * 128, x_off);
 #pragma unroll
-        for (int g = 0; g < N; ++g)
-          acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, st.w[g]), xv, acc[g], 0, 0, 0);
-      } else {
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int g = 0; g < N; ++g)
+            acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, st.w[g][h]),
+                                                             __builtin_bit_cast(bf16x8, tok.x[h]), acc[g], 0, 0, 0);
+      }
+    } else {
+      for (int s = ws.wave; s < p.I / 32; s += W) {
         ColumnStep<N, true> st;
         st.load(w + s * 32 * row_bytes, w_off, row_bytes, x + s * 64, x_off);
         st.multiply(acc);
@@ -393,7 +413,10 @@ __global__ __launch_bounds__(W * 64) void few_fc1_int8_kernel(FewArgs p) {
   const Waves<W> ws;
   const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
   uint16_t* list = list_of(p);
-  if (blockIdx.x == 0) prepare_done<W * 64>(p, reinterpret_cast<uint32_t*>(red));
+  if (static_cast<int>(blockIdx.x) == p.slots * p.tiles) {  // the workgroup behind the tiles
+    prepare_done<W * 64>(p, reinterpret_cast<uint32_t*>(red));
+    return;
+  }
   const Work wk(p, list, route_lds);
   if (!wk.count) return;
   const int col = wk.tile * C;
@@ -406,17 +429,19 @@ __global__ __launch_bounds__(W * 64) void few_fc1_int8_kernel(FewArgs p) {
     const uint32_t x_off = static_cast<uint32_t>(token) * p.H + 16 * q;
     i32x4 acc[2 * G];
     clear(acc);
-    for (int s = ws.wave; s < p.H / 64; s += W) {
-      RowWeights<G> gate, up;
-      i32x4 xv;
-      gate.load(w + s * 64, 16 * p.H, w_off);
-      up.load(w + up_bytes + s * 64, 16 * p.H, w_off);
-      __builtin_memcpy(&xv, static_cast<const char*>(p.x) + s * 64 + x_off, 16);
+    for (int s = ws.wave; s < p.H / 128; s += W) {
+      RowStep<G> gate, up;
+      TokenStep tok;
+      gate.load(w + s * 128, 16 * p.H, w_off);
+      up.load(w + up_bytes + s * 128, 16 * p.H, w_off);
+      tok.load(static_cast<const char*>(p.x) + s * 128, x_off);
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(gate.w[g], xv, acc[g], 0, 0, 0);
-        acc[G + g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(up.w[g], xv, acc[G + g], 0, 0, 0);
-      }
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(gate.w[g][h], tok.x[h], acc[g], 0, 0, 0);
+          acc[G + g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(up.w[g][h], tok.x[h], acc[G + g], 0, 0, 0);
+        }
     }
     if (c0) __syncthreads();  // the 16 tokens before have been joined
     ws.leave(red, acc);
@@ -476,21 +501,25 @@ __global__ __launch_bounds__(W * 64) void few_fc2_int8_kernel(FewArgs p) {
     const uint32_t sc_off = static_cast<uint32_t>(route) * (p.I / kGroup) * 4;
     f32x4 acc[G];
     clear(acc);
-    for (int s = ws.wave; s < p.I / 64; s += W) {
-      RowWeights<G> st;
-      i32x4 xv;
-      float sv[2];
-      st.load(w + s * 64, 16 * p.I, w_off);
-      __builtin_memcpy(&xv, static_cast<const char*>(p.act) + s * 64 + x_off, 16);
-      __builtin_memcpy(sv, reinterpret_cast<const char*>(p.act_scale) + s * (64 / kGroup * 4) + sc_off, 8);
+    for (int s = ws.wave; s < p.I / 128; s += W) {
+      RowStep<G> st;
+      TokenStep tok;
+      float sv[4];
+      st.load(w + s * 128, 16 * p.I, w_off);
+      tok.load(static_cast<const char*>(p.act) + s * 128, x_off);
+      __builtin_memcpy(sv, reinterpret_cast<const char*>(p.act_scale) + s * (128 / kGroup * 4) + sc_off, 16);
       const i32x4 zero = {0, 0, 0, 0};
-      const i32x4 lo = lane < 32 ? xv : zero, hi = lane < 32 ? zero : xv;
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const i32x4 a = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.w[g], lo, zero, 0, 0, 0);
-        const i32x4 b = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.w[g], hi, zero, 0, 0, 0);
+      for (int h = 0; h < 2; ++h) {
+        const i32x4 lo = lane < 32 ? tok.x[h] : zero, hi = lane < 32 ? zero : tok.x[h];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[g][r] += static_cast<float>(a[r]) * sv[0] + static_cast<float>(b[r]) * sv[1];
+        for (int g = 0; g < G; ++g) {
+          const i32x4 a = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.w[g][h], lo, zero, 0, 0, 0);
+          const i32x4 b = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.w[g][h], hi, zero, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            acc[g][r] += static_cast<float>(a[r]) * sv[2 * h] + static_cast<float>(b[r]) * sv[2 * h + 1];
+        }
       }
     }
     if (c0) __syncthreads();  // the 16 tokens before have been joined
@@ -545,9 +574,10 @@ int launch_both(FewArgs p, const Launch& a, const Launch& b, hipStream_t s) {
   MM_CHECK_ARG(static_cast<int64_t>(slots) * (tiles1 > tiles2 ? tiles1 : tiles2) < (int64_t(1) << 23),
                "mm_moe_few: too many tiles");
   const size_t lds = route_lds_bytes(p.R);
+  p.slots = slots;
   p.fc2_tiles = tiles2;
   p.tiles = tiles1;
-  a.kernel<<<slots * tiles1, a.waves * 64, lds, s>>>(p);
+  a.kernel<<<slots * tiles1 + 1, a.waves * 64, lds, s>>>(p);
   const int rc = mm_check_launch("few_fc1_kernel");
   if (rc) return rc;
   p.tiles = tiles2;
@@ -585,7 +615,7 @@ extern "C" int mm_moe_few(const uint16_t* x, const int32_t* selected, const floa
             static_cast<int32_t>(tokens * top_k), top_k, num_experts, hidden, inter, static_cast<int32_t>(tokens),
             act_kind, situ_beta, situ_linear_beta, clamp_limit, base + f.act, nullptr,
             reinterpret_cast<float*>(base + f.y), reinterpret_cast<int32_t*>(base + f.done),
-            reinterpret_cast<bf16*>(out), 0, 0};
+            reinterpret_cast<bf16*>(out), 0, 0, 0};
   const hipStream_t s = mm_hip_stream(stream);
   // 64 columns a tile read whole lines; with fewer workgroups than two to a CU
   // 32 columns, twice as many, win (8 experts of 1024 columns: 25 us against 40;
@@ -616,7 +646,7 @@ extern "C" int mm_moe_few_int8(const int8_t* x, const float* x_scale, const int3
             static_cast<int32_t>(tokens * top_k), top_k, num_experts, hidden, inter, static_cast<int32_t>(tokens),
             act_kind, situ_beta, situ_linear_beta, clamp_limit, base + f.act,
             reinterpret_cast<float*>(base + f.act_scale), reinterpret_cast<float*>(base + f.y),
-            reinterpret_cast<int32_t*>(base + f.done), reinterpret_cast<bf16*>(out), 0, 0};
+            reinterpret_cast<int32_t*>(base + f.done), reinterpret_cast<bf16*>(out), 0, 0, 0};
   const hipStream_t s = mm_hip_stream(stream);
   return launch_both(p, {few_fc1_int8_kernel<4>, 4, kGroup}, {few_fc2_int8_kernel<4>, 4, 64}, s);
 }
