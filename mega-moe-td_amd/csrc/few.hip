@@ -9,11 +9,13 @@
 // itself, and reads its weights once, straight into matrix-instruction
 // operands. Weights are the instruction's rows and tokens its 16 columns, so 1
 // to 16 rows of an expert cost the same and absent ones need no masking: a
-// result column depends on its own token only. An expert of more rows takes
-// them 16 at a time, its weights from L2 from the second time on. The waves of
+// result column depends on its own token only. A pass takes 16, 32 or 64 rows of
+// an expert; the weights of a further pass come from L2. The waves of
 // a workgroup share the sum's axis and join through LDS in wave order. The
 // second launch leaves fp32 rows in scratch; the workgroup that finishes a
 // tile of columns last adds the tokens' slots in slot order. Every sum has a fixed order.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -21,7 +23,6 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTokens = 16;       // columns of the matrix instructions
 constexpr int kGroup = MM_FEW_ACT_GROUP;
 constexpr float kScaleFloor = 1e-30f;
 // 32-bit byte offsets of a lane: 24 rows of w1 (4 I bytes each), 64 tokens of x
@@ -136,27 +137,32 @@ __device__ void prepare_done(const FewArgs& p, uint32_t* bits) {
 // whole carry the non-temporal hint (7168 x 4096, 64-column tiles: 373 us
 // against 411 for 41 experts); halves of lines do not, as the hint drops the
 // half that the neighbour comes for (640 against 503).
-template <int CL, bool STREAM>
+template <int CL, int NT, bool STREAM>
 struct ColumnStep {
   typedef uint32_t Raw __attribute__((ext_vector_type(CL / 2)));
   Raw w[8];
-  bf16x8 x;
-  __device__ __forceinline__ void load(const char* wp, uint32_t w_off, int64_t row_bytes, const char* xp, uint32_t x_off) {
+  bf16x8 x[NT];
+  __device__ __forceinline__ void load(const char* wp, uint32_t w_off, int64_t row_bytes, const char* xp,
+                                       const uint32_t (&x_off)[NT]) {
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const Raw* p = reinterpret_cast<const Raw*>(wp + r * row_bytes + w_off);
       w[r] = STREAM ? __builtin_nontemporal_load(p) : *p;
     }
-    __builtin_memcpy(&x, xp + x_off, 16);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) __builtin_memcpy(&x[n], xp + x_off[n], 16);
   }
-  __device__ __forceinline__ void multiply(f32x4 (&acc)[CL]) const {
+  __device__ __forceinline__ void multiply(f32x4 (&acc)[CL * NT]) const {
 #pragma unroll
     for (int c = 0; c < CL; ++c) {
       const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;
       u32x4 v;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_perm(w[2 * i + 1][c >> 1], w[2 * i][c >> 1], sel);
-      acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), x, acc[c], 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        acc[c * NT + n] =
+            __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), x[n], acc[c * NT + n], 0, 0, 0);
     }
   }
 };
@@ -178,13 +184,23 @@ struct RowStep {
   }
 };
 // The tokens' two operands of a piece.
+template <int NT>
 struct TokenStep {
-  i32x4 x[2];
-  __device__ __forceinline__ void load(const char* xp, uint32_t x_off) {
-    __builtin_memcpy(&x[0], xp + x_off, 16);
-    __builtin_memcpy(&x[1], xp + 64 + x_off, 16);
+  i32x4 x[NT][2];
+  __device__ __forceinline__ void load(const char* xp, const uint32_t (&x_off)[NT]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) __builtin_memcpy(&x[n][h], xp + h * 64 + x_off[n], 16);
   }
 };
+
+// The routes of the lane's columns: NT blocks of 16, the last route repeated.
+template <int NT>
+__device__ __forceinline__ void routes_of(const uint16_t* list, int c0, int count, int (&route)[NT]) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n) route[n] = list[min(c0 + n * 16 + static_cast<int>(threadIdx.x & 15), count - 1)];
+}
 
 template <int N, class V>
 __device__ __forceinline__ void clear(V (&acc)[N]) {
@@ -223,11 +239,11 @@ size_t route_lds_bytes(int R) { return static_cast<size_t>((R + 63) / 64) * 8 + 
 
 // ------------------------------------------------------------------ first launch, bf16
 // Tile of C = 8 * CL columns: operand rows 0..7 are gate, 8..15 up columns.
-template <int CL, int W>
+template <int CL, int W, int NT>
 __global__ __launch_bounds__(W * 64) void few_fc1_kernel(FewArgs p) {
   constexpr int C = 8 * CL;
-  __shared__ f32x4 red[W * CL * 64];
-  __shared__ __attribute__((aligned(16))) bf16 stage[kTokens][C + 8];
+  __shared__ f32x4 red[W * CL * NT * 64];
+  __shared__ __attribute__((aligned(16))) bf16 stage[NT * 16][C + 8];
   const Waves<W> ws;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
   uint16_t* list = list_of(p);
@@ -240,31 +256,40 @@ __global__ __launch_bounds__(W * 64) void few_fc1_kernel(FewArgs p) {
   const int64_t row_bytes = 4 * static_cast<int64_t>(p.I);
   const char* w = static_cast<const char*>(p.w1) + static_cast<int64_t>(wk.expert) * p.H * row_bytes + wk.tile * C * 2;
   const uint32_t w_off = static_cast<uint32_t>(8 * q * row_bytes) + (j < 8 ? 0 : 2 * p.I) + CL * 2 * (j & 7);
-  for (int c0 = 0; c0 < wk.count; c0 += kTokens) {
-    const int route = list[min(c0 + j, wk.count - 1)];
-    const uint32_t x_off = (static_cast<uint32_t>(route / p.top_k) * p.H + 8 * q) * 2;
-    const float wt = p.w[route];
-    f32x4 acc[CL];
+  for (int c0 = 0; c0 < wk.count; c0 += NT * 16) {
+    int route[NT];
+    uint32_t x_off[NT];
+    float wt[NT];
+    routes_of<NT>(list, c0, wk.count, route);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      x_off[n] = (static_cast<uint32_t>(route[n] / p.top_k) * p.H + 8 * q) * 2;
+      wt[n] = p.w[route[n]];
+    }
+    f32x4 acc[CL * NT];
     clear(acc);
     for (int s = ws.wave; s < p.H / 32; s += W) {
-      ColumnStep<CL, C * 2 >= 128> st;
+      ColumnStep<CL, NT, C * 2 >= 128> st;
       st.load(w + s * 32 * row_bytes, w_off, row_bytes, static_cast<const char*>(p.x) + s * 64, x_off);
       st.multiply(acc);
     }
     ws.leave(red, acc);
     __syncthreads();
     for (int c = ws.wave; c < CL; c += W) {
-      const f32x4 v = ws.template join<CL>(red, c);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float up = __shfl(v[r], (lane + 32) & 63);
-        if (lane < 32)
-          stage[j][CL * (4 * q + r) + c] =
-              static_cast<bf16>(gated_act(p.act_kind, v[r], up, p.beta, p.lbeta, p.limit) * wt);
+      for (int n = 0; n < NT; ++n) {
+        const f32x4 v = ws.template join<CL * NT>(red, c * NT + n);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float up = __shfl(v[r], (lane + 32) & 63);
+          if (lane < 32)
+            stage[n * 16 + j][CL * (4 * q + r) + c] =
+                static_cast<bf16>(gated_act(p.act_kind, v[r], up, p.beta, p.lbeta, p.limit) * wt[n]);
+        }
       }
     }
     __syncthreads();
-    for (int item = tid; item < kTokens * (C / 8); item += W * 64) {
+    for (int item = tid; item < NT * 16 * (C / 8); item += W * 64) {
       const int row = item / (C / 8), vec = item % (C / 8);
       if (c0 + row < wk.count)
         *reinterpret_cast<uint4*>(static_cast<bf16*>(p.act) + static_cast<int64_t>(list[c0 + row]) * p.I + wk.tile * C +
@@ -347,10 +372,10 @@ __device__ __forceinline__ void finish_empty(const FewArgs& p, const Work& wk) {
 
 // ROWS: w2's sum axis is contiguous (N groups of 16 columns), else its columns
 // are (N = CL columns a lane).
-template <bool ROWS, int N, int W>
+template <bool ROWS, int N, int W, int NT>
 __global__ __launch_bounds__(W * 64) void few_fc2_kernel(FewArgs p) {
   constexpr int C = 16 * N;
-  __shared__ f32x4 red[W * N * 64];
+  __shared__ f32x4 red[W * N * NT * 64];
   const Waves<W> ws;
   const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
   uint16_t* list = list_of(p);
@@ -365,38 +390,45 @@ __global__ __launch_bounds__(W * 64) void few_fc2_kernel(FewArgs p) {
   const uint32_t w_off = ROWS ? static_cast<uint32_t>(j * row_bytes) + 16 * q
                               : static_cast<uint32_t>(8 * q * row_bytes) + N * 2 * j;
   const char* x = static_cast<const char*>(p.act);
-  for (int c0 = 0; c0 < wk.count; c0 += kTokens) {
-    const int64_t route = list[min(c0 + j, wk.count - 1)];
-    const uint32_t x_off = (static_cast<uint32_t>(route) * p.I + 8 * q) * 2;
-    f32x4 acc[N];
+  for (int c0 = 0; c0 < wk.count; c0 += NT * 16) {
+    int route[NT];
+    uint32_t x_off[NT];
+    routes_of<NT>(list, c0, wk.count, route);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x_off[n] = (static_cast<uint32_t>(route[n]) * p.I + 8 * q) * 2;
+    f32x4 acc[N * NT];
     clear(acc);
     if constexpr (ROWS) {
       for (int s = ws.wave; s < p.I / 64; s += W) {
         RowStep<N> st;
-        TokenStep tok;
+        TokenStep<NT> tok;
         st.load(w + s * 128, 16 * row_bytes, w_off);
         tok.load(x + s * 128, x_off);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int g = 0; g < N; ++g)
-            acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, st.w[g][h]),
-                                                             __builtin_bit_cast(bf16x8, tok.x[h]), acc[g], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              acc[g * NT + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, st.w[g][h]),
+                                                                        __builtin_bit_cast(bf16x8, tok.x[n][h]),
+                                                                        acc[g * NT + n], 0, 0, 0);
       }
     } else {
       for (int s = ws.wave; s < p.I / 32; s += W) {
-        ColumnStep<N, true> st;
+        ColumnStep<N, NT, true> st;
         st.load(w + s * 32 * row_bytes, w_off, row_bytes, x + s * 64, x_off);
         st.multiply(acc);
       }
     }
-    if (c0) __syncthreads();  // the 16 tokens before have been joined
+    if (c0) __syncthreads();  // the tokens before have been joined
     ws.leave(red, acc);
     __syncthreads();
     // rows 4q..4q + 3 of an operand and token j are kept side by side in y
-    for (int op = ws.wave; op < N; op += W) {
-      const f32x4 v = ws.template join<N>(red, op);
-      if (c0 + j < wk.count) put_y(p.y + route * p.H + col + op * 16 + 4 * q, v);
+    for (int op = ws.wave; op < N * NT; op += W) {
+      const f32x4 v = ws.template join<N * NT>(red, op);
+      const int at = c0 + op % NT * 16 + j;
+      if (at < wk.count) put_y(p.y + static_cast<int64_t>(list[at]) * p.H + col + op / NT * 16 + 4 * q, v);
     }
   }
   finish<C, W * 64>(p, wk, live, [](int at) { return ROWS ? at : at % 16 * N + at / 16; });
@@ -404,12 +436,12 @@ __global__ __launch_bounds__(W * 64) void few_fc2_kernel(FewArgs p) {
 
 // ------------------------------------------------------------------ int8
 // Tile of 32 columns: operands 0, 1 are gate rows of w1, 2, 3 up rows. The
-// first wave joins them and has the 32 columns of 16 tokens in its registers,
-// 8 of a token in a lane, the others 16, 32 and 48 lanes on.
-template <int W>
+// wave that joins 16 tokens has their 32 columns in its registers, 8 of a token
+// in a lane, the others 16, 32 and 48 lanes on.
+template <int W, int NT>
 __global__ __launch_bounds__(W * 64) void few_fc1_int8_kernel(FewArgs p) {
   constexpr int C = kGroup, G = 2;
-  __shared__ i32x4 red[W * 2 * G * 64];
+  __shared__ i32x4 red[W * 2 * G * NT * 64];
   const Waves<W> ws;
   const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
   uint16_t* list = list_of(p);
@@ -423,68 +455,77 @@ __global__ __launch_bounds__(W * 64) void few_fc1_int8_kernel(FewArgs p) {
   const int64_t up_bytes = static_cast<int64_t>(p.I) * p.H;
   const char* w = static_cast<const char*>(p.w1) + 2 * wk.expert * up_bytes + static_cast<int64_t>(col) * p.H;
   const uint32_t w_off = j * p.H + 16 * q;
-  for (int c0 = 0; c0 < wk.count; c0 += kTokens) {
-    const int64_t route = list[min(c0 + j, wk.count - 1)];
-    const int token = static_cast<int>(route) / p.top_k;
-    const uint32_t x_off = static_cast<uint32_t>(token) * p.H + 16 * q;
-    i32x4 acc[2 * G];
+  for (int c0 = 0; c0 < wk.count; c0 += NT * 16) {
+    int routes[NT];
+    uint32_t x_off[NT];
+    routes_of<NT>(list, c0, wk.count, routes);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x_off[n] = static_cast<uint32_t>(routes[n] / p.top_k) * p.H + 16 * q;
+    i32x4 acc[2 * G * NT];
     clear(acc);
     for (int s = ws.wave; s < p.H / 128; s += W) {
       RowStep<G> gate, up;
-      TokenStep tok;
+      TokenStep<NT> tok;
       gate.load(w + s * 128, 16 * p.H, w_off);
       up.load(w + up_bytes + s * 128, 16 * p.H, w_off);
       tok.load(static_cast<const char*>(p.x) + s * 128, x_off);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(gate.w[g][h], tok.x[h], acc[g], 0, 0, 0);
-          acc[G + g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(up.w[g][h], tok.x[h], acc[G + g], 0, 0, 0);
-        }
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            i32x4 &a = acc[g * NT + n], &b = acc[(G + g) * NT + n];
+            a = __builtin_amdgcn_mfma_i32_16x16x64_i8(gate.w[g][h], tok.x[n][h], a, 0, 0, 0);
+            b = __builtin_amdgcn_mfma_i32_16x16x64_i8(up.w[g][h], tok.x[n][h], b, 0, 0, 0);
+          }
     }
-    if (c0) __syncthreads();  // the 16 tokens before have been joined
+    if (c0) __syncthreads();  // the tokens before have been joined
     ws.leave(red, acc);
     __syncthreads();
-    if (ws.wave) continue;
+    // one wave joins a block of 16 tokens
+    for (int n = ws.wave; n < NT; n += W) {
+      const int at = c0 + n * 16 + j, route = list[min(at, wk.count - 1)];
+      const float sx = p.x_scale[route / p.top_k], wt = p.w[route];
+      const float* sc = p.w1_scale + static_cast<int64_t>(wk.expert) * 2 * p.I + col + 4 * q;
+      float a[G][4];
+      uint32_t top = 0;  // of the bit patterns, where NaN lies above infinity
 #pragma unroll
-    for (int g = 0; g < 2 * G; ++g) acc[g] = ws.template join<2 * G>(red, g);
-    const float sx = p.x_scale[token], wt = p.w[route];
-    const float* sc = p.w1_scale + static_cast<int64_t>(wk.expert) * 2 * p.I + col + 4 * q;
-    float a[G][4];
-    uint32_t top = 0;  // of the bit patterns, where NaN lies above infinity
+      for (int g = 0; g < G; ++g) {
+        const i32x4 gate = ws.template join<2 * G * NT>(red, g * NT + n), up = ws.template join<2 * G * NT>(red, (G + g) * NT + n);
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        a[g][r] = gated_act(p.act_kind, static_cast<float>(acc[g][r]) * (sx * sc[g * 16 + r]),
-                            static_cast<float>(acc[G + g][r]) * (sx * sc[p.I + g * 16 + r]), p.beta, p.lbeta, p.limit) * wt;
-        top = max(top, __float_as_uint(a[g][r]) & 0x7fffffffu);
+        for (int r = 0; r < 4; ++r) {
+          a[g][r] = gated_act(p.act_kind, static_cast<float>(gate[r]) * (sx * sc[g * 16 + r]),
+                              static_cast<float>(up[r]) * (sx * sc[p.I + g * 16 + r]), p.beta, p.lbeta, p.limit) * wt;
+          top = max(top, __float_as_uint(a[g][r]) & 0x7fffffffu);
+        }
       }
-    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-    if (c0 + j >= wk.count) continue;
-    const bool finite = top < 0x7f800000u;
-    const float most = fmaxf(__uint_as_float(top), kScaleFloor), inv = finite ? 127.0f / most : 0.0f;
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+      if (at >= wk.count) continue;
+      const bool finite = top < 0x7f800000u;
+      const float most = fmaxf(__uint_as_float(top), kScaleFloor), inv = finite ? 127.0f / most : 0.0f;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      uint32_t b = 0;
+      for (int g = 0; g < G; ++g) {
+        uint32_t b = 0;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        b |= static_cast<uint32_t>(finite ? static_cast<int>(__builtin_rintf(a[g][r] * inv)) & 0xff : 0) << (8 * r);
-      *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(p.act) + route * p.I + col + g * 16 + 4 * q) = b;
+        for (int r = 0; r < 4; ++r)
+          b |= static_cast<uint32_t>(finite ? static_cast<int>(__builtin_rintf(a[g][r] * inv)) & 0xff : 0) << (8 * r);
+        *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(p.act) + static_cast<int64_t>(route) * p.I + col + g * 16 + 4 * q) = b;
+      }
+      if (q == 0)
+        p.act_scale[static_cast<int64_t>(route) * (p.I / C) + col / C] = finite ? most / 127.0f : __uint_as_float(0x7fc00000u);
     }
-    if (q == 0) p.act_scale[route * (p.I / C) + col / C] = finite ? most / 127.0f : __uint_as_float(0x7fc00000u);
   }
 }
 
 // Tile of 64 columns. An instruction's 64 elements span two scale groups (the
 // operand's lanes 0..31 and 32..63), so each is multiplied with the other's
 // activations zeroed and joins the fp32 sum under its own scale.
-template <int W>
+template <int W, int NT>
 __global__ __launch_bounds__(W * 64) void few_fc2_int8_kernel(FewArgs p) {
   constexpr int G = 4, C = 16 * G;
-  __shared__ f32x4 red[W * G * 64];
+  __shared__ f32x4 red[W * G * NT * 64];
   const Waves<W> ws;
   const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
   uint16_t* list = list_of(p);
@@ -495,43 +536,52 @@ __global__ __launch_bounds__(W * 64) void few_fc2_int8_kernel(FewArgs p) {
   const int col = wk.tile * C;
   const char* w = static_cast<const char*>(p.w2) + (static_cast<int64_t>(wk.expert) * p.H + col) * p.I;
   const uint32_t w_off = j * p.I + 16 * q;
-  for (int c0 = 0; c0 < wk.count; c0 += kTokens) {
-    const int64_t route = list[min(c0 + j, wk.count - 1)];
-    const uint32_t x_off = static_cast<uint32_t>(route) * p.I + 16 * q;
-    const uint32_t sc_off = static_cast<uint32_t>(route) * (p.I / kGroup) * 4;
-    f32x4 acc[G];
+  for (int c0 = 0; c0 < wk.count; c0 += NT * 16) {
+    int route[NT];
+    uint32_t x_off[NT], sc_off[NT];
+    routes_of<NT>(list, c0, wk.count, route);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      x_off[n] = static_cast<uint32_t>(route[n]) * p.I + 16 * q;
+      sc_off[n] = static_cast<uint32_t>(route[n]) * (p.I / kGroup) * 4;
+    }
+    f32x4 acc[G * NT];
     clear(acc);
     for (int s = ws.wave; s < p.I / 128; s += W) {
       RowStep<G> st;
-      TokenStep tok;
-      float sv[4];
+      TokenStep<NT> tok;
+      f32x4 sv[NT];
       st.load(w + s * 128, 16 * p.I, w_off);
       tok.load(static_cast<const char*>(p.act) + s * 128, x_off);
-      __builtin_memcpy(sv, reinterpret_cast<const char*>(p.act_scale) + s * (128 / kGroup * 4) + sc_off, 16);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        __builtin_memcpy(&sv[n], reinterpret_cast<const char*>(p.act_scale) + s * (128 / kGroup * 4) + sc_off[n], 16);
       const i32x4 zero = {0, 0, 0, 0};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const i32x4 lo = lane < 32 ? tok.x[h] : zero, hi = lane < 32 ? zero : tok.x[h];
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const i32x4 a = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.w[g][h], lo, zero, 0, 0, 0);
-          const i32x4 b = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.w[g][h], hi, zero, 0, 0, 0);
+        for (int n = 0; n < NT; ++n) {
+          const i32x4 lo = lane < 32 ? tok.x[n][h] : zero, hi = lane < 32 ? zero : tok.x[n][h];
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            acc[g][r] += static_cast<float>(a[r]) * sv[2 * h] + static_cast<float>(b[r]) * sv[2 * h + 1];
+          for (int g = 0; g < G; ++g) {
+            const i32x4 a = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.w[g][h], lo, zero, 0, 0, 0);
+            const i32x4 b = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.w[g][h], hi, zero, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              acc[g * NT + n][r] += static_cast<float>(a[r]) * sv[n][2 * h] + static_cast<float>(b[r]) * sv[n][2 * h + 1];
+          }
         }
-      }
     }
-    if (c0) __syncthreads();  // the 16 tokens before have been joined
+    if (c0) __syncthreads();  // the tokens before have been joined
     ws.leave(red, acc);
     __syncthreads();
-    for (int op = ws.wave; op < G; op += W) {
-      f32x4 v = ws.template join<G>(red, op);
-      const int at = col + op * 16 + 4 * q;
-      const float* sc = p.w2_scale + static_cast<int64_t>(wk.expert) * p.H + at;
+    for (int op = ws.wave; op < G * NT; op += W) {
+      f32x4 v = ws.template join<G * NT>(red, op);
+      const int at = c0 + op % NT * 16 + j, c = col + op / NT * 16 + 4 * q;
+      const float* sc = p.w2_scale + static_cast<int64_t>(wk.expert) * p.H + c;
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] *= sc[k];
-      if (c0 + j < wk.count) put_y(p.y + route * p.H + at, v);
+      if (at < wk.count) put_y(p.y + static_cast<int64_t>(list[at]) * p.H + c, v);
     }
   }
   finish<C, W * 64>(p, wk, live, [](int at) { return at; });
@@ -585,6 +635,17 @@ int launch_both(FewArgs p, const Launch& a, const Launch& b, hipStream_t s) {
   return mm_check_launch("few_fc2_kernel");
 }
 
+// Blocks of 16 tokens in a pass over an expert's weights, by the mean rows of an
+// expert: more than its rows need cost occupancy (60 experts of 8.5 rows: 85 us
+// with one, 95 with two), fewer read the weights again (32 of 16 rows: 234 us
+// with one, 150 with two; 8 of 64: 30 us with two, 19 with four).
+template <class F>
+int by_blocks(const FewArgs& p, F&& f) {
+  if (p.tokens <= 16 || p.R <= 10 * p.E) return f(std::integral_constant<int, 1>{});
+  if (p.tokens <= 32 || p.R <= 24 * p.E) return f(std::integral_constant<int, 2>{});
+  return f(std::integral_constant<int, 4>{});
+}
+
 }  // namespace
 
 extern "C" size_t mm_moe_few_scratch_bytes(int64_t tokens, int32_t top_k, int32_t hidden, int32_t inter, int32_t int8) {
@@ -621,8 +682,13 @@ extern "C" int mm_moe_few(const uint16_t* x, const int32_t* selected, const floa
   // 32 columns, twice as many, win (8 experts of 1024 columns: 25 us against 40;
   // of 768, one token: 12.3 against 17.8; 112 experts of 768: 156 against 117)
   const bool wide = static_cast<int64_t>(slots_of(p)) * (inter / 64) >= 512;
-  return launch_both(p, wide ? Launch{few_fc1_kernel<8, 8>, 8, 64} : Launch{few_fc1_kernel<4, 8>, 8, 32},
-                     rows ? Launch{few_fc2_kernel<true, 4, 8>, 8, 64} : Launch{few_fc2_kernel<false, 4, 8>, 8, 64}, s);
+  auto run = [&](auto blocks) {
+    constexpr int NT = decltype(blocks)::value;
+    constexpr int WIDE = NT < 4 ? 8 : 4;  // the partial sums of 64 tokens and 64 columns do not fit LDS
+    return launch_both(p, wide ? Launch{few_fc1_kernel<WIDE, 8, NT>, 8, 8 * WIDE} : Launch{few_fc1_kernel<4, 8, NT>, 8, 32},
+                       rows ? Launch{few_fc2_kernel<true, 4, 8, NT>, 8, 64} : Launch{few_fc2_kernel<false, 4, 8, NT>, 8, 64}, s);
+  };
+  return by_blocks(p, run);
 }
 
 extern "C" int mm_moe_few_int8(const int8_t* x, const float* x_scale, const int32_t* selected,
@@ -648,5 +714,9 @@ extern "C" int mm_moe_few_int8(const int8_t* x, const float* x_scale, const int3
             reinterpret_cast<float*>(base + f.act_scale), reinterpret_cast<float*>(base + f.y),
             reinterpret_cast<int32_t*>(base + f.done), reinterpret_cast<bf16*>(out), 0, 0, 0};
   const hipStream_t s = mm_hip_stream(stream);
-  return launch_both(p, {few_fc1_int8_kernel<4>, 4, kGroup}, {few_fc2_int8_kernel<4>, 4, 64}, s);
+  auto run = [&](auto blocks) {
+    constexpr int NT = decltype(blocks)::value;
+    return launch_both(p, {few_fc1_int8_kernel<4, NT>, 4, kGroup}, {few_fc2_int8_kernel<4, NT>, 4, 64}, s);
+  };
+  return by_blocks(p, run);
 }

@@ -391,7 +391,7 @@ class FusedMoEForward(torch.nn.Module):
         Arguments and result as ``forward``; sums are fp32 and only the
         activation and the output are rounded to bf16 (``forward`` also rounds
         gate, up and the expert outputs), so the last bits differ from
-        ``forward``'s. Nothing is saved for a backward, no workspace of the
+        ``forward``'s; they do not depend on the other tokens of the call. Nothing is saved for a backward, no workspace of the
         operator is used and its routing generation does not move: calls may run
         on any stream, between a forward and its backward, and captured.
         No counterpart in the reference.

@@ -200,12 +200,12 @@ def test_a_token_does_not_see_the_others():
 
 
 @pytest.mark.parametrize("int8", [False, True])
-def test_batch_of_one_has_the_same_bits(int8):
-    """A token's output does not depend on which others are in the call while
-    the call stays within 16 tokens, nor beyond (17 to 64)."""
-    E, k, H, F = 24, 3, 384, 256
-    for T in (16, 40):
-        sel, w = _routing(T, E, k, "even", 8)
+def test_bits_do_not_depend_on_the_batch(int8):
+    """A token's output is the same alone and with others, whatever tiles the
+    sizes choose (16, 32 and 64 rows of an expert, 32 and 64 columns)."""
+    for E, k, F in ((24, 3, 256), (4, 4, 256), (64, 8, 1024)):
+        H, T = 384, 64
+        sel, w = _routing(T, E, k, "drop", 8)
         op = _operator(E, k, H)
         if int8:
             x, xs, ex = _int8_inputs(T, E, H, F)
@@ -215,8 +215,8 @@ def test_batch_of_one_has_the_same_bits(int8):
             x = torch.randn(T, H, device="cuda").to(BF)
             run = lambda a, b: op.forward_few(x[a:b], sel[a:b], gu, dn, w[a:b])
         full = run(0, T)
-        for a, b in ((0, T - 3), (T - 17 if T > 17 else 1, T)):
-            assert torch.equal(run(a, b), full[a:b])
+        for a, b in ((0, 1), (5, 21), (7, 40), (63, 64)):
+            assert torch.equal(run(a, b), full[a:b]), (E, a, b)
 
 
 def test_experts_past_32_bits():
