@@ -122,6 +122,26 @@ def call(name: str, *args):
         raise MegaMoEError(f"{name} failed ({rc}): {msg}")
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The native torch front (``_torch_ops.so``, built with the library), on
+    the library that ``load()`` has loaded. No fallback: without it the
+    operators it serves raise."""
+    global _torch_ops
+    if _torch_ops is None:
+        try:
+            from . import _torch_ops as ops
+        except ImportError as e:
+            raise RuntimeError("mega_moe/_torch_ops.so is missing or does not fit this torch; build it with "
+                               "`make -C mega-moe-td_amd/csrc`") from e
+        load()
+        ops.bind(_LIB_PATH, MegaMoEError)
+        _torch_ops = ops
+    return _torch_ops
+
+
 def ptr(t: torch.Tensor | None):
     """Raw device address of a tensor (None -> NULL)."""
     return None if t is None else ctypes.c_void_p(t.data_ptr())

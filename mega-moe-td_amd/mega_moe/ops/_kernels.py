@@ -326,156 +326,3 @@ def layer_backward(dy, x, w1, w2, tokens: int, top_k: int, offsets, send_token, 
               dab.data_ptr(), dscale.data_ptr(), grad_fc2.data_ptr(), dx.data_ptr(), gh.data_ptr(), grw.data_ptr(),
               ggu.data_ptr(), torch.cuda.current_stream(dy.device).cuda_stream)
     return grad_act, dab, dscale, grad_fc2, dx, gh, grw, ggu
-
-
-def _raw_stream(index: int) -> int:
-    return torch.cuda.current_stream(index).cuda_stream
-
-
-# the handle without the Stream object around it, where this torch has it (2 us less a call)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-
-
-def _launch(device: torch.device, name: str, *args):
-    """Call an entry point on torch's current stream of ``device``, which need
-    not be the current device (kernels launch on the current one)."""
-    index = device.index
-    if index == _current_device():
-        _lib.call(name, *args, _raw_stream(index))
-    else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, _raw_stream(index))
-
-
-def _empty(like: torch.Tensor, dtype=None) -> torch.Tensor:
-    """A contiguous tensor of ``like``'s shape and device."""
-    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
-
-
-def _rows(name: str, t: torch.Tensor):
-    """(address, row stride, rows) of ``t`` [..., columns] as evenly spaced rows."""
-    if t.dim() == 2:
-        rows, columns = t.shape
-        ld, step = t.stride()
-        if step == 1 or columns <= 1:
-            return t.data_ptr(), ld, rows
-    columns = t.shape[-1]
-    if columns > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name} must have unit column stride")
-    if t.dim() == 1:
-        return t.data_ptr(), columns, 1
-    try:
-        flat = t.view(-1, columns)
-    except RuntimeError:
-        raise ValueError(f"the rows of {name} must be evenly spaced in memory") from None
-    return flat.data_ptr(), flat.stride(0), flat.shape[0]
-
-
-_TYPES = _lib.ELEMENT_TYPES
-
-
-def rms_norm(x, weight, residual, eps: float, out_dtype, keep_rstd: bool = False):
-    """(y, scale | None, h | None, rstd | None) for operands ``ops.norm`` has checked."""
-    dev, hidden = x.device, x.shape[-1]
-    xp, ldx, rows = _rows("x", x)
-    rp = ldr = 0
-    h = None
-    xt = ht = _TYPES[x.dtype]
-    if residual is not None:
-        rp, ldr, _ = _rows("residual", residual)
-        ht = _TYPES[residual.dtype]
-        h = _empty(residual)
-    y = _empty(x, out_dtype)
-    scale = None if out_dtype == x.dtype else torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if keep_rstd else None
-    if rows:
-        _launch(dev, "mm_rms_norm", xp, ldx, xt, rp, ldr, ht, None if weight is None else weight.data_ptr(),
-                0 if weight is None else _TYPES[weight.dtype], rows, hidden, eps, None if h is None else h.data_ptr(),
-                y.data_ptr(), _TYPES[out_dtype], None if scale is None else scale.data_ptr(),
-                None if rstd is None else rstd.data_ptr())
-    return y, scale, h, rstd
-
-
-def rms_norm_bwd(dy, dh, h, weight, rstd, x_dtype, want_residual: bool, want_weight: bool):
-    """(dx, dresidual | None, dweight | None); dresidual is dx itself where the types agree."""
-    dev, hidden = h.device, h.shape[-1]
-    dy = dy.contiguous()  # a gradient comes in any layout (an expanded scalar, a transposed view)
-    dhp = 0
-    if dh is not None:
-        dh = dh.contiguous()
-        dhp = dh.data_ptr()
-    hp, ldh, rows = _rows("h", h)
-    dx = _empty(h, x_dtype)
-    dres = None
-    if want_residual:
-        dres = dx if h.dtype == x_dtype else _empty(h)
-    dw = ws = None
-    nbytes = 0
-    if want_weight:
-        dw = torch.empty(hidden, dtype=weight.dtype, device=dev)
-        nbytes = _lib.load().mm_rms_norm_bwd_workspace_bytes(rows, hidden)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    if rows or want_weight:
-        _launch(dev, "mm_rms_norm_bwd", dy.data_ptr(), hidden, dhp, hidden, hp, ldh, None if weight is None else weight.data_ptr(),
-                0 if weight is None else _TYPES[weight.dtype], rstd.data_ptr(), _TYPES[x_dtype], _TYPES[h.dtype], rows,
-                hidden, dx.data_ptr(), None if dres is None or dres is dx else dres.data_ptr(),
-                None if dw is None else dw.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
-    return dx, dres, dw
-
-
-def quantize_rows(x, dtype):
-    """(q, scale) of the rows of ``x``."""
-    xp, ldx, rows = _rows("x", x)
-    q = _empty(x, dtype)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    if rows:
-        _launch(x.device, "mm_quantize_rows", xp, ldx, _TYPES[x.dtype], rows, x.shape[-1], q.data_ptr(), _TYPES[dtype],
-                scale.data_ptr())
-    return q, scale
-
-
-def int8_matmul(a, b, a_scale, b_scale, bias, out_dtype):
-    """[..., N] product of operands ``ops.int8`` has checked."""
-    ap, lda, m = _rows("a", a)
-    n, k = b.shape
-    out = torch.empty(m, n, dtype=out_dtype, device=a.device)
-    if m:
-        if m > 1 and not k <= lda <= 1 << 23:
-            raise ValueError(f"the rows of a must be {k} to {1 << 23} elements apart (no overlap), got {lda}")
-        _launch(a.device, "mm_int8_matmul", ap, lda, b.data_ptr(), b.stride(0), a_scale.data_ptr(), b_scale.data_ptr(),
-                None if bias is None else bias.data_ptr(), 0 if bias is None else _TYPES[bias.dtype], m, n, k,
-                out.data_ptr(), n, _TYPES[out_dtype])
-    return out if a.dim() == 2 else out.view(*a.shape[:-1], n)
-
-
-def few_forward(x, selected, routing_weights, w1, w2, num_experts: int, activation: str, situ_beta: float,
-                situ_linear_beta, clamp_limit: float):
-    """The layer for a few tokens (``mm_moe_few``), for operands the operator has validated."""
-    tokens, top_k = selected.shape
-    hidden, inter = x.shape[1], w1.shape[2] // 2
-    out = torch.empty(tokens, hidden, dtype=torch.bfloat16, device=x.device)
-    nbytes = _lib.load().mm_moe_few_scratch_bytes(tokens, top_k, hidden, inter, 0)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    se, sh, sf = w2.stride()
-    _launch(x.device, "mm_moe_few", x.data_ptr(), selected.data_ptr(), routing_weights.data_ptr(), w1.data_ptr(),
-            w2.data_ptr(), se, sh, sf, tokens, top_k, num_experts, hidden, inter, _lib.ACT_KINDS[activation],
-            situ_beta, situ_linear_beta if situ_linear_beta is not None else 0.0, clamp_limit, out.data_ptr(),
-            scratch.data_ptr(), nbytes)
-    return out
-
-
-def few_forward_int8(x, x_scale, selected, routing_weights, experts, num_experts: int, activation: str,
-                     situ_beta: float, situ_linear_beta, clamp_limit: float):
-    """The int8 layer for a few tokens (``mm_moe_few_int8``), for operands the operator has validated."""
-    tokens, top_k = selected.shape
-    hidden, inter = x.shape[1], experts.down.shape[2]
-    out = torch.empty(tokens, hidden, dtype=torch.bfloat16, device=x.device)
-    nbytes = _lib.load().mm_moe_few_scratch_bytes(tokens, top_k, hidden, inter, 1)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    _launch(x.device, "mm_moe_few_int8", x.data_ptr(), x_scale.data_ptr(), selected.data_ptr(),
-            routing_weights.data_ptr(), experts.gate_up.data_ptr(), experts.gate_up_scale.data_ptr(),
-            experts.down.data_ptr(), experts.down_scale.data_ptr(), tokens, top_k, num_experts, hidden, inter,
-            _lib.ACT_KINDS[activation], situ_beta, situ_linear_beta if situ_linear_beta is not None else 0.0,
-            clamp_limit, out.data_ptr(), scratch.data_ptr(), nbytes)
-    return out

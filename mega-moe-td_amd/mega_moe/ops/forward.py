@@ -129,6 +129,7 @@ class FusedMoEForward(torch.nn.Module):
         self._routing_generation = 0
         self._forward_stream = None
         self._device = None
+        self._few = None  # the native description of the layer for a few tokens
         # optional runtime.timing.StageTimer: HIP events between stages
         # (MOE_FWD_TIMING=1 attaches one, as the reference's phase stamps are
         # switched on by that variable, ops/forward.py:1656-1660)
@@ -380,6 +381,19 @@ class FusedMoEForward(torch.nn.Module):
             raise ValueError(f"at most {MAX_FEW_TOKENS} tokens, got {selected_experts.shape[0]}; "
                              "use forward for more")
 
+    def _few_layer(self, rows):
+        """The native front and this operator's description for it; ``None`` for
+        the latter where ``rows`` are not on the operator's device."""
+        ops = _lib.torch_ops()
+        if self._few is None:
+            lbeta = self.situ_linear_beta
+            self._few = ops.Layer(min(MAX_FEW_TOKENS, self.max_tokens_per_rank), self.top_k, self.experts_per_rank,
+                                  self.hidden_size, _lib.ACT_KINDS[self.activation], self.situ_beta,
+                                  0.0 if lbeta is None else lbeta, self.clamp_limit)
+        if self._device is None and rows.is_cuda:
+            self._device = rows.device
+        return ops, self._few if rows.device == self._device else None
+
     def _validate_few_sizes(self, two_inter):
         if self.hidden_size % 128 or two_inter % 256:
             raise ValueError("hidden_size and ffn size must be multiples of 128 for the MFMA tiles")
@@ -396,17 +410,19 @@ class FusedMoEForward(torch.nn.Module):
         on any stream, between a forward and its backward, and captured.
         No counterpart in the reference.
         """
+        ops, layer = self._few_layer(hidden_states)
+        out = layer and ops.few_forward(layer, hidden_states, selected_experts, gate_up_weight, down_weight,
+                                        routing_weights)
+        if out is not None:
+            return out
+        # the operands do not fit the layer: one of these checks says why
         self._validate_dispatch_inputs(hidden_states, selected_experts)
         self._validate_few(selected_experts)
         self._validate_gate_up_weight(gate_up_weight, hidden_states.device)
         self._validate_routing_weights(routing_weights, selected_experts)
         self._validate_down_weight(down_weight, gate_up_weight, hidden_states.device)
         self._validate_few_sizes(gate_up_weight.shape[2])
-        if not hidden_states.shape[0]:
-            return torch.empty_like(hidden_states)
-        return K.few_forward(hidden_states, selected_experts, routing_weights, gate_up_weight, down_weight,
-                             self.experts_per_rank, self.activation, self.situ_beta, self.situ_linear_beta,
-                             self.clamp_limit)
+        raise ValueError("the operands do not fit the operator")
 
     def forward_few_int8(self, tokens, token_scale, selected_experts, experts: Int8Experts, routing_weights):
         """``forward_few`` on int8 rows and int8 experts.
@@ -417,10 +433,16 @@ class FusedMoEForward(torch.nn.Module):
         rounded to int8 in groups of 32 columns with the group's largest value
         at 127. A NaN or infinite scale makes its own token's output NaN.
         """
-        self._validate_topk_indices(selected_experts)
-        self._validate_few(selected_experts)
         if not isinstance(experts, Int8Experts):
             raise TypeError("experts must be an Int8Experts")
+        ops, layer = self._few_layer(tokens)
+        out = layer and ops.few_forward_int8(layer, tokens, token_scale, selected_experts, experts.gate_up,
+                                             experts.gate_up_scale, experts.down, experts.down_scale, routing_weights)
+        if out is not None:
+            return out
+        # the operands do not fit the layer: one of these checks says why
+        self._validate_topk_indices(selected_experts)
+        self._validate_few(selected_experts)
         expected = (selected_experts.shape[0], self.hidden_size)
         if tokens.dtype != torch.int8:
             raise TypeError(f"tokens must use torch.int8, got {tokens.dtype}")
@@ -438,11 +460,7 @@ class FusedMoEForward(torch.nn.Module):
         device = selected_experts.device
         if tokens.device != device or token_scale.device != device or experts.gate_up.device != device:
             raise ValueError("tokens, token_scale, selected_experts and experts must be on the same device")
-        if not expected[0]:
-            return torch.empty(expected, dtype=torch.bfloat16, device=device)
-        return K.few_forward_int8(tokens, token_scale, selected_experts, routing_weights, experts,
-                                  self.experts_per_rank, self.activation, self.situ_beta, self.situ_linear_beta,
-                                  self.clamp_limit)
+        raise ValueError("the operands do not fit the operator")
 
     # ------------------------------------------------------------ full forward
     def _forward_staged(self, hidden_states, selected_experts, gate_up_weight, down_weight, routing_weights,

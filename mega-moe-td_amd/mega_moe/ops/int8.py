@@ -13,12 +13,8 @@ from typing import Optional
 
 import torch
 
-from . import _kernels as K
+from .. import _lib
 from .norm import MAX_HIDDEN, quantize_rows
-
-MAX_STRIDE = 1 << 23  # of a row, 256 of which a kernel's offsets have to span
-MAX_K = (1 << 17) - 1  # the int32 sum is exact below 2^17 products of two int8 values
-_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, *,
@@ -32,43 +28,7 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
     in int32; scales and bias are applied in fp32 and the result is rounded
     once to bf16, fp16 or fp32. No gradient.
     """
-    if a.dtype != torch.int8 or b.dtype != torch.int8:
-        raise TypeError(f"a and b must be torch.int8, got {a.dtype} and {b.dtype}")
-    if a.dim() == 0 or b.dim() != 2:
-        raise ValueError(f"a must have shape [..., K] and b [N, K], got {tuple(a.shape)} and {tuple(b.shape)}")
-    n, k = b.shape
-    if a.shape[-1] != k:
-        raise ValueError(f"a has {a.shape[-1]} columns, b has {k}")
-    if not 1 <= k <= MAX_K or n < 1:
-        raise ValueError(f"b must have shape [N, K] with N >= 1 and 1 <= K <= {MAX_K}, got {tuple(b.shape)}")
-    ldb, step = b.stride()
-    if k > 1 and step != 1:
-        raise ValueError("b must have unit column stride ([N, K], K contiguous)")
-    if n > 1 and not k <= ldb <= MAX_STRIDE:
-        raise ValueError(f"the rows of b must be {k} to {MAX_STRIDE} elements apart (no overlap), got {ldb}")
-    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
-        raise TypeError(f"a_scale and b_scale must be torch.float32, got {a_scale.dtype} and {b_scale.dtype}")
-    if a_scale.shape != a.shape[:-1] or not a_scale.is_contiguous():
-        raise ValueError(f"a_scale must be contiguous with shape {tuple(a.shape[:-1])}, got {tuple(a_scale.shape)}")
-    if b_scale.dim() != 1 or b_scale.shape[0] != n or not b_scale.is_contiguous():
-        raise ValueError(f"b_scale must be contiguous with shape ({n},), got {tuple(b_scale.shape)}")
-    if bias is not None:
-        if bias.dtype not in _FLOATS:
-            raise TypeError(f"bias must be bfloat16, float16 or float32, got {bias.dtype}")
-        if bias.dim() != 1 or bias.shape[0] != n or not bias.is_contiguous():
-            raise ValueError(f"bias must be contiguous with shape ({n},), got {tuple(bias.shape)}")
-    device = a.device
-    if b.device != device or a_scale.device != device or b_scale.device != device or (
-            bias is not None and bias.device != device):
-        raise ValueError("all operands must be on the device of a")
-    if out_dtype not in _FLOATS:
-        raise TypeError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
-    if (a_scale.requires_grad or b_scale.requires_grad or (bias is not None and bias.requires_grad)) \
-            and torch.is_grad_enabled():
-        raise ValueError("int8_matmul carries no gradient; call under torch.no_grad() or on detached operands")
-    if not a.is_cuda:
-        raise ValueError("a must be a HIP device tensor")
-    return K.int8_matmul(a, b, a_scale, b_scale, bias, out_dtype)
+    return _lib.torch_ops().int8_matmul(a, b, a_scale, b_scale, bias, out_dtype)
 
 
 @dataclass(frozen=True)

@@ -195,3 +195,16 @@ def test_few_entry_refuses_strides_and_small_scratch():
     assert b"scratch" in lib.mm_last_error()
     need = lib.mm_moe_few_scratch_bytes(1, 1, 128, 128, 1)
     assert lib.mm_moe_few_int8(*[FAKE] * 8, *tail, need - 1, None) == -2
+
+
+@built
+def test_an_operator_can_be_copied_and_pickled():
+    """The native description of the few-token layer travels with the operator."""
+    import copy
+    import pickle
+
+    op = mega_moe.FusedMoEForward(None, max_tokens_per_rank=8, hidden_size=128, top_k=2, num_experts=4)
+    op._few_layer(torch.zeros(1, 128))
+    assert op._few is not None
+    for other in (copy.deepcopy(op), pickle.loads(pickle.dumps(op))):
+        assert other.top_k == 2 and other._few is not None and other._few is not op._few
