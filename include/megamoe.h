@@ -440,8 +440,9 @@ int mm_moe_few_int8(const int8_t* x, const float* x_scale,
  * scale [rows] a row: a = max |y| of the row, scale = max(a, 1e-30) / Q (Q =
  * 127 or 448; 1 where a = 0), y = round(y / scale). A row that holds a NaN or
  * an infinity gets scale NaN and bytes 0. rstd ([rows], or NULL) receives
- * 1 / sqrt(mean(h^2) + eps) for the backward. No counterpart in the reference,
- * whose layer begins behind the norm.
+ * 1 / sqrt(mean(h^2) + eps) for the backward. Outputs overlap neither inputs
+ * nor each other, here and in the entries below. No counterpart in the
+ * reference, whose layer begins behind the norm.
  */
 int mm_rms_norm(const void* x, int64_t ldx, int32_t x_type, const void* residual,
                 int64_t ldr, int32_t h_type, const void* weight,
@@ -477,9 +478,9 @@ int mm_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int64_t rows,
 /*
  * out[i, j] = a_scale[i] * b_scale[j] * sum_k a[i, k] * b[j, k] + bias[j]
  * for int8 a [m, k] and b [n, k], unit column strides, row strides lda and ldb
- * from k to 2^23 at any alignment. The sum is exact in int32 (k < 2^17); scales and bias
- * (NULL: none; BF16, FP16 or FP32) are applied in fp32 and the result is
- * rounded once to out_type (BF16, FP16 or FP32; row stride ldo). No
+ * from k to 2^23 at any alignment. The sum is exact in int32 (k < 2^17);
+ * scales and bias (NULL: none; BF16, FP16 or FP32) are applied in fp32 and the
+ * result is rounded once to out_type (BF16, FP16 or FP32; row stride ldo). No
  * counterpart in the reference.
  */
 int mm_int8_matmul(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb,

@@ -621,7 +621,7 @@ struct Launch {
 
 int launch_both(FewArgs p, const Launch& a, const Launch& b, hipStream_t s) {
   const int slots = slots_of(p), tiles1 = p.I / a.width, tiles2 = p.H / b.width;
-  MM_CHECK_ARG(static_cast<int64_t>(slots) * (tiles1 > tiles2 ? tiles1 : tiles2) < (int64_t(1) << 23),
+  MM_CHECK_ARG(static_cast<int64_t>(slots) * (tiles1 > tiles2 ? tiles1 : tiles2) + 1 < (int64_t(1) << 23),
                "mm_moe_few: too many tiles");
   const size_t lds = route_lds_bytes(p.R);
   p.slots = slots;

@@ -14,6 +14,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -114,6 +115,12 @@ void check_device(const char* name, const Tensor& t) {
   CHECK_VALUE(t.is_cuda(), name, " must be a HIP device tensor");
 }
 
+// Forward-mode derivatives do not exist here; a tangent would be lost silently.
+void check_no_tangent(const char* op, std::initializer_list<const OptTensor*> tensors) {
+  for (const OptTensor* t : tensors)
+    CHECK_VALUE(!*t || !(*t)->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+}
+
 void check_vector(const char* name, const Tensor& t, int64_t n) {
   CHECK_VALUE(t.dim() == 1 && t.size(0) == n && t.is_contiguous(), name, " must be contiguous with shape (", n,
               ",), got ", t.sizes());
@@ -189,6 +196,21 @@ Tensor once_only(Tensor grad) {
   return std::move(raise({grad.detach().requires_grad_(true)})[0]);
 }
 
+// The engine hands a gradient over on the stream of the node that takes it. A
+// leaf's node keeps the stream of the first graph that used it while that
+// graph lives; where this is the default stream, which cannot be captured, the
+// hand-over would break a capture, and the process with it.
+void check_capture(const torch::autograd::Node& node, const at::Device& device) {
+  if (c10::hip::getCurrentHIPStream(device.index()).stream() == nullptr) return;
+  for (const torch::autograd::Edge& e : node.next_edges()) {
+    if (!e.is_valid()) continue;
+    const auto stream = e.function->stream();
+    if (stream && stream->id() == 0 && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+      throw CallError("rms_norm: this backward cannot be captured: a graph that was built on the default stream still "
+                      "uses an input; drop that graph, or build it on the stream of the capture");
+  }
+}
+
 struct RMSNorm : torch::autograd::Function<RMSNorm> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x,
                                                 const OptTensor& weight, const OptTensor& residual, double eps) {
@@ -205,6 +227,7 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
                                                  torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &h = saved[0], &rstd = saved[2];
+    check_capture(*torch::autograd::get_current_node(), h.device());
     OptTensor weight;
     if (saved[1].defined()) weight = saved[1];
     const bool residual = ctx->saved_data["residual"].toBool();
@@ -270,6 +293,7 @@ py::object rms_norm(const Tensor& x, const OptTensor& weight, const OptTensor& r
   const bool needs_grad = wants_grad({&ox, &weight, &residual}), eight = is_eight_bits(out);
   CHECK_VALUE(!eight || !needs_grad,
               "an 8-bit output carries no gradient; call under torch.no_grad() or on detached inputs");
+  check_no_tangent("rms_norm", {&ox, &weight, &residual});
   check_device("x", x);
   if (needs_grad) {
     auto o = RMSNorm::apply(x, weight, residual, eps);
@@ -290,6 +314,8 @@ py::tuple quantize_rows(const Tensor& x, ScalarType dtype) {
   CHECK_TYPE(is_eight_bits(dtype), "dtype must be int8 or float8_e4m3fn, got ", dtype);
   CHECK_VALUE(!x.requires_grad() || !at::GradMode::is_enabled(),
               "an 8-bit output carries no gradient; call under torch.no_grad() or on a detached input");
+  const OptTensor ox(x);
+  check_no_tangent("quantize_rows", {&ox});
   check_device("x", x);
   const Rows r("x", x);
   Tensor q = empty_as(x, dtype);
@@ -332,6 +358,7 @@ Tensor int8_matmul(const Tensor& a, const Tensor& b, const Tensor& a_scale, cons
   const OptTensor sa(a_scale), sb(b_scale);
   CHECK_VALUE(!wants_grad({&sa, &sb, &bias}),
               "int8_matmul carries no gradient; call under torch.no_grad() or on detached operands");
+  check_no_tangent("int8_matmul", {&sa, &sb, &bias});
   check_device("a", a);
   const Rows ra("a", a);
   CHECK_VALUE(ra.rows <= 1 || (ra.ld >= k && ra.ld <= kMaxStride), "the rows of a must be ", k, " to ", kMaxStride,

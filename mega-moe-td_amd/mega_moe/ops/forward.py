@@ -383,7 +383,8 @@ class FusedMoEForward(torch.nn.Module):
 
     def _few_layer(self, rows):
         """The native front and this operator's description for it; ``None`` for
-        the latter where ``rows`` are not on the operator's device."""
+        the latter where ``rows`` are not on the operator's device, which is that
+        of the first call."""
         ops = _lib.torch_ops()
         if self._few is None:
             lbeta = self.situ_linear_beta
@@ -405,10 +406,10 @@ class FusedMoEForward(torch.nn.Module):
         Arguments and result as ``forward``; sums are fp32 and only the
         activation and the output are rounded to bf16 (``forward`` also rounds
         gate, up and the expert outputs), so the last bits differ from
-        ``forward``'s; they do not depend on the other tokens of the call. Nothing is saved for a backward, no workspace of the
-        operator is used and its routing generation does not move: calls may run
-        on any stream, between a forward and its backward, and captured.
-        No counterpart in the reference.
+        ``forward``'s; they do not depend on the other tokens of the call. Nothing
+        is saved for a backward, no workspace of the operator is used and its
+        routing generation does not move: calls may run on any stream, between a
+        forward and its backward, and captured. No counterpart in the reference.
         """
         ops, layer = self._few_layer(hidden_states)
         out = layer and ops.few_forward(layer, hidden_states, selected_experts, gate_up_weight, down_weight,

@@ -21,10 +21,10 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
                 bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``(a * a_scale[..., None]) @ (b * b_scale[:, None]).T + bias`` in ``out_dtype``.
 
-    ``a`` int8 [..., K] (rows evenly spaced in memory, unit column stride) with
-    fp32 ``a_scale`` of ``a``'s leading shape, one a token; ``b`` int8 [N, K]
-    (unit column stride, rows up to 2^23 elements apart, as ``a``'s) with fp32 ``b_scale`` [N], one a
-    channel; ``bias`` [N] in bf16, fp16 or fp32. 1 <= K < 2^17: the sum is exact
+    ``a`` int8 [..., K] with fp32 ``a_scale`` of ``a``'s leading shape, one a
+    token; ``b`` int8 [N, K] with fp32 ``b_scale`` [N], one a channel; ``bias``
+    [N] in bf16, fp16 or fp32. Rows have unit column stride and are evenly
+    spaced in memory, K to 2^23 elements apart. 1 <= K < 2^17: the sum is exact
     in int32; scales and bias are applied in fp32 and the result is rounded
     once to bf16, fp16 or fp32. No gradient.
     """

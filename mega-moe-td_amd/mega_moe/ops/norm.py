@@ -4,8 +4,8 @@
 ``hidden_states``, or, in 8 bits with one scale a row, the rows that
 ``int8_matmul`` and ``FusedMoEForward.forward_few_int8`` take.
 ``quantize_rows`` makes such rows of weights and of activations. The reference
-has neither: its layer begins behind the norm. Checks, outputs and the autograd node
-are native (csrc/torch_ops.cpp).
+has neither: its layer begins behind the norm. Checks, outputs and the autograd
+node are native (csrc/torch_ops.cpp).
 """
 
 from __future__ import annotations
@@ -38,7 +38,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
 
     Differentiable in ``x``, ``weight`` and ``residual`` (once) where the output
     is floating; 8-bit outputs carry no gradient and refuse inputs that ask for
-    one.
+    one. A captured backward raises while a graph built on the default stream
+    still uses the same leaves.
     """
     return _lib.torch_ops().rms_norm(x, weight, residual, eps, out_dtype)
 

@@ -289,6 +289,99 @@ def test_repeats_bit_for_bit_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), rep
 
 
+def test_norm_and_layer_train_together():
+    """norm -> layer -> residual, forward and backward, as a decoder block chains
+    them: the block's gradients are the norm's backward of the layer's own, and a
+    captured step repeats them."""
+    T, E, k, H, F = 130, 6, 2, 256, 128
+    x, res, w, g = _make(T, H, BF, BF, BF, seed=11)
+    sel = torch.rand(T, E, generator=g, device="cuda").argsort(1)[:, :k].to(torch.int32).contiguous()
+    rw = torch.rand(T, k, generator=g, device="cuda")
+    gu = (torch.randn(E, H, 2 * F, generator=g, device="cuda") * H**-0.5).to(BF)
+    dn = (torch.randn(E, H, F, generator=g, device="cuda") * F**-0.5).to(BF)
+    dy = torch.randn(T, H, generator=g, device="cuda").to(BF)
+    none = torch.empty(0, device="cuda")
+    side = torch.cuda.Stream()
+
+    def step(op):
+        leaves = [t.detach().requires_grad_() for t in (x, w, res, rw, gu, dn)]
+        y, h = mega_moe.rms_norm(leaves[0], leaves[1], residual=leaves[2], eps=EPS)
+        out = h + mega_moe.MegaMoEFunction.apply(op, y, leaves[3], sel, *leaves[4:], none, None)
+        return [out, *torch.autograd.grad(out, leaves, dy)]
+
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        op = mega_moe.FusedMoEForward(None, max_tokens_per_rank=T, hidden_size=H, top_k=k, num_experts=E,
+                                      config=mega_moe.MoEForwardConfig())
+        first = [t.detach().clone() for t in step(op)]
+        # the same in two pieces: the layer's gradients from its own call, the norm's in 64 bits
+        y, h = mega_moe.rms_norm(x, w, residual=res, eps=EPS)
+        leaves = [t.detach().requires_grad_() for t in (y, rw, gu, dn)]
+        out = mega_moe.MegaMoEFunction.apply(op, leaves[0], leaves[1], sel, *leaves[2:], none, None)
+        part = torch.autograd.grad(out, leaves, dy)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first[4:], part[1:]))
+    _, hd, r, _ = _reference(x, res, w)
+    t, dyd = part[0].double() * w.double(), part[0].double()
+    dx = r * t - hd * r.pow(3) * (t * hd).mean(-1, keepdim=True) + dy.double()
+    slack = ((r * t).abs() + hd.abs() * r.pow(3) * (t * hd).abs().mean(-1, keepdim=True) + dy.double().abs()) * 2**-17
+    _check(first[1], dx, slack, BF, "dx")
+    _check(first[3], dx, slack, BF, "dresidual")
+    _check(first[2], (dyd * hd * r).sum(0), (dyd * hd * r).abs().sum(0) * 2**-13, BF, "dweight")
+    del out, leaves, y, h, part
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs = step(op)
+    for rep in range(3):
+        x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            want = [t.detach().clone() for t in step(op)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), rep
+
+
+def test_a_captured_backward_beside_an_eager_graph_is_refused():
+    """A graph built on the default stream keeps its leaves' nodes on that stream,
+    which no capture can reach: the backward raises before the hand-over, the
+    capture stays whole, and without that graph the same steps are captured."""
+    x = torch.randn(5, 264, device="cuda", requires_grad=True)
+    w = torch.rand(264, device="cuda", requires_grad=True)
+    dy = torch.randn(5, 264, device="cuda")
+    alive = mega_moe.rms_norm(x, w)
+    want = [alive.detach().clone(), *torch.autograd.grad(alive, (x, w), dy, retain_graph=True)]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        y = mega_moe.rms_norm(x, w)
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            torch.autograd.grad(y, (x, w), dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want[0])
+    del alive, y, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        y = mega_moe.rms_norm(x, w)
+        got = [y, *torch.autograd.grad(y, (x, w), dy)]
+    for _ in range(3):
+        for t in got:
+            t.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # not refused: no capture, and the eager graph alive
+    alive = mega_moe.rms_norm(x, w)
+    with torch.cuda.stream(side):
+        y = mega_moe.rms_norm(x, w)
+        got = torch.autograd.grad(y, (x, w), dy)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[1:]))
+
+
 def test_rows_past_32_bits():
     """Row offsets beyond 2^31 elements: the last rows of a 4.3 GB input."""
     rows, hidden = (1 << 20) + 3, 2056

@@ -208,3 +208,22 @@ def test_an_operator_can_be_copied_and_pickled():
     assert op._few is not None
     for other in (copy.deepcopy(op), pickle.loads(pickle.dumps(op))):
         assert other.top_k == 2 and other._few is not None and other._few is not op._few
+
+
+@built
+@pytest.mark.parametrize("call", [
+    lambda x: mega_moe.rms_norm(x),
+    lambda x: mega_moe.rms_norm(torch.zeros_like(x), x[0]),
+    lambda x: mega_moe.rms_norm(torch.zeros_like(x), residual=x),
+    lambda x: mega_moe.rms_norm(x, out_dtype=I8),
+    lambda x: mega_moe.quantize_rows(x),
+    lambda x: mega_moe.int8_matmul(torch.zeros(2, 8, dtype=I8), torch.zeros(2, 8, dtype=I8), x[:, 0].clone(), torch.ones(2)),
+    lambda x: mega_moe.int8_matmul(torch.zeros(2, 8, dtype=I8), torch.zeros(2, 8, dtype=I8), torch.ones(2), torch.ones(2),
+                                   bias=x[:, 0].clone()),
+])
+def test_forward_mode_tangents_are_refused(call):
+    """A tangent would be lost: no operator here has a forward-mode derivative."""
+    import torch.autograd.forward_ad as fwd
+
+    with fwd.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        call(fwd.make_dual(torch.ones(2, 8), torch.ones(2, 8)))
