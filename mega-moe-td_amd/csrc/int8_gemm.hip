@@ -246,11 +246,20 @@ constexpr int BK = 128;
 // which gives the 16 rows of one pass of a fragment read distinct banks.
 __device__ __forceinline__ int slot_of(int r, int s) { return r * BK + ((s ^ ((r >> 1) & 7)) << 4); }
 
-// ROWS rows of a stage: KS sub-panels of [ROWS][128], filled by NT threads.
+// ROWS rows of a stage: KS sub-panels of [ROWS][128], filled by NT threads. With
+// SHIFT a vector's fifth word is the first of the next lane's vector; only the
+// last lane of a run loads it, and words are joined on their way to LDS (128 x
+// 7169 x 4096 in 32 x 64 tiles: 21 us, 23 with five words loaded by every lane).
 template <int ROWS, int NT, int KS, bool SHIFT>
 struct Panel {
   static constexpr int VPR = 8 * KS, PER = ROWS * VPR / NT;  // 16-byte vectors a row, a thread
   static_assert(PER * NT == ROWS * VPR && NT % VPR == 0, "whole vectors");
+  // A run: consecutive lanes with consecutive vectors of a row, within the 16
+  // lanes that exchange words.
+  static constexpr int LAST = VPR < 16 ? VPR - 1 : 15;
+  struct Stage {
+    uint32_t d[PER][SHIFT ? 5 : 4];
+  };
   const char* base;
   uint32_t off[PER];
   __device__ __forceinline__ void init(const int8_t* p, int64_t ld, int r0, int rows) {
@@ -262,21 +271,49 @@ struct Panel {
       off[v] = static_cast<uint32_t>(min(c / VPR, rows - 1 - r0)) * static_cast<uint32_t>(ld) + rest + c % VPR * 16;
     }
   }
-  __device__ __forceinline__ void load(i32x4 (&r)[PER], int k) const {
-#pragma unroll
-    for (int v = 0; v < PER; ++v) r[v] = load16<SHIFT>(base + k, off[v]);
-  }
-  __device__ __forceinline__ void load_cut(i32x4 (&r)[PER], int k, int K) const {
-    const int in = threadIdx.x % VPR * 16;  // the same for all of a thread's vectors
-#pragma unroll
-    for (int v = 0; v < PER; ++v) r[v] = load16_cut(base + k, off[v], K - k - in);
-  }
-  __device__ __forceinline__ static void put(int8_t* lds, const i32x4 (&r)[PER]) {
+  __device__ __forceinline__ static bool last_of_run() { return (threadIdx.x & LAST) == LAST; }
+  __device__ __forceinline__ void load(Stage& r, int k) const {
 #pragma unroll
     for (int v = 0; v < PER; ++v) {
-      const int c = v * NT + threadIdx.x, s = c % VPR;
-      *reinterpret_cast<i32x4*>(lds + s / 8 * ROWS * BK + slot_of(c / VPR, s % 8)) = r[v];
+      if constexpr (SHIFT) {
+        const uint32_t sh = off[v] & 3;
+        const char* p = base + k + (off[v] - sh);
+        __builtin_memcpy(r.d[v], __builtin_assume_aligned(p, 4), 16);
+        if (last_of_run()) __builtin_memcpy(r.d[v] + 4, __builtin_assume_aligned(p + (sh ? 16 : 12), 4), 4);
+      } else {
+        __builtin_memcpy(r.d[v], base + k + off[v], 16);
+      }
     }
+  }
+  __device__ __forceinline__ void put(int8_t* lds, const Stage& r) const {
+#pragma unroll
+    for (int v = 0; v < PER; ++v) {
+      if constexpr (SHIFT) {
+        uint32_t d[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) d[i] = r.d[v][i];
+        const uint32_t next = __builtin_amdgcn_update_dpp(d[4], d[0], 0x101, 0xf, 0xf, false);  // of lane + 1
+        if (!last_of_run()) d[4] = next;
+        put(lds, v, join16(d, off[v] & 3));
+      } else {
+        i32x4 x;
+        __builtin_memcpy(&x, r.d[v], 16);
+        put(lds, v, x);
+      }
+    }
+  }
+  // The stage that K cuts, from memory to LDS.
+  __device__ __forceinline__ void put_cut(int8_t* lds, int k, int K) const {
+    const int in = threadIdx.x % VPR * 16;  // the same for all of a thread's vectors
+    i32x4 x[PER];
+#pragma unroll
+    for (int v = 0; v < PER; ++v) x[v] = load16_cut(base + k, off[v], K - k - in);
+#pragma unroll
+    for (int v = 0; v < PER; ++v) put(lds, v, x[v]);
+  }
+  __device__ __forceinline__ static void put(int8_t* lds, int v, const i32x4& x) {
+    const int c = v * NT + threadIdx.x, s = c % VPR;
+    *reinterpret_cast<i32x4*>(lds + s / 8 * ROWS * BK + slot_of(c / VPR, s % 8)) = x;
   }
 };
 
@@ -289,8 +326,10 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) 
   tile_of(num_m, num_n, mt, nt);
   const int m0 = mt * BM, n0 = nt * BN;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ks = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
-  Panel<BM, NT, KS, SHIFT> pa;
-  Panel<BN, NT, KS, SHIFT> pb;
+  using PanelA = Panel<BM, NT, KS, SHIFT>;
+  using PanelB = Panel<BN, NT, KS, SHIFT>;
+  PanelA pa;
+  PanelB pb;
   pa.init(p.a, p.lda, m0, p.m);
   pb.init(p.b, p.ldb, n0, p.n);
   i32x16 acc[MI][NI];
@@ -302,18 +341,19 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) 
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
   const int cut = p.k % STEP, stages = (p.k + STEP - 1) / STEP;
-  i32x4 ra[PRE][Panel<BM, NT, KS, SHIFT>::PER], rb[PRE][Panel<BN, NT, KS, SHIFT>::PER];
+  typename PanelA::Stage ra[PRE];
+  typename PanelB::Stage rb[PRE];
   // stage s > 0 begins at byte (s - 1) * STEP, or s * STEP where K cuts none
   const int shift = cut ? STEP : 0;
   if (cut) {
-    pa.load_cut(ra[0], p.k - cut, p.k);
-    pb.load_cut(rb[0], p.k - cut, p.k);
+    pa.put_cut(smem[0], p.k - cut, p.k);
+    pb.put_cut(smem[0] + BM * STEP, p.k - cut, p.k);
   } else {
     pa.load(ra[0], 0);
     pb.load(rb[0], 0);
+    pa.put(smem[0], ra[0]);
+    pb.put(smem[0] + BM * STEP, rb[0]);
   }
-  Panel<BM, NT, KS, SHIFT>::put(smem[0], ra[0]);
-  Panel<BN, NT, KS, SHIFT>::put(smem[0] + BM * STEP, rb[0]);
   // loads past the last stage repeat it (K >= STEP: there is a whole one)
   auto at = [&](int s) { return max(min(s, stages - 1) * STEP - shift, 0); };
 #pragma unroll
@@ -353,11 +393,11 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) 
       frags((kk + 1) & 1, kk < 3 ? cur : nxt, (kk + 1) & 3);
       mfmas(kk & 1);
       if (kk == 0) {
-        Panel<BM, NT, KS, SHIFT>::put(nxt, ra[R]);
+        pa.put(nxt, ra[R]);
         pa.load(ra[R], at(s + 1 + PRE));
       }
       if (kk == 1) {
-        Panel<BN, NT, KS, SHIFT>::put(nxt + BM * STEP, rb[R]);
+        pb.put(nxt + BM * STEP, rb[R]);
         pb.load(rb[R], at(s + 1 + PRE));
       }
 #pragma unroll
