@@ -12,6 +12,11 @@
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+// What results are stored in, at any alignment of their type. One value, not
+// elements: the compiler breaks an array's copy up to share it with the branch
+// for a row's end (4096 x 256 x 4096: 24 us, 18 so).
+typedef int Out4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef int Out2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMaxK = (1 << 17) - 1;
@@ -46,48 +51,44 @@ __device__ __forceinline__ float load_any(const void* p, int type, int64_t at) {
   return static_cast<float>(static_cast<const bf16*>(p)[at]);
 }
 
-// Four consecutive columns of a row, from their whole sums. Scales and bias are
-// loaded once for all of a lane's rows: fetched row by row, each store waited
-// for them (8192 x 4097 x 4096 in 256 x 256 tiles: 232 us that way, 198 this).
-struct Columns4 {
-  float sb[4], bias[4];
-  int col, left;  // columns left from col on
-  __device__ __forceinline__ Columns4(const I8Args& p, int c) : col(c), left(p.n - c) {
+// Four results in 16 bits each.
+__device__ __forceinline__ uint2 pack4(const f32x4& f, int out_type) {
+  return out_type == MM_T_FP16 ? make_uint2(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]))
+                               : make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+}
+
+// Columns col .. col + 3 of a row, from their sums.
+__device__ __forceinline__ void store4(const I8Args& p, int row, int col, const i32x4& v) {
+  const int left = p.n - col;
+  const float sa = p.sa[row];
+  f32x4 f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int at = min(c + r, p.n - 1);
-      sb[r] = p.sb[at];
-      bias[r] = p.bias ? load_any(p.bias, p.bias_type, at) : 0.0f;
-    }
+  for (int r = 0; r < 4; ++r) {
+    const int at = min(col + r, p.n - 1);
+    f[r] = static_cast<float>(v[r]) * sa * p.sb[at] + (p.bias ? load_any(p.bias, p.bias_type, at) : 0.0f);
   }
-  __device__ __forceinline__ void store(const I8Args& p, int row, float sa, const i32x4& v) const {
-    float f[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) f[r] = static_cast<float>(v[r]) * sa * sb[r] + bias[r];
-    const int64_t at = row * p.ldo + col;
-    if (p.out_type == MM_T_FP32) {
-      float* out = static_cast<float*>(p.out) + at;
-      if (left >= 4) {
-        __builtin_memcpy(out, f, 16);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 3; ++r)
-          if (r < left) out[r] = f[r];
-      }
-      return;
-    }
-    const uint2 h = p.out_type == MM_T_FP16 ? make_uint2(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]))
-                                            : make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
-    uint16_t* out = static_cast<uint16_t*>(p.out) + at;
+  const int64_t at = row * p.ldo + col;
+  if (p.out_type == MM_T_FP32) {
+    float* out = static_cast<float*>(p.out) + at;
     if (left >= 4) {
-      __builtin_memcpy(out, &h, 8);
+      *reinterpret_cast<Out4*>(out) = __builtin_bit_cast(i32x4, f);
     } else {
-      if (left > 0) out[0] = static_cast<uint16_t>(h.x);
-      if (left > 1) out[1] = static_cast<uint16_t>(h.x >> 16);
-      if (left > 2) out[2] = static_cast<uint16_t>(h.y);
+#pragma unroll
+      for (int r = 0; r < 3; ++r)
+        if (r < left) out[r] = f[r];
     }
+    return;
   }
-};
+  const uint2 h = pack4(f, p.out_type);
+  uint16_t* out = static_cast<uint16_t*>(p.out) + at;
+  if (left >= 4) {
+    *reinterpret_cast<Out2*>(out) = Out2{static_cast<int>(h.x), static_cast<int>(h.y)};
+  } else {
+    if (left > 0) out[0] = static_cast<uint16_t>(h.x);
+    if (left > 1) out[1] = static_cast<uint16_t>(h.x >> 16);
+    if (left > 2) out[2] = static_cast<uint16_t>(h.y);
+  }
+}
 
 // Sixteen bytes of a row as an operand. Rows that do not begin on 4-byte
 // borders (SHIFT) are read as the five aligned words around them and shifted:
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(W * 64) void int8_direct_kernel(I8Args p) {
 #pragma unroll
     for (int w = 1; w < W; ++w) v += red[(w * G * NT + op) * 64 + lane];
     const int row = m0 + op / G * 16 + j;
-    if (row < p.m) Columns4(p, n0 + op % G * 16 + 4 * q).store(p, row, p.sa[row], v);
+    if (row < p.m) store4(p, row, n0 + op % G * 16 + 4 * q, v);
   }
 }
 
@@ -317,6 +318,25 @@ struct Panel {
   }
 };
 
+// 32 staged rows of a wave to memory, 16 bytes a lane.
+template <int COLS, int PITCH, class T>
+__device__ __forceinline__ void store_rows(const I8Args& p, const int8_t* staged, int row0, int col0) {
+  constexpr int PER = 16 / sizeof(T), LANES = COLS / PER;  // columns a lane, lanes a row
+  const int lane = threadIdx.x & 63, r0 = lane / LANES, c = lane % LANES * PER, left = p.n - col0 - c;
+  T* out = static_cast<T*>(p.out) + (row0 + r0) * p.ldo + col0 + c;
+  const int64_t step = 64 / LANES * p.ldo;
+#pragma unroll
+  for (int r = 0; r < 32; r += 64 / LANES, out += step) {
+    if (row0 + r0 + r >= p.m) break;
+    const int8_t* from = staged + (r0 + r) * PITCH + c * sizeof(T);
+    if (left >= PER) {
+      *reinterpret_cast<Out4*>(out) = *reinterpret_cast<const i32x4*>(from);
+    } else {
+      for (int u = 0; u < left; ++u) out[u] = reinterpret_cast<const T*>(from)[u];
+    }
+  }
+}
+
 template <int BM, int BN, int WM, int WN, int KS, int PRE, bool SHIFT>
 __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) {
   constexpr int NT = WM * WN * KS * 64, STEP = KS * BK, MI = BM / WM / 32, NI = BN / WN / 32;
@@ -332,6 +352,15 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) 
   PanelB pb;
   pa.init(p.a, p.lda, m0, p.m);
   pb.init(p.b, p.ldb, n0, p.n);
+  // the tile's scales and bias, for the epilogue: a row and a channel a thread
+  __shared__ __attribute__((aligned(16))) float row_scale[BM], col_scale[BN], col_bias[BN];
+  static_assert(NT >= BM && NT >= BN, "a thread for each");
+  if (threadIdx.x < BM) row_scale[threadIdx.x] = p.sa[min(m0 + static_cast<int>(threadIdx.x), p.m - 1)];
+  if (threadIdx.x < BN) {
+    const int channel = min(n0 + static_cast<int>(threadIdx.x), p.n - 1);
+    col_scale[threadIdx.x] = p.sb[channel];
+    col_bias[threadIdx.x] = p.bias ? load_any(p.bias, p.bias_type, channel) : 0.0f;
+  }
   i32x16 acc[MI][NI];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
@@ -417,11 +446,12 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) 
     }
   }
 
-  // Epilogue, 32 rows of a wave at a time: through its own LDS (the padding
-  // keeps 16-byte writes of consecutive rows on different banks), so that
-  // neighbouring lanes store neighbouring columns.
-  constexpr int COLS = BN / WN, PITCH = COLS + 4, LANES = COLS / 4;
-  static_assert(WM * WN * 32 * PITCH * 4 <= sizeof(smem), "epilogue staging");
+  // Epilogue: sums are scaled and rounded where they lie (a lane has 4
+  // consecutive columns of one row in each quarter of a block); 32 rows of a
+  // wave at a time go through its own LDS, padded to spread a pass over the
+  // banks, so that neighbouring lanes store neighbouring 16 bytes.
+  constexpr int COLS = BN / WN, PITCH = COLS * 4 + 16, PITCH16 = COLS * 2 + 16;  // bytes of a staged row
+  static_assert(WM * WN * 32 * PITCH <= sizeof(smem), "epilogue staging");
   __syncthreads();
   if constexpr (KS > 1) {  // group 0 adds the others' sums, one group at a time
     static_assert(BM * BN * 4 <= sizeof(smem), "a group's sums");
@@ -454,24 +484,43 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) 
     }
     if (ks) return;
   }
-  i32x4* out = reinterpret_cast<i32x4*>(&smem[0][0]) + wave * (32 * PITCH / 4);
-  const int c = lane % LANES * 4;
-  const Columns4 columns(p, n0 + wn * COLS + c);
+  int8_t* const staged = &smem[0][0] + wave * (32 * PITCH);
+  const int c0 = wn * COLS, lane_row = lane & 31, lane_col = lane >> 5 << 2;
+  f32x4 sc[NI][4], bi[NI][4];
+#pragma unroll
+  for (int j = 0; j < NI; ++j)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = c0 + j * 32 + g * 8 + lane_col;
+      sc[j][g] = *reinterpret_cast<const f32x4*>(col_scale + c);
+      bi[j][g] = *reinterpret_cast<const f32x4*>(col_bias + c);
+    }
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    const int r0 = m0 + wm * (BM / WM) + i * 32;
-    const float sa = p.sa[min(r0 + (lane & 31), p.m - 1)];
+    const int r0 = wm * (BM / WM) + i * 32;
+    const float s = row_scale[r0 + lane_row];
+    // the lane's four results in quarter g of block j
+    auto results = [&](int j, int g) __attribute__((always_inline)) {
+      f32x4 f;
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
+      for (int r = 0; r < 4; ++r) f[r] = static_cast<float>(acc[i][j][4 * g + r]) * s * sc[j][g][r] + bi[j][g][r];
+      return f;
+    };
+    if (p.out_type == MM_T_FP32) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        out[((lane & 31) * PITCH + j * 32 + g * 8 + (lane >> 5) * 4) / 4] =
-            i32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-#pragma unroll 4
-    for (int k = 0; k < 32 * LANES / 64; ++k) {
-      const int r = k * (64 / LANES) + lane / LANES;
-      const float s = __shfl(sa, r);
-      if (r0 + r < p.m) columns.store(p, r0 + r, s, out[(r * PITCH + c) / 4]);
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(staged + lane_row * PITCH + (j * 32 + g * 8 + lane_col) * 4) = results(j, g);
+      store_rows<COLS, PITCH, float>(p, staged, m0 + r0, n0 + c0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<uint2*>(staged + lane_row * PITCH16 + (j * 32 + g * 8 + lane_col) * 2) =
+              pack4(results(j, g), p.out_type);
+      store_rows<COLS, PITCH16, uint16_t>(p, staged, m0 + r0, n0 + c0);
     }
   }
 }
@@ -506,8 +555,8 @@ struct TileCost {
   double round, byte;
 };
 constexpr TileCost kTileCosts[] = {
-    {256, 256, 128, 17.0, 13.3e-3}, {128, 128, 128, 4.0, 5.0e-3}, {64, 64, 128, 1.5, 1.75e-3},
-    {32, 64, 512, 2.0, 1.4e-3},     {32, 32, 1024, 2.0, 1.15e-3},
+    {256, 256, 128, 11.5, 13.3e-3}, {128, 128, 128, 3.3, 5.0e-3}, {64, 64, 128, 1.4, 1.75e-3},
+    {32, 64, 512, 1.8, 1.4e-3},     {32, 32, 1024, 1.8, 1.15e-3},
 };
 
 int best_tile(const I8Args& p) {
@@ -534,7 +583,7 @@ int launch_best(const I8Args& p, hipStream_t s) {
     case 1: return launch_tiles<128, 128, 2, 2, 1, 2, false>(p, s);
     case 2:
       // the sum shared by two groups of waves until the chip is full (256 x
-      // 7168 x 4096, 256 tiles: 19 us against 24; 464 tiles of 2309: 23 against 20)
+      // 7168 x 4096, 256 tiles: 18 us against 24; 464 tiles of 2309: 22 against 19)
       if (p.k >= 2 * BK && tiles_of(p, 64, 64) <= 256)
         return shift ? launch_tiles<64, 64, 2, 2, 2, 2, true>(p, s) : launch_tiles<64, 64, 2, 2, 2, 2, false>(p, s);
       return shift ? launch_tiles<64, 64, 2, 2, 1, 2, true>(p, s) : launch_tiles<64, 64, 2, 2, 1, 2, false>(p, s);
