@@ -492,7 +492,8 @@ __global__ __launch_bounds__(W * 64) void few_fc1_int8_kernel(FewArgs p) {
       uint32_t top = 0;  // of the bit patterns, where NaN lies above infinity
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const i32x4 gate = ws.template join<2 * G * NT>(red, g * NT + n), up = ws.template join<2 * G * NT>(red, (G + g) * NT + n);
+        const i32x4 gate = ws.template join<2 * G * NT>(red, g * NT + n);
+        const i32x4 up = ws.template join<2 * G * NT>(red, (G + g) * NT + n);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           a[g][r] = gated_act(p.act_kind, static_cast<float>(gate[r]) * (sx * sc[g * 16 + r]),

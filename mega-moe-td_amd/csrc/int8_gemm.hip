@@ -162,9 +162,11 @@ __global__ __launch_bounds__(W * 64) void int8_direct_kernel(I8Args p) {
   const char* a = aligned_base(p.a + m0 * p.lda, rest_a);
   const char* b = aligned_base(p.b + n0 * p.ldb, rest_b);
 #pragma unroll
-  for (int g = 0; g < G; ++g) b_off[g] = static_cast<uint32_t>(min(g * 16 + j, p.n - 1 - n0)) * static_cast<uint32_t>(p.ldb) + rest_b + 16 * q;
+  for (int g = 0; g < G; ++g)
+    b_off[g] = static_cast<uint32_t>(min(g * 16 + j, p.n - 1 - n0)) * static_cast<uint32_t>(p.ldb) + rest_b + 16 * q;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) a_off[n] = static_cast<uint32_t>(min(n * 16 + j, p.m - 1 - m0)) * static_cast<uint32_t>(p.lda) + rest_a + 16 * q;
+  for (int n = 0; n < NT; ++n)
+    a_off[n] = static_cast<uint32_t>(min(n * 16 + j, p.m - 1 - m0)) * static_cast<uint32_t>(p.lda) + rest_a + 16 * q;
   i32x4 acc[G][NT];
 #pragma unroll
   for (int g = 0; g < G; ++g)
@@ -345,7 +347,8 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) 
   int mt, nt;
   tile_of(num_m, num_n, mt, nt);
   const int m0 = mt * BM, n0 = nt * BN;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ks = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ks = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
   using PanelA = Panel<BM, NT, KS, SHIFT>;
   using PanelB = Panel<BN, NT, KS, SHIFT>;
   PanelA pa;
@@ -395,10 +398,12 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) 
   auto frags = [&](int set, const int8_t* buf, int kk) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
-      fa[set][i] = *reinterpret_cast<const i32x4*>(buf + ks * BM * BK + slot_of(wm * (BM / WM) + i * 32 + (lane & 31), kk * 2 + (lane >> 5)));
+      fa[set][i] = *reinterpret_cast<const i32x4*>(
+          buf + ks * BM * BK + slot_of(wm * (BM / WM) + i * 32 + (lane & 31), kk * 2 + (lane >> 5)));
 #pragma unroll
     for (int j = 0; j < NI; ++j)
-      fb[set][j] = *reinterpret_cast<const i32x4*>(buf + BM * STEP + ks * BN * BK + slot_of(wn * (BN / WN) + j * 32 + (lane & 31), kk * 2 + (lane >> 5)));
+      fb[set][j] = *reinterpret_cast<const i32x4*>(
+          buf + BM * STEP + ks * BN * BK + slot_of(wn * (BN / WN) + j * 32 + (lane & 31), kk * 2 + (lane >> 5)));
   };
   auto mfmas = [&](int set) __attribute__((always_inline)) {
 #pragma unroll

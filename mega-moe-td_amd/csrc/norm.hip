@@ -160,7 +160,8 @@ __device__ __forceinline__ uint2 quantize8(const float* v, float inv, bool e4m3)
     } else {
       w[h] = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[h] |= (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(s[i]))) & 0xffu) << (8 * i);
+      for (int i = 0; i < 4; ++i)
+        w[h] |= (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(s[i]))) & 0xffu) << (8 * i);
     }
   }
   return make_uint2(w[0], w[1]);
@@ -311,7 +312,8 @@ __global__ __launch_bounds__(WAVE ? kWaveThreads : 1024) void rms_norm_bwd_kerne
     if (p.w) wv.to_f32(p.w_type, w[u]);
   }
   int parity = 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * rpb + sub; row < p.rows; row += static_cast<int64_t>(gridDim.x) * rpb) {
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * rpb + sub; row < p.rows;
+       row += static_cast<int64_t>(gridDim.x) * rpb) {
     Vec8<TX> gv[NV];
     Vec8<TH> hv[NV], ev[NV];
 #pragma unroll
@@ -431,22 +433,31 @@ __global__ __launch_bounds__(256) void rms_norm_short_bwd_kernel(NormBwdArgs p) 
   }
 }
 
-// dw[c] = sum over the workgroups' partial rows, in order within each of 16
-// interleaved shares and then over the shares.
+// dw[c] = sum over the workgroups' partial rows, in order within each of 32
+// interleaved shares and then over the shares. A share reads a line of 32
+// columns: with 64 columns and 16 shares, half as many workgroups, 1024 partial
+// rows of 2048 columns took 4.7 us, so 4.0.
+constexpr int kSumColumns = 32, kShares = 1024 / kSumColumns;
 __global__ __launch_bounds__(1024) void dw_sum_kernel(const float* __restrict__ partial, int parts, int H, int w_type,
                                                       void* __restrict__ dw) {
-  __shared__ float lds[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6;
+  __shared__ float lds[kShares][kSumColumns];
+  const int c = blockIdx.x * kSumColumns + threadIdx.x % kSumColumns, share = threadIdx.x / kSumColumns;
   float s = 0.0f;
   if (c < H)
-#pragma unroll 8
-    for (int i = share; i < parts; i += 16) s += partial[static_cast<int64_t>(i) * H + c];
-  lds[share][threadIdx.x & 63] = s;
+    for (int i = share; i < parts; i += 8 * kShares) {  // 8 rows in flight, also the last
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        v[u] = i + u * kShares < parts ? partial[static_cast<int64_t>(i + u * kShares) * H + c] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
+  lds[share][threadIdx.x % kSumColumns] = s;
   __syncthreads();
   if (share || c >= H) return;
   s = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s += lds[i][threadIdx.x];
+  for (int i = 0; i < kShares; ++i) s += lds[i][threadIdx.x];
   if (w_type == MM_T_FP32)
     static_cast<float*>(dw)[c] = s;
   else if (w_type == MM_T_FP16)
@@ -495,13 +506,16 @@ struct LaunchFwd {
 
 // Workgroups of the backward: 16 waves of one vector a CU, or 8 of two, keep
 // the memory busy; more would only lengthen the sum over their partial rows
-// (8192 x 2048, one vector: 26 + 5 us, with half as many 31 + 4; 16384 x 1024,
-// two: 26 + 4, with twice as many 30 + 4).
+// (8192 x 2048, one vector: 26 + 4 us, with half as many 31 + 4; 16384 x 1024,
+// two: 26 + 4, with twice as many 30 + 4). All take equally many rows, so that
+// none leaves a partial row for fewer (1021 x 2305: 511 workgroups of 2 rows
+// 10.2 + 4.0 us, 819 of 1 or 2 rows 10.9 + 4.9).
 template <int NV, bool WAVE>
 int bwd_groups(int64_t rows, int threads) {
   const int rpb = WAVE ? kWaveRows : 1, waves = (WAVE ? kWaveThreads : threads) / 64;
   const int64_t need = (rows + rpb - 1) / rpb, most = 4096 / NV / waves;
-  return static_cast<int>(need < most ? need : most);
+  const int64_t each = need > most ? (need + most - 1) / most : 1;
+  return static_cast<int>((need + each - 1) / each);
 }
 
 int short_bwd_groups(int64_t rows) { return static_cast<int>((rows + 255) / 256 < 256 ? (rows + 255) / 256 : 256); }
@@ -525,7 +539,7 @@ struct LaunchBwd {
   int add_up(int groups) const {
     const int rc = mm_check_launch("rms_norm_bwd_kernel");
     if (rc || !dw) return rc;
-    dw_sum_kernel<<<(p.hidden + 63) / 64, 1024, 0, s>>>(p.partial, groups, p.hidden, p.w_type, dw);
+    dw_sum_kernel<<<(p.hidden + kSumColumns - 1) / kSumColumns, 1024, 0, s>>>(p.partial, groups, p.hidden, p.w_type, dw);
     return mm_check_launch("dw_sum_kernel");
   }
 };
@@ -603,7 +617,7 @@ extern "C" int mm_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int
   const hipStream_t s = mm_hip_stream(stream);
   if (rows == 0) {  // no rows: the weight's gradient is an empty sum
     if (!dweight) return MM_OK;
-    dw_sum_kernel<<<(hidden + 63) / 64, 1024, 0, s>>>(nullptr, 0, hidden, weight_type, dweight);
+    dw_sum_kernel<<<(hidden + kSumColumns - 1) / kSumColumns, 1024, 0, s>>>(nullptr, 0, hidden, weight_type, dweight);
     return mm_check_launch("dw_sum_kernel");
   }
   const NormBwdArgs p{dy,   dh,   h,   weight, rstd,   dx, dresidual, dweight ? static_cast<float*>(workspace) : nullptr,

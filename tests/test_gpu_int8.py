@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import mega_moe
+from mega_moe import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -146,9 +147,29 @@ def test_streams_and_graphs(m):
         assert torch.equal(out, mega_moe.int8_matmul(a, b, sa, sb)), rep
 
 
-def test_outputs_past_32_bits():
+@pytest.mark.parametrize("dtype,code,bias", [(BF, 0, F16), (F16, 1, None), (F32, 2, F32)])
+@pytest.mark.parametrize("m,n,k", [
+    (9, 203, 700), (33, 203, 96), (40, 4003, 4100), (40, 4003, 4101), (130, 4003, 2052), (130, 4003, 2053), (300, 1003, 1000),
+    (300, 1003, 1001), (1021, 1795, 2308), (1021, 1795, 2309), (1501, 2003, 300), (4091, 4099, 640)])
+def test_padded_outputs(m, n, k, dtype, code, bias):
+    """The C entry with output rows that are padded, at odd strides: what lies
+    between the rows stays as it was."""
+    a, b, sa, sb = _operands(m, n, k, seed=3)
+    bias = None if bias is None else torch.randn(n, device="cuda").to(bias)
+    want = mega_moe.int8_matmul(a, b, sa, sb, bias=bias, out_dtype=dtype)
+    _check(want, a, b, sa, sb, bias, dtype)
+    for pad in (1, 6):
+        out = torch.full((m + 1, n + pad), 7.0, device="cuda", dtype=dtype)
+        _lib.call("mm_int8_matmul", _lib.ptr(a), k, _lib.ptr(b), k, _lib.ptr(sa), _lib.ptr(sb), _lib.ptr(bias),
+                  0 if bias is None else _lib.ELEMENT_TYPES[bias.dtype], m, n, k, _lib.ptr(out), n + pad, code,
+                  torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(out[:m, :n], want) and (out[:, n:] == 7).all() and (out[m] == 7).all()
+
+
+@pytest.mark.parametrize("k", [64, 132])  # operands from memory, and the largest tiles
+def test_outputs_past_32_bits(k):
     """An output of more than 2^31 elements: its last row and column."""
-    m, n, k = 70000, 32768, 64
+    m, n = 70000, 32768
     a, b, sa, sb = _operands(m, n, k)
     out = mega_moe.int8_matmul(a, b, sa, sb)
     _check(out[-5:], a[-5:], b, sa[-5:], sb, None, BF)
