@@ -555,22 +555,26 @@ int launch_tiles(const I8Args& p, hipStream_t s) {
 // Time of a product in us by its tiles: every 256 of them take `round` + `byte`
 // a byte of K, as measured on full rounds (and about 4 us in all). Tiles below
 // 64 x 64 gain from the bytes they have in flight while the chip is not full.
+// 128 x 64 tiles fill a CU's LDS alone and are for one round (512 x 7168 x
+// 4096: 27 us, in 64 x 64 33; 968 x 4992 x 6016, two: 64 us, in 128 x 128 48).
 struct TileCost {
   int bm, bn, step;  // step: K has to reach one whole stage
   double round, byte;
+  int rounds = 1 << 30;  // for so many
 };
 constexpr TileCost kTileCosts[] = {
-    {256, 256, 128, 11.5, 13.3e-3}, {128, 128, 128, 3.3, 5.0e-3}, {64, 64, 128, 1.4, 1.75e-3},
-    {32, 64, 512, 1.8, 1.4e-3},     {32, 32, 1024, 1.8, 1.15e-3},
+    {256, 256, 128, 11.5, 13.3e-3}, {128, 128, 128, 3.3, 5.0e-3}, {128, 64, 256, 4.0, 2.9e-3, 1},
+    {64, 64, 128, 1.4, 1.75e-3},    {32, 64, 512, 1.8, 1.4e-3},   {32, 32, 1024, 1.8, 1.15e-3},
 };
 
 int best_tile(const I8Args& p) {
   int best = 0;
   double least = 1e300;
-  for (int i = 0; i < 5; ++i) {
+  for (int i = 0; i < 6; ++i) {
     const TileCost& c = kTileCosts[i];
-    const double t = static_cast<double>((tiles_of(p, c.bm, c.bn) + 255) / 256) * (c.round + c.byte * p.k);
-    if (p.k >= c.step && t < least) best = i, least = t;
+    const int64_t rounds = (tiles_of(p, c.bm, c.bn) + 255) / 256;
+    const double t = static_cast<double>(rounds) * (c.round + c.byte * p.k);
+    if (p.k >= c.step && rounds <= c.rounds && t < least) best = i, least = t;
   }
   return best;
 }
@@ -587,12 +591,14 @@ int launch_best(const I8Args& p, hipStream_t s) {
     case 0: return launch_tiles<256, 256, 2, 2, 1, 1, false>(p, s);
     case 1: return launch_tiles<128, 128, 2, 2, 1, 2, false>(p, s);
     case 2:
+      return shift ? launch_tiles<128, 64, 2, 2, 2, 2, true>(p, s) : launch_tiles<128, 64, 2, 2, 2, 2, false>(p, s);
+    case 3:
       // the sum shared by two groups of waves until the chip is full (256 x
       // 7168 x 4096, 256 tiles: 18 us against 24; 464 tiles of 2309: 22 against 19)
       if (p.k >= 2 * BK && tiles_of(p, 64, 64) <= 256)
         return shift ? launch_tiles<64, 64, 2, 2, 2, 2, true>(p, s) : launch_tiles<64, 64, 2, 2, 2, 2, false>(p, s);
       return shift ? launch_tiles<64, 64, 2, 2, 1, 2, true>(p, s) : launch_tiles<64, 64, 2, 2, 1, 2, false>(p, s);
-    case 3: return shift ? launch_tiles<32, 64, 1, 2, 4, 2, true>(p, s) : launch_tiles<32, 64, 1, 2, 4, 2, false>(p, s);
+    case 4: return shift ? launch_tiles<32, 64, 1, 2, 4, 2, true>(p, s) : launch_tiles<32, 64, 1, 2, 4, 2, false>(p, s);
     default: return shift ? launch_tiles<32, 32, 1, 1, 8, 1, true>(p, s) : launch_tiles<32, 32, 1, 1, 8, 1, false>(p, s);
   }
 }

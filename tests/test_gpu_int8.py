@@ -150,7 +150,8 @@ def test_streams_and_graphs(m):
 @pytest.mark.parametrize("dtype,code,bias", [(BF, 0, F16), (F16, 1, None), (F32, 2, F32)])
 @pytest.mark.parametrize("m,n,k", [
     (9, 203, 700), (33, 203, 96), (40, 4003, 4100), (40, 4003, 4101), (130, 4003, 2052), (130, 4003, 2053), (300, 1003, 1000),
-    (300, 1003, 1001), (1021, 1795, 2308), (1021, 1795, 2309), (1501, 2003, 300), (4091, 4099, 640)])
+    (300, 1003, 1001), (1021, 1795, 2308), (1021, 1795, 2309), (520, 1795, 700),
+    (520, 1795, 701), (120, 4095, 2052), (120, 4095, 2053), (1501, 2003, 300), (4091, 4095, 1281)])
 def test_padded_outputs(m, n, k, dtype, code, bias):
     """The C entry with output rows that are padded, at odd strides: what lies
     between the rows stays as it was."""

@@ -8,7 +8,7 @@ Tolerances (relative to the sums of absolute terms, counted in 64 bits):
   * the backward's dot product has the same depth on terms of either sign: its
     error is 2^-18 of the sum of the absolute terms; with the products around
     it 2^-17 of |r w dy| + |h| r^3 mean|w dy h| + |dh|;
-  * dweight adds a thread's rows (under 2^10 here), 4 waves, 64 shares and 16:
+  * dweight adds a thread's rows (under 2^10 here), 4 waves, 32 of a share and 32 shares:
     2^-13 of the sum of the absolute terms bounds it;
   * each output is rounded once: half a step, or half the smallest subnormal.
 """
