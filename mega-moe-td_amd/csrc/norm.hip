@@ -4,7 +4,7 @@
 //   h = round(x + residual)          (h = x without a residual)
 //   y = h * r * w,  r = 1 / sqrt(mean(h^2) + eps)
 //   8 bits: s = max(a, 1e-30) / Q with a = max |y| over the row (s = 1 where
-//           a = 0), q = round(y / s); Q = 127 (int8) or 448 (E4M3)
+//           a = 0), q = round(y / s) of the unrounded y; Q = 127 (int8) or 448 (E4M3)
 //   backward: dx = dh + r w dy - h r^3 mean(w dy h),  dw = sum_rows dy h r
 //
 // The norm is taken of h as it is stored, so that the backward (which reads h)
@@ -145,15 +145,49 @@ __device__ __forceinline__ uint32_t row_umax(uint32_t v, uint32_t* lds) {
   return v;
 }
 
-// 8 values into int8 or E4M3 (round to nearest even; |v| stays below the
-// largest value's rounding border, so neither saturates).
-__device__ __forceinline__ uint2 quantize8(const float* v, float inv, bool e4m3) {
+// Rows in 8 bits. r = mant * pow2 with 1 <= mant < 2, and a row's values are
+// held as t = h pow2 w = y / mant: for 16-bit h and w that is exact, and mant
+// drops out of the quotient y / s = t Q / max |t|. Quotients that lie on a
+// rounding border exactly, about 1 in 10^4 of them, thus come out exact and
+// round to even; a rounded y would send them either way.
+struct Rsqrt {
+  float mant, pow2;
+  __device__ __forceinline__ explicit Rsqrt(float r)  // of 0 and infinity: 1 and itself
+      : mant(__uint_as_float((__float_as_uint(r) & 0x007fffffu) | 0x3f800000u)),
+        pow2(__uint_as_float(__float_as_uint(r) & 0x7f800000u)) {}
+};
+
+struct Quantizer {
+  float top, most, inv, fix, scale;
+  bool finite;
+  // bits: largest |t| as a bit pattern, where NaN lies above infinity, so that a
+  // row that holds either shows it
+  __device__ __forceinline__ Quantizer(uint32_t bits, float mant, bool e4m3) : top(__uint_as_float(bits)) {
+    const float q = e4m3 ? kFp8Max : 127.0f, a = top * mant;
+    const bool small = a < kScaleFloor, large = top > 1e30f;  // Q / top, t Q would leave the range
+    finite = a < __builtin_inff();
+    most = large ? 1.0f : q;
+    inv = small ? mant / kScaleFloor : large ? q / top : 1.0f / top;
+    fix = small || large ? 0.0f : inv;
+    scale = !finite ? __uint_as_float(0x7fc00000u) : bits == 0 ? 1.0f : fmaxf(a, kScaleFloor) / q;
+  }
+  // t Q / top: one correction of the quotient makes it exact where it is
+  // representable. |value| stays below the border of the largest, so neither
+  // type saturates.
+  __device__ __forceinline__ float value(float t) const {
+    const float p = t * most, q = p * inv;
+    return fmaf(fmaf(-q, top, p), fix, q);
+  }
+};
+
+// 8 values into int8 or E4M3, round to nearest even.
+__device__ __forceinline__ uint2 quantize8(const float* v, const Quantizer& z, bool e4m3) {
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float s[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = v[4 * h + i] * inv;
+    for (int i = 0; i < 4; ++i) s[i] = z.value(v[4 * h + i]);
     if (e4m3) {
       int d = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
       w[h] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], d, true));
@@ -203,6 +237,8 @@ __global__ __launch_bounds__(WAVE ? kWaveThreads : 1024) void rms_norm_kernel(No
         h.to_f32(v[u]);
       }
     }
+    const bool eight = p.y_type == MM_T_INT8 || p.y_type == MM_T_E4M3;
+    float mant = 1.0f;
     if (p.norm) {
       float ss = 0.0f;
 #pragma unroll
@@ -211,8 +247,13 @@ __global__ __launch_bounds__(WAVE ? kWaveThreads : 1024) void rms_norm_kernel(No
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss += c.counts(i) ? v[u][i] * v[u][i] : 0.0f;
       }
-      const float r = rsqrtf(row_sum<WAVE>(ss, sums) / static_cast<float>(H) + p.eps);
+      float r = rsqrtf(row_sum<WAVE>(ss, sums) / static_cast<float>(H) + p.eps);
       if (p.rstd && t == 0) p.rstd[row] = r;
+      if (eight) {
+        const Rsqrt split(r);
+        mant = split.mant;
+        r = split.pow2;
+      }
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
         float w[8];
@@ -221,7 +262,7 @@ __global__ __launch_bounds__(WAVE ? kWaveThreads : 1024) void rms_norm_kernel(No
         for (int i = 0; i < 8; ++i) v[u][i] *= p.w ? r * w[i] : r;
       }
     }
-    if (p.y_type != MM_T_INT8 && p.y_type != MM_T_E4M3) {
+    if (!eight) {
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
         const Columns c(u * threads + t, H);
@@ -229,22 +270,18 @@ __global__ __launch_bounds__(WAVE ? kWaveThreads : 1024) void rms_norm_kernel(No
       }
       continue;
     }
-    // The maximum is taken of the bit patterns: NaN lies above infinity there,
-    // so a row that holds either shows it.
     uint32_t top = 0;
 #pragma unroll
     for (int u = 0; u < NV; ++u)
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[u][i]) & 0x7fffffffu);
-    top = row_umax<WAVE>(top, tops);
-    const bool e4m3 = p.y_type == MM_T_E4M3, finite = top < 0x7f800000u;
-    const float most = e4m3 ? kFp8Max : 127.0f, a = fmaxf(__uint_as_float(top), kScaleFloor);
-    if (t == 0) p.scale[row] = !finite ? __uint_as_float(0x7fc00000u) : top == 0 ? 1.0f : a / most;
-    const float inv = most / a;
+    const bool e4m3 = p.y_type == MM_T_E4M3;
+    const Quantizer z(row_umax<WAVE>(top, tops), mant, e4m3);
+    if (t == 0) p.scale[row] = z.scale;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const Columns c(u * threads + t, H);
-      const uint2 q = finite ? quantize8(v[u], inv, e4m3) : make_uint2(0, 0);
+      const uint2 q = z.finite ? quantize8(v[u], z, e4m3) : make_uint2(0, 0);
       if (c.any()) __builtin_memcpy(static_cast<uint8_t*>(p.y) + row * H + c.at, &q, 8);
     }
   }
@@ -266,12 +303,19 @@ __global__ __launch_bounds__(256) void rms_norm_short_kernel(NormArgs p) {
       }
       ss += v[i] * v[i];
     }
+    const bool eight = p.y_type == MM_T_INT8 || p.y_type == MM_T_E4M3;
+    float mant = 1.0f;
     if (p.norm) {
-      const float r = rsqrtf(ss / static_cast<float>(H) + p.eps);
+      float r = rsqrtf(ss / static_cast<float>(H) + p.eps);
       if (p.rstd) p.rstd[row] = r;
+      if (eight) {
+        const Rsqrt split(r);
+        mant = split.mant;
+        r = split.pow2;
+      }
       for (int i = 0; i < H; ++i) v[i] *= p.w ? r * load_any(p.w, p.w_type, i) : r;
     }
-    if (p.y_type != MM_T_INT8 && p.y_type != MM_T_E4M3) {
+    if (!eight) {
       for (int i = 0; i < H; ++i) static_cast<TX*>(p.y)[row * H + i] = static_cast<TX>(v[i]);
       continue;
     }
@@ -280,10 +324,10 @@ __global__ __launch_bounds__(256) void rms_norm_short_kernel(NormArgs p) {
       if (i >= H) v[i] = 0.0f;
       top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
     }
-    const bool e4m3 = p.y_type == MM_T_E4M3, finite = top < 0x7f800000u;
-    const float most = e4m3 ? kFp8Max : 127.0f, a = fmaxf(__uint_as_float(top), kScaleFloor);
-    p.scale[row] = !finite ? __uint_as_float(0x7fc00000u) : top == 0 ? 1.0f : a / most;
-    const uint2 q = finite ? quantize8(v, most / a, e4m3) : make_uint2(0, 0);
+    const bool e4m3 = p.y_type == MM_T_E4M3;
+    const Quantizer z(top, mant, e4m3);
+    p.scale[row] = z.scale;
+    const uint2 q = z.finite ? quantize8(v, z, e4m3) : make_uint2(0, 0);
     for (int i = 0; i < H; ++i)
       static_cast<uint8_t*>(p.y)[row * H + i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
   }

@@ -112,6 +112,27 @@ def test_quantize_rows(shape, dtype):
     _check_rows8(q, scale, x.double(), dtype, 127.0 if dtype == torch.int8 else 448.0)
 
 
+@pytest.mark.parametrize("hidden", [7, 64, 515, 2048, 7168, 16384])
+@pytest.mark.parametrize("weight", [None, BF, F32])
+def test_borders_round_to_even(hidden, weight):
+    """Quotients that lie on a rounding border exactly, whatever the row's rms:
+    whole numbers up to 254 in int8 (a scale of 2 times the row's), up to 448 in
+    E4M3 (of 1). The weight's 1.5 is in every value and drops out."""
+    g = torch.Generator(device="cuda").manual_seed(hidden)
+    rows = 33
+    w = None if weight is None else torch.full((hidden,), 1.5, dtype=weight, device="cuda")
+    scale = 2.0 ** torch.randint(-9, 9, (rows, 1), generator=g, device="cuda")  # another rms a row
+    for out, top, want in ((torch.int8, 254, lambda n: (n / 2).round()), (E4M3, 448, lambda n: n.to(E4M3).float())):
+        n = torch.randint(-top, top + 1, (rows, hidden), generator=g, device="cuda").float()
+        if out == E4M3:
+            n = n.to(BF).float().clamp(-top, top)  # 8 bits: borders of 4 among them
+        n[:, hidden // 2] = -top
+        q, s = mega_moe.rms_norm((n * scale).to(BF), w, eps=EPS, out_dtype=out)
+        assert torch.equal(q.float(), want(n))
+        q, s = mega_moe.quantize_rows((n * scale).to(BF), out)
+        assert torch.equal(q.float(), want(n)) and torch.equal(s, scale[:, 0] * (2 if out == torch.int8 else 1))
+
+
 def test_tiny_rows_keep_their_scale_normal():
     x = torch.full((2, 64), 1e-37, device="cuda")
     x[1] = 1e-28
