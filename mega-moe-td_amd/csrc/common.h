@@ -154,13 +154,17 @@ __device__ __forceinline__ float mm_tanh(float x) {
   return 2.0f * mm_sigmoid(2.0f * x) - 1.0f;
 }
 
+// The clamp selects instead of taking a minimum, which would drop NaN.
+__device__ __forceinline__ float clamp_above(float x, float most) { return x > most ? most : x; }
+__device__ __forceinline__ float clamp_both(float x, float most) { return x < -most ? -most : clamp_above(x, most); }
+
 __device__ __forceinline__ float gated_act(int kind, float g, float u, float beta, float lbeta,
                                            float clamp_limit) {
   if (kind == MM_ACT_SWIGLU) {
     return (g * mm_sigmoid(g)) * u;
   } else if (kind == MM_ACT_CLAMP_SWIGLU) {
-    float gc = fminf(g, clamp_limit);
-    float uc = fminf(fmaxf(u, -clamp_limit), clamp_limit);
+    float gc = clamp_above(g, clamp_limit);
+    float uc = clamp_both(u, clamp_limit);
     return (gc * mm_sigmoid(gc)) * uc;
   } else {
     float a = beta * mm_tanh(g / beta) * mm_sigmoid(g);

@@ -1,0 +1,80 @@
+"""NaN and infinities through the gated activations on the GPU.
+
+The clamp of ``clamp_swiglu`` keeps NaN (torch's ``clamp`` does, and the
+oracle's), so a token whose row holds one comes out NaN under every activation
+and the other tokens keep their bits."""
+
+import pytest
+import torch
+
+import mega_moe
+
+pytestmark = pytest.mark.gpu
+
+BF, F32, I8 = torch.bfloat16, torch.float32, torch.int8
+NAN, INF = float("nan"), float("inf")
+E, K, H, F, T = 4, 2, 256, 128, 12
+ACTS = [("swiglu", {}), ("clamp_swiglu", dict(clamp_limit=1.5)), ("situglu", dict(situ_beta=2.0)),
+        ("situglu", dict(situ_beta=2.0, situ_linear_beta=3.0))]
+
+
+def _operator(act, kw):
+    cfg = mega_moe.MoEForwardConfig(activation=act, **kw)
+    return mega_moe.FusedMoEForward(None, max_tokens_per_rank=64, hidden_size=H, top_k=K, num_experts=E, config=cfg)
+
+
+def _layer(seed=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    sel = torch.rand(T, E, generator=g, device="cuda").argsort(1)[:, :K].to(torch.int32).contiguous()
+    rw = torch.rand(T, K, generator=g, device="cuda") + 0.1
+    return rnd(T, H).to(BF), sel, (rnd(E, H, 2 * F) * H**-0.5).to(BF), (rnd(E, H, F) * F**-0.5).to(BF), rw
+
+
+def _int8_layer(seed=2):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r8 = lambda *s: torch.randint(-127, 128, s, generator=g, device="cuda", dtype=I8)
+    sc = lambda *s: torch.rand(*s, generator=g, device="cuda") + 0.5
+    ex = mega_moe.Int8Experts(r8(E, 2 * F, H), sc(E, 2 * F) * H**-0.5 / 74, r8(E, H, F), sc(E, H) * F**-0.5 / 74)
+    return r8(T, H), sc(T) / 74, ex
+
+
+def _others_kept(got, want, bad):
+    keep = [t for t in range(T) if t not in bad]
+    assert torch.equal(got[keep], want[keep]) and torch.isfinite(want).all()
+    for t in bad:
+        assert torch.isnan(got[t]).all(), (t, got[t].float().abs().max())
+
+
+@pytest.mark.parametrize("act,kw", ACTS)
+@pytest.mark.parametrize("entry", ["forward", "forward_few"])
+def test_nan_rows(entry, act, kw):
+    x, sel, gu, dn, rw = _layer()
+    op = _operator(act, kw)
+    run = getattr(op, entry)
+    want = run(x, sel, gu, dn, rw).clone()
+    bad = x.clone()
+    bad[5, 3], bad[7] = NAN, NAN
+    _others_kept(run(bad, sel, gu, dn, rw), want, (5, 7))
+
+
+@pytest.mark.parametrize("act,kw", ACTS)
+def test_nan_scales(act, kw):
+    _, sel, _, _, rw = _layer()
+    xq, xs, ex = _int8_layer()
+    op = _operator(act, kw)
+    want = op.forward_few_int8(xq, xs, sel, ex, rw)
+    xs[2] = NAN
+    _others_kept(op.forward_few_int8(xq, xs, sel, ex, rw), want, (2,))
+
+
+@pytest.mark.parametrize("act,kw", ACTS)
+def test_a_broken_row_through_norm_and_layer(act, kw):
+    """The norm marks a row that holds an infinity by its scale; the layer keeps the mark."""
+    x, sel, _, _, rw = _layer()
+    _, _, ex = _int8_layer()
+    op = _operator(act, kw)
+    x[4, 9] = INF
+    q, s = mega_moe.rms_norm(x, out_dtype=I8)
+    out = op.forward_few_int8(q, s, sel, ex, rw)
+    assert torch.isnan(out[4]).all() and torch.isfinite(out[[t for t in range(T) if t != 4]]).all()
