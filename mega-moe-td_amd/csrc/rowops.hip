@@ -159,8 +159,8 @@ __device__ __forceinline__ void act_pair(int kind, float a, float b, float beta,
     v = b;
     dv = 1.0f;
   } else if (kind == MM_ACT_CLAMP_SWIGLU) {
-    const float gc = fminf(a, L);
-    const float uc = fminf(fmaxf(b, -L), L);
+    const float gc = clamp_above(a, L);
+    const float uc = clamp_both(b, L);
     const float s = mm_sigmoid(gc);
     act_a = gc * s;
     dact_a = (s + gc * s * (1.0f - s)) * (a <= L ? 1.0f : 0.0f);

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import mega_moe
+from oracle import moe_oracle as O
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +79,47 @@ def test_a_broken_row_through_norm_and_layer(act, kw):
     q, s = mega_moe.rms_norm(x, out_dtype=I8)
     out = op.forward_few_int8(q, s, sel, ex, rw)
     assert torch.isnan(out[4]).all() and torch.isfinite(out[[t for t in range(T) if t != 4]]).all()
+
+
+@pytest.mark.parametrize("act,kw", ACTS)
+def test_nan_in_the_backward(act, kw):
+    """A NaN token's gradients are NaN as the oracle's derivative pair has them;
+    the other tokens' keep their bits."""
+    x, sel, gu, dn, rw = _layer()
+    dy = torch.randn(T, H, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(BF)
+    op = _operator(act, kw)
+    bad = x.clone()
+    bad[5, 3] = NAN
+    grads = []
+    for rows in (x, bad):
+        _, saved = op.forward(rows, sel, gu, dn, rw, return_saved=True)
+        g = mega_moe.moe_backward_triton(saved, dy)
+        grads.append((g["grad_hidden"].clone(), g["grad_routing_weights"].clone()))
+    for want, got in zip(*grads):
+        _others_kept(got, want, (5,))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "fp16"])
+def test_derivative_pair_keeps_nan(fmt):
+    """Element for element: NaN where the oracle's clamp derivatives are NaN."""
+    from mega_moe.ops import _kernels as KS
+
+    torch.manual_seed(4)
+    rows, inter, limit = 3, 128, 1.5
+    dt = BF if fmt == "bf16" else torch.float16
+    gu = torch.randn(rows, 2 * inter, device="cuda").mul_(2).to(dt)
+    gu[0, 3], gu[1, inter + 5], gu[2, 7], gu[2, inter + 7] = NAN, NAN, NAN, NAN
+    dc = torch.randn(rows, inter, device="cuda").to(BF)
+    offs = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    scale = torch.ones(rows, device="cuda")
+    dab, dscale = KS.swiglu_bwd(dc, gu, scale, offs, rows, "clamp_swiglu", 1.0, None, limit)
+    torch.cuda.synchronize()
+    g, u, d = gu[:, :inter].double().cpu(), gu[:, inter:].double().cpu(), dc.double().cpu()
+    a, da, v, dv = O.gated_act_grad(g, u, "clamp_swiglu", clamp_limit=limit)
+    ref = torch.cat([d * da * v, d * a * dv], dim=1)
+    got = dab[:rows].double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    # exp and reciprocal good to 2^-16, one rounding to bf16; dact sums two terms of one size
+    fine = ~torch.isnan(ref)
+    assert ((got - ref).abs()[fine] <= ref.abs()[fine] * 2**-8 + d.abs().repeat(1, 2)[fine] * 4 * 2**-14).all()
+    assert torch.isnan(dscale[:rows]).all()
