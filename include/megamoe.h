@@ -407,7 +407,9 @@ int mm_moe_few(const uint16_t* x, const int32_t* selected,
  * contiguous. Products are summed in int32. The activation (fp32, times the
  * routing weight) is rounded to int8 in groups of MM_FEW_ACT_GROUP columns
  * with scale = max |act| / 127 of the group; FC2 sums a group in int32 and the
- * groups in fp32. Scratch of mm_moe_few_scratch_bytes with int8 = 1.
+ * groups in fp32. A row whose x_scale is NaN or infinite is NaN in act, and so
+ * in out where a slot of it has an expert. Scratch of mm_moe_few_scratch_bytes
+ * with int8 = 1.
  */
 int mm_moe_few_int8(const int8_t* x, const float* x_scale,
                     const int32_t* selected, const float* routing_weights,

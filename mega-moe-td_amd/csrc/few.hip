@@ -486,7 +486,9 @@ __global__ __launch_bounds__(W * 64) void few_fc1_int8_kernel(FewArgs p) {
     // one wave joins a block of 16 tokens
     for (int n = ws.wave; n < NT; n += W) {
       const int at = c0 + n * 16 + j, route = list[min(at, wk.count - 1)];
-      const float sx = p.x_scale[route / p.top_k], wt = p.w[route];
+      // an infinite scale marks a broken row as NaN does; a clamp or a tanh would hide it
+      const float mark = p.x_scale[route / p.top_k], wt = p.w[route];
+      const float sx = fabsf(mark) < __builtin_inff() ? mark : __uint_as_float(0x7fc00000u);
       const float* sc = p.w1_scale + static_cast<int64_t>(wk.expert) * 2 * p.I + col + 4 * q;
       float a[G][4];
       uint32_t top = 0;  // of the bit patterns, where NaN lies above infinity

@@ -432,7 +432,8 @@ class FusedMoEForward(torch.nn.Module):
         ``quantize_rows`` make them; returns bf16 [T, H]. The products are summed
         in int32; between them the activation (times the routing weight) is
         rounded to int8 in groups of 32 columns with the group's largest value
-        at 127. A NaN or infinite scale makes its own token's output NaN.
+        at 127. A NaN or infinite scale makes its own token's output NaN (where
+        any slot of the token has an expert) and no other's.
         """
         if not isinstance(experts, Int8Experts):
             raise TypeError("experts must be an Int8Experts")

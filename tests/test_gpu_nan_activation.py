@@ -123,3 +123,16 @@ def test_derivative_pair_keeps_nan(fmt):
     fine = ~torch.isnan(ref)
     assert ((got - ref).abs()[fine] <= ref.abs()[fine] * 2**-8 + d.abs().repeat(1, 2)[fine] * 4 * 2**-14).all()
     assert torch.isnan(dscale[:rows]).all()
+
+
+@pytest.mark.parametrize("bad", [INF, -INF])
+@pytest.mark.parametrize("act,kw", ACTS)
+def test_infinite_scales(act, kw, bad):
+    """A row's scale is finite or marks the row as broken, also where the
+    activation saturates (clamp, tanh) and would hide an infinity."""
+    _, sel, _, _, rw = _layer()
+    xq, xs, ex = _int8_layer()
+    op = _operator(act, kw)
+    want = op.forward_few_int8(xq, xs, sel, ex, rw)
+    xs[2], xs[9] = bad, bad
+    _others_kept(op.forward_few_int8(xq, xs, sel, ex, rw), want, (2, 9))
