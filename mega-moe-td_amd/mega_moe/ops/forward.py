@@ -129,7 +129,8 @@ class FusedMoEForward(torch.nn.Module):
         self._routing_generation = 0
         self._forward_stream = None
         self._device = None
-        self._few = None  # the native description of the layer for a few tokens
+        self._few = None  # the native description of the layer for a few tokens,
+        self._few_of = None  # and the attributes that it was made of
         # optional runtime.timing.StageTimer: HIP events between stages
         # (MOE_FWD_TIMING=1 attaches one, as the reference's phase stamps are
         # switched on by that variable, ops/forward.py:1656-1660)
@@ -386,11 +387,11 @@ class FusedMoEForward(torch.nn.Module):
         the latter where ``rows`` are not on the operator's device, which is that
         of the first call."""
         ops = _lib.torch_ops()
-        if self._few is None:
-            lbeta = self.situ_linear_beta
-            self._few = ops.Layer(min(MAX_FEW_TOKENS, self.max_tokens_per_rank), self.top_k, self.experts_per_rank,
-                                  self.hidden_size, _lib.ACT_KINDS[self.activation], self.situ_beta,
-                                  0.0 if lbeta is None else lbeta, self.clamp_limit)
+        lbeta = self.situ_linear_beta
+        of = (min(MAX_FEW_TOKENS, self.max_tokens_per_rank), self.top_k, self.experts_per_rank, self.hidden_size,
+              _lib.ACT_KINDS[self.activation], self.situ_beta, 0.0 if lbeta is None else lbeta, self.clamp_limit)
+        if of != self._few_of:  # the attributes may change between calls, as forward reads them at each
+            self._few, self._few_of = ops.Layer(*of), of
         if self._device is None and rows.is_cuda:
             self._device = rows.device
         return ops, self._few if rows.device == self._device else None
