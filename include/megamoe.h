@@ -404,9 +404,9 @@ int mm_moe_few(const uint16_t* x, const int32_t* selected,
  * mm_moe_few on int8 rows and int8 experts: x [tokens, hidden] with x_scale
  * [tokens], w1 [E, 2 inter, hidden] (gate rows, then up rows) with w1_scale
  * [E, 2 inter], w2 [E, hidden, inter] with w2_scale [E, hidden], all
- * contiguous. Products are summed in int32. The activation (fp32, times the
- * routing weight) is rounded to int8 in groups of MM_FEW_ACT_GROUP columns
- * with scale = max |act| / 127 of the group; FC2 sums a group in int32 and the
+ * contiguous, hidden below 2^17. Products are summed in int32. The activation
+ * (fp32, times the routing weight) is rounded to int8 in groups of
+ * MM_FEW_ACT_GROUP columns with scale = max |act| / 127 of the group; FC2 sums a group in int32 and the
  * groups in fp32. A row whose x_scale is NaN or infinite is NaN in act, and so
  * in out where a slot of it has an expert. Scratch of mm_moe_few_scratch_bytes
  * with int8 = 1.

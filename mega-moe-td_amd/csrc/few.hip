@@ -29,6 +29,7 @@ constexpr float kScaleFloor = 1e-30f;
 // (2 H), and the activation's routes (checked with the sizes)
 constexpr int kMaxDim = 1 << 20;
 constexpr int64_t kMaxStride = int64_t(1) << 25;  // and 24 rows of w2
+constexpr int kMaxInt8Hidden = (1 << 17) - 1;      // an int32 sum of products of -128 and -128
 
 struct FewArgs {
   const void* x;              // [T, H] bf16 or int8
@@ -608,10 +609,10 @@ struct FewScratch {
   }
 };
 
-bool few_sizes_ok(int64_t tokens, int32_t top_k, int32_t E, int32_t H, int32_t I) {
+bool few_sizes_ok(int64_t tokens, int32_t top_k, int32_t E, int32_t H, int32_t I, bool int8) {
   return tokens >= 0 && tokens <= MM_FEW_MAX_TOKENS && top_k > 0 && top_k <= 64 && E > 0 && E <= 32768 && H > 0 &&
-         H % 128 == 0 && I > 0 && I % 128 == 0 && H <= kMaxDim && I <= kMaxDim &&
-         tokens * top_k * I < (int64_t(1) << 31);
+         H % 128 == 0 && I > 0 && I % 128 == 0 && H <= (int8 ? kMaxInt8Hidden : kMaxDim) &&
+         I <= kMaxDim && tokens * top_k * I < (int64_t(1) << 31);
 }
 
 int slots_of(const FewArgs& p) { return p.E <= p.R ? p.E : p.R; }
@@ -652,7 +653,7 @@ int by_blocks(const FewArgs& p, F&& f) {
 }  // namespace
 
 extern "C" size_t mm_moe_few_scratch_bytes(int64_t tokens, int32_t top_k, int32_t hidden, int32_t inter, int32_t int8) {
-  if (!few_sizes_ok(tokens, top_k, 1, hidden, inter)) return 0;
+  if (!few_sizes_ok(tokens, top_k, 1, hidden, inter, int8 != 0)) return 0;
   return FewScratch(tokens * top_k, hidden, inter, int8 != 0).bytes;
 }
 
@@ -661,7 +662,7 @@ extern "C" int mm_moe_few(const uint16_t* x, const int32_t* selected, const floa
                           int32_t top_k, int32_t num_experts, int32_t hidden, int32_t inter, int32_t act_kind,
                           float situ_beta, float situ_linear_beta, float clamp_limit, uint16_t* out, void* scratch,
                           size_t scratch_bytes, mm_stream_t stream) {
-  MM_CHECK_ARG(few_sizes_ok(tokens, top_k, num_experts, hidden, inter), "mm_moe_few: bad sizes");
+  MM_CHECK_ARG(few_sizes_ok(tokens, top_k, num_experts, hidden, inter, false), "mm_moe_few: bad sizes");
   MM_CHECK_ARG(w2_sh == 1 || w2_sf == 1, "mm_moe_few: w2 needs a unit stride along hidden or inter");
   MM_CHECK_ARG(w2_sh >= 0 && w2_sh <= kMaxStride && w2_sf >= 0 && w2_sf <= kMaxStride,
                "mm_moe_few: w2 rows more than 2^25 elements apart");
@@ -700,7 +701,8 @@ extern "C" int mm_moe_few_int8(const int8_t* x, const float* x_scale, const int3
                                int32_t hidden, int32_t inter, int32_t act_kind, float situ_beta,
                                float situ_linear_beta, float clamp_limit, uint16_t* out, void* scratch,
                                size_t scratch_bytes, mm_stream_t stream) {
-  MM_CHECK_ARG(few_sizes_ok(tokens, top_k, num_experts, hidden, inter), "mm_moe_few_int8: bad sizes");
+  MM_CHECK_ARG(few_sizes_ok(tokens, top_k, num_experts, hidden, inter, true),
+               "mm_moe_few_int8: bad sizes (hidden at most %d)", kMaxInt8Hidden);
   MM_CHECK_ARG(act_kind >= MM_ACT_SWIGLU && act_kind <= MM_ACT_CLAMP_SWIGLU, "mm_moe_few_int8: bad activation");
   if (tokens == 0) return MM_OK;
   const FewScratch f(tokens * top_k, hidden, inter, true);

@@ -437,7 +437,7 @@ std::optional<Tensor> few_forward_int8(const Layer& l, const Tensor& x, const Te
                                        const Tensor& gate_up, const Tensor& gate_up_scale, const Tensor& down,
                                        const Tensor& down_scale, const Tensor& weights) {
   const int64_t inter = down.size(2), tokens = few_tokens(l, x, at::kChar, selected, weights, inter);
-  if (tokens < 0 || !is_whole(x_scale, at::kFloat, {tokens}, x) ||
+  if (tokens < 0 || l.hidden > kMaxK || !is_whole(x_scale, at::kFloat, {tokens}, x) ||
       !is_whole(gate_up, at::kChar, {l.experts, 2 * inter, l.hidden}, x))
     return std::nullopt;
   Tensor out = at::empty({tokens, l.hidden}, x.options().dtype(at::kBFloat16));

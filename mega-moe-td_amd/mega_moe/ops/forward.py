@@ -41,6 +41,7 @@ from .int8 import Int8Experts
 MAX_EXPERTS = 32768
 MAX_TOP_K = 64
 MAX_FEW_TOKENS = _lib.FEW_MAX_TOKENS
+MAX_INT8_SUM = 1 << 17  # columns of int8 rows (csrc/few.hip)
 
 
 @dataclass
@@ -430,10 +431,10 @@ class FusedMoEForward(torch.nn.Module):
         """``forward_few`` on int8 rows and int8 experts.
 
         ``tokens`` int8 [T, H] with fp32 ``token_scale`` [T], as ``rms_norm`` and
-        ``quantize_rows`` make them; returns bf16 [T, H]. The products are summed
-        in int32; between them the activation (times the routing weight) is
-        rounded to int8 in groups of 32 columns with the group's largest value
-        at 127. A NaN or infinite scale makes its own token's output NaN (where
+        ``quantize_rows`` make them, H below 2^17; returns bf16 [T, H]. The
+        products are summed in int32; between them the activation (times the
+        routing weight) is rounded to int8 in groups of 32 columns with the
+        group's largest value at 127. A NaN or infinite scale makes its own token's output NaN (where
         any slot of the token has an expert) and no other's.
         """
         if not isinstance(experts, Int8Experts):
@@ -460,6 +461,8 @@ class FusedMoEForward(torch.nn.Module):
             raise ValueError(f"experts hold {num_experts} experts of hidden size {hidden}, expected "
                              f"{self.experts_per_rank} of {self.hidden_size}")
         self._validate_few_sizes(two_inter)
+        if hidden >= MAX_INT8_SUM:
+            raise ValueError(f"hidden_size must be below {MAX_INT8_SUM} for exact int32 sums, got {hidden}")
         device = selected_experts.device
         if tokens.device != device or token_scale.device != device or experts.gate_up.device != device:
             raise ValueError("tokens, token_scale, selected_experts and experts must be on the same device")
