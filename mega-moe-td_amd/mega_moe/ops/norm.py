@@ -27,8 +27,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
     ``x`` [..., H] in bf16, fp16 or fp32 with H up to 32768, unit column stride
     and rows that are evenly spaced in memory; ``residual`` of the same shape in
     ``x.dtype`` or fp32; ``weight`` [H] in any of the three types (``None``: all
-    ones). Statistics are fp32; every output is rounded once, and the norm is
-    taken of ``h`` as it is stored.
+    ones). Statistics and ``eps`` are fp32, over the whole range of ``h``; every
+    output is rounded once, and the norm is taken of ``h`` as it is stored.
 
     Returns ``y`` in ``x.dtype``; with ``residual`` ``(y, h)``. With
     ``out_dtype`` int8 or float8_e4m3fn ``y`` is replaced by ``q, scale``:
