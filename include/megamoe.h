@@ -454,9 +454,9 @@ int mm_rms_norm(const void* x, int64_t ldx, int32_t x_type, const void* residual
 
 /*
  * Backward of mm_rms_norm with y_type == x_type:
- *   g = dh + rstd * weight * dy - h * rstd^3 * mean(weight * dy * h),
+ *   g = dh + rstd * (weight * dy - n * mean(weight * dy * n)), n = h * rstd,
  *   dx = g in x_type, dresidual = g in h_type (NULL: not wanted),
- *   dweight = sum over rows of dy * h * rstd in weight_type (NULL: not wanted)
+ *   dweight = sum over rows of dy * n in weight_type (NULL: not wanted)
  * dy [rows, hidden] in x_type; dh (gradient of h_out, or NULL) and h in
  * h_type; dx and dresidual contiguous. The rows' sums have a fixed order.
  * The workspace is needed with dweight only.

@@ -5,7 +5,9 @@
 //   y = h * r * w,  r = 1 / sqrt(mean(h^2) + eps)
 //   8 bits: s = max(a, 1e-30) / Q with a = max |y| over the row (s = 1 where
 //           a = 0), q = round(y / s) of the unrounded y; Q = 127 (int8) or 448 (E4M3)
-//   backward: dx = dh + r w dy - h r^3 mean(w dy h),  dw = sum_rows dy h r
+//   backward, with n = h r: dx = dh + r (w dy - n mean(w dy n)),  dw = sum_rows dy n
+//           (n is near 1 whatever the row's size; r^3 would leave fp32 from rows
+//           of 1e13 on)
 //
 // The norm is taken of h as it is stored, so that the backward (which reads h)
 // and a caller who adds and norms in two steps compute the same function. Sums
@@ -393,6 +395,7 @@ __global__ __launch_bounds__(WAVE ? kWaveThreads : 1024) void rms_norm_bwd_kerne
   int parity = 0;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * rpb + sub; row < p.rows;
        row += static_cast<int64_t>(gridDim.x) * rpb) {
+    const float r = p.rstd[row];  // first, as the dot product waits for it (8192 x 2048: 29 us behind the rows, 26 so)
     Vec8<TX> gv[NV];
     Vec8<TH> hv[NV], ev[NV];
 #pragma unroll
@@ -404,7 +407,6 @@ __global__ __launch_bounds__(WAVE ? kWaveThreads : 1024) void rms_norm_bwd_kerne
     if (p.dh)
 #pragma unroll
       for (int u = 0; u < NV; ++u) ev[u].load(p.dh, row * p.lddh + Columns(u * threads + t, H).at);
-    const float r = p.rstd[row];
     float g[NV][8], h[NV][8];
     float dot = 0.0f;
 #pragma unroll
@@ -414,20 +416,21 @@ __global__ __launch_bounds__(WAVE ? kWaveThreads : 1024) void rms_norm_bwd_kerne
       hv[u].to_f32(h[u]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        dw[u][i] += g[u][i] * (h[u][i] * r);
+        h[u][i] *= r;
+        dw[u][i] += g[u][i] * h[u][i];
         g[u][i] *= w[u][i];
         dot += c.counts(i) ? g[u][i] * h[u][i] : 0.0f;
       }
     }
     dot = row_sum<WAVE>(dot, sums[parity]);
     parity ^= 1;
-    const float c1 = r * r * r * (dot / static_cast<float>(H));
+    const float mean = dot / static_cast<float>(H);
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const Columns c(u * threads + t, H);
       float d[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[i] = r * g[u][i] - h[u][i] * c1;
+      for (int i = 0; i < 8; ++i) d[i] = r * (g[u][i] - h[u][i] * mean);
       if (p.dh) {
         float e[8];
         ev[u].to_f32(e);
@@ -483,16 +486,16 @@ __global__ __launch_bounds__(256) void rms_norm_short_bwd_kernel(NormBwdArgs p) 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       g[i] = i < H ? static_cast<float>(static_cast<const TX*>(p.dy)[row * p.lddy + i]) : 0.0f;
-      h[i] = i < H ? static_cast<float>(static_cast<const TH*>(p.h)[row * p.ldh + i]) : 0.0f;
-      dw[i] += g[i] * (h[i] * r);
+      h[i] = i < H ? static_cast<float>(static_cast<const TH*>(p.h)[row * p.ldh + i]) * r : 0.0f;
+      dw[i] += g[i] * h[i];
       g[i] *= w[i];
       dot += g[i] * h[i];
     }
-    const float c1 = r * r * r * (dot / static_cast<float>(H));
+    const float mean = dot / static_cast<float>(H);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (i >= H) continue;
-      float d = r * g[i] - h[i] * c1;
+      float d = r * (g[i] - h[i] * mean);
       if (p.dh) d += static_cast<float>(static_cast<const TH*>(p.dh)[row * p.lddh + i]);
       static_cast<TX*>(p.dx)[row * H + i] = static_cast<TX>(d);
       if (p.dres) static_cast<TH*>(p.dres)[row * H + i] = static_cast<TH>(d);

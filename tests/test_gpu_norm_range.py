@@ -32,6 +32,32 @@ def _rows(hidden, sizes, dtype, seed):
     return (x * size).to(dtype), g
 
 
+def _backward(hidden, sizes, dtype, eps, residual, rel=2**-17):
+    x, g = _rows(hidden, sizes, dtype, hidden)
+    w = (1 + 0.3 * torch.randn(hidden, generator=g, device="cuda")).requires_grad_()
+    dy = torch.randn(len(sizes), hidden, generator=g, device="cuda").to(dtype)
+    x.requires_grad_()
+    res = (x.detach() * 0.5).requires_grad_() if residual else None
+    out = mega_moe.rms_norm(x, w, residual=res, eps=eps)
+    y, h = out if residual else (out, x)
+    grads = torch.autograd.grad(y, (x, w), dy)
+    hd, wd, dyd = h.detach().double(), w.detach().double(), dy.double()
+    r = 1 / (hd.square().mean(-1, keepdim=True) + eps).sqrt()
+    t, n = dyd * wd, hd * r
+    mean = (t * n).mean(-1, keepdim=True)
+    _near(grads[0], r * (t - n * mean), r * (t.abs() + n.abs() * (t * n).abs().mean(-1, keepdim=True)) * rel, "dx")
+    _near(grads[1], (dyd * n).sum(0), (dyd * n).abs().sum(0) * rel, "dweight")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("hidden", HIDDEN)
+def test_backward_of_large_and_small_rows(hidden, residual, dtype):
+    """1 / rms cubed leaves fp32 for these rows; no step of the gradient does."""
+    _backward(hidden, (1.0, 1e12, 1e13, 3e15, 1e17), dtype, 1e-6, residual)
+    _backward(hidden, (1.0, 1e-12, 1e-13, 1e-14), dtype, 0.0, residual)
+
+
 FAR = (1.0, 1e19, 1e25, 3e37, 1e-4)       # squares past the largest fp32
 NEAR = (1.0, 1e-19, 1e-25, 1e-36, 1e4)    # and below the smallest; eps = 0
 
@@ -60,6 +86,14 @@ def test_eight_bits_where_squares_leave_the_range(hidden, out_dtype, most):
     q, s = mega_moe.rms_norm(x, w, eps=0.0, out_dtype=out_dtype)
     far_q, far_s = mega_moe.rms_norm((x.float() * k).to(BF), w, eps=0.0, out_dtype=out_dtype)
     assert torch.equal(far_q.float(), q.float()) and torch.equal(far_s, s)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("hidden", HIDDEN)
+def test_backward_where_squares_leave_the_range(hidden, residual, dtype):
+    _backward(hidden, FAR, dtype, 1e-6, residual)
+    _backward(hidden, NEAR, dtype, 0.0, residual)
 
 
 def test_eps_counts_in_every_range():
