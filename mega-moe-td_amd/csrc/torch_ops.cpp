@@ -407,9 +407,23 @@ int64_t few_tokens(const Layer& l, const Tensor& x, ScalarType x_type, const Ten
   return ok ? tokens : -1;
 }
 
-// [tokens, hidden] of the layer, or None for operands that do not fit it.
-std::optional<Tensor> few_forward(const Layer& l, const Tensor& x, const Tensor& selected, const Tensor& gate_up,
+// No backward exists: a gradient asked for would be lost silently, and a tangent.
+void check_detached(const char* op, std::initializer_list<const Tensor*> tensors) {
+  const bool recording = at::GradMode::is_enabled();
+  for (const Tensor* t : tensors) {
+    CHECK_VALUE(!recording || !t->requires_grad(), op,
+                " carries no gradient; call under torch.no_grad() or on detached operands, or use MegaMoEFunction");
+    CHECK_VALUE(!t->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+  }
+}
+
+// [tokens, hidden] of the layer, or None for operands that do not fit it (none
+// fit a null layer).
+std::optional<Tensor> few_forward(const Layer* layer, const Tensor& x, const Tensor& selected, const Tensor& gate_up,
                                   const Tensor& down, const Tensor& weights) {
+  check_detached("forward_few", {&x, &gate_up, &down, &weights});
+  if (!layer) return std::nullopt;
+  const Layer& l = *layer;
   if (gate_up.dim() != 3 || down.dim() != 3 || gate_up.size(2) % 2) return std::nullopt;
   const int64_t inter = gate_up.size(2) / 2, tokens = few_tokens(l, x, at::kBFloat16, selected, weights, inter);
   if (tokens < 0 || !is_whole(gate_up, at::kBFloat16, {l.experts, l.hidden, 2 * inter}, x) ||
@@ -433,9 +447,12 @@ std::optional<Tensor> few_forward(const Layer& l, const Tensor& x, const Tensor&
 
 // The same on int8 rows and experts, whose tensors Int8Experts has checked
 // against each other.
-std::optional<Tensor> few_forward_int8(const Layer& l, const Tensor& x, const Tensor& x_scale, const Tensor& selected,
-                                       const Tensor& gate_up, const Tensor& gate_up_scale, const Tensor& down,
-                                       const Tensor& down_scale, const Tensor& weights) {
+std::optional<Tensor> few_forward_int8(const Layer* layer, const Tensor& x, const Tensor& x_scale,
+                                       const Tensor& selected, const Tensor& gate_up, const Tensor& gate_up_scale,
+                                       const Tensor& down, const Tensor& down_scale, const Tensor& weights) {
+  check_detached("forward_few_int8", {&x_scale, &gate_up_scale, &down_scale, &weights});
+  if (!layer) return std::nullopt;
+  const Layer& l = *layer;
   const int64_t inter = down.size(2), tokens = few_tokens(l, x, at::kChar, selected, weights, inter);
   if (tokens < 0 || l.hidden > kMaxK || !is_whole(x_scale, at::kFloat, {tokens}, x) ||
       !is_whole(gate_up, at::kChar, {l.experts, 2 * inter, l.hidden}, x))

@@ -409,13 +409,13 @@ class FusedMoEForward(torch.nn.Module):
         activation and the output are rounded to bf16 (``forward`` also rounds
         gate, up and the expert outputs), so the last bits differ from
         ``forward``'s; they do not depend on the other tokens of the call. Nothing
-        is saved for a backward, no workspace of the operator is used and its
+        is saved for a backward and operands that ask for a gradient are refused
+        (``MegaMoEFunction`` has one); no workspace of the operator is used and its
         routing generation does not move: calls may run on any stream, between a
         forward and its backward, and captured. No counterpart in the reference.
         """
         ops, layer = self._few_layer(hidden_states)
-        out = layer and ops.few_forward(layer, hidden_states, selected_experts, gate_up_weight, down_weight,
-                                        routing_weights)
+        out = ops.few_forward(layer, hidden_states, selected_experts, gate_up_weight, down_weight, routing_weights)
         if out is not None:
             return out
         # the operands do not fit the layer: one of these checks says why
@@ -440,8 +440,8 @@ class FusedMoEForward(torch.nn.Module):
         if not isinstance(experts, Int8Experts):
             raise TypeError("experts must be an Int8Experts")
         ops, layer = self._few_layer(tokens)
-        out = layer and ops.few_forward_int8(layer, tokens, token_scale, selected_experts, experts.gate_up,
-                                             experts.gate_up_scale, experts.down, experts.down_scale, routing_weights)
+        out = ops.few_forward_int8(layer, tokens, token_scale, selected_experts, experts.gate_up,
+                                   experts.gate_up_scale, experts.down, experts.down_scale, routing_weights)
         if out is not None:
             return out
         # the operands do not fit the layer: one of these checks says why
