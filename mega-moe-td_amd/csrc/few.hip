@@ -688,9 +688,11 @@ extern "C" int mm_moe_few(const uint16_t* x, const int32_t* selected, const floa
   const bool wide = static_cast<int64_t>(slots_of(p)) * (inter / 64) >= 512;
   auto run = [&](auto blocks) {
     constexpr int NT = decltype(blocks)::value;
-    constexpr int WIDE = NT < 4 ? 8 : 4;  // the partial sums of 64 tokens and 64 columns do not fit LDS
-    return launch_both(p, wide ? Launch{few_fc1_kernel<WIDE, 8, NT>, 8, 8 * WIDE} : Launch{few_fc1_kernel<4, 8, NT>, 8, 32},
-                       rows ? Launch{few_fc2_kernel<true, 4, 8, NT>, 8, 64} : Launch{few_fc2_kernel<false, 4, 8, NT>, 8, 64}, s);
+    Launch fc1{few_fc1_kernel<4, 8, NT>, 8, 32};
+    if constexpr (NT < 4) {  // the partial sums of 64 tokens and 64 columns do not fit LDS
+      if (wide) fc1 = {few_fc1_kernel<8, 8, NT>, 8, 64};
+    }
+    return launch_both(p, fc1, rows ? Launch{few_fc2_kernel<true, 4, 8, NT>, 8, 64} : Launch{few_fc2_kernel<false, 4, 8, NT>, 8, 64}, s);
   };
   return by_blocks(p, run);
 }
