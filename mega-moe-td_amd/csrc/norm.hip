@@ -556,13 +556,15 @@ constexpr int kMaxHidden = 32768;  // 1024 threads of 4 vectors
 // half a CU (7168 columns: 118 us with one, 92 with two). The backward keeps
 // short rows in waves, 4 to a workgroup, so that few partial sums are left
 // (16384 x 1024: 24 us + 4 for their sum, in workgroups 27 + 7).
-template <class F>
-int by_hidden(int H, bool backward, F&& f) {
+template <bool BACKWARD, class F>
+int by_hidden(int H, F&& f) {
   if (H < 8) return f.short_rows();
   const int v = (H + 7) / 8;
   auto threads = [&](int nv) { return (v + 64 * nv - 1) / (64 * nv) * 64; };
   if (v <= 64) return f.template operator()<1, true>(64);
-  if (backward && v <= 128) return f.template operator()<2, true>(64);
+  if constexpr (BACKWARD) {
+    if (v <= 128) return f.template operator()<2, true>(64);
+  }
   if (v <= 512) return f.template operator()<1, false>(threads(1));
   if (v <= 2048) return f.template operator()<2, false>(threads(2));
   return f.template operator()<4, false>(threads(4));
@@ -635,14 +637,14 @@ struct CountBwd {
 
 bool is_float_type(int t) { return t == MM_T_BF16 || t == MM_T_FP16 || t == MM_T_FP32; }
 
-template <template <class, class> class L, class... A>
-int by_types(int x_type, int h_type, int H, bool backward, const A&... a) {
-  if (x_type == MM_T_FP32) return by_hidden(H, backward, L<float, float>{a...});
+template <bool BACKWARD, template <class, class> class L, class... A>
+int by_types(int x_type, int h_type, int H, const A&... a) {
+  if (x_type == MM_T_FP32) return by_hidden<BACKWARD>(H, L<float, float>{a...});
   if (x_type == MM_T_FP16)
-    return h_type == MM_T_FP32 ? by_hidden(H, backward, L<_Float16, float>{a...})
-                               : by_hidden(H, backward, L<_Float16, _Float16>{a...});
-  return h_type == MM_T_FP32 ? by_hidden(H, backward, L<bf16, float>{a...})
-                             : by_hidden(H, backward, L<bf16, bf16>{a...});
+    return h_type == MM_T_FP32 ? by_hidden<BACKWARD>(H, L<_Float16, float>{a...})
+                               : by_hidden<BACKWARD>(H, L<_Float16, _Float16>{a...});
+  return h_type == MM_T_FP32 ? by_hidden<BACKWARD>(H, L<bf16, float>{a...})
+                             : by_hidden<BACKWARD>(H, L<bf16, bf16>{a...});
 }
 
 bool rows_ok(int64_t rows) { return rows >= 0 && rows < (int64_t(1) << 31); }
@@ -662,7 +664,7 @@ extern "C" int mm_rms_norm(const void* x, int64_t ldx, int32_t x_type, const voi
   if (rows == 0) return MM_OK;
   MM_CHECK_ARG(x && y && (!residual || h_out) && (!eight || scale), "mm_rms_norm: null pointer");
   const NormArgs p{x, residual, weight, h_out, y, scale, rstd, ldx, ldr, rows, hidden, weight_type, y_type, 1, eps};
-  return by_types<LaunchFwd>(x_type, residual ? h_type : x_type, hidden, false, p, mm_hip_stream(stream));
+  return by_types<false, LaunchFwd>(x_type, residual ? h_type : x_type, hidden, p, mm_hip_stream(stream));
 }
 
 extern "C" int mm_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int64_t rows, int32_t cols, void* q,
@@ -673,12 +675,12 @@ extern "C" int mm_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int6
   if (rows == 0) return MM_OK;
   MM_CHECK_ARG(x && q && scale, "mm_quantize_rows: null pointer");
   const NormArgs p{x, nullptr, nullptr, nullptr, q, scale, nullptr, ldx, 0, rows, cols, 0, q_type, 0, 0.0f};
-  return by_types<LaunchFwd>(x_type, x_type, cols, false, p, mm_hip_stream(stream));
+  return by_types<false, LaunchFwd>(x_type, x_type, cols, p, mm_hip_stream(stream));
 }
 
 extern "C" size_t mm_rms_norm_bwd_workspace_bytes(int64_t rows, int32_t hidden) {
   if (!rows_ok(rows) || hidden <= 0 || hidden > kMaxHidden) return 0;
-  return static_cast<size_t>(by_hidden(hidden, true, CountBwd{rows})) * hidden * 4;
+  return static_cast<size_t>(by_hidden<true>(hidden, CountBwd{rows})) * hidden * 4;
 }
 
 extern "C" int mm_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh,
@@ -704,5 +706,5 @@ extern "C" int mm_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int
   }
   const NormBwdArgs p{dy,   dh,   h,   weight, rstd,   dx, dresidual, dweight ? static_cast<float*>(workspace) : nullptr,
                       lddy, lddh, ldh, rows,   hidden, weight_type};
-  return by_types<LaunchBwd>(x_type, h_type, hidden, true, p, dweight, s);
+  return by_types<true, LaunchBwd>(x_type, h_type, hidden, p, dweight, s);
 }
