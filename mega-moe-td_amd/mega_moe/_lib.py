@@ -22,9 +22,8 @@ FC1_FORMATS = {"bf16": 0, "fp16": 1, "fp8": 2}
 FC1_SCALE_GROUP = 128
 # element types of the norm and the int8 product (MM_T_*)
 ELEMENT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.int8: 3, torch.float8_e4m3fn: 4}
-# the few-token layer (MM_FEW_MAX_TOKENS, MM_FEW_ACT_GROUP)
+# the few-token layer (MM_FEW_MAX_TOKENS)
 FEW_MAX_TOKENS = 64
-FEW_ACT_GROUP = 32
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
