@@ -184,11 +184,12 @@ struct Quantizer {
     scale = !finite ? __uint_as_float(0x7fc00000u) : bits == 0 ? 1.0f : fmaxf(a, kScaleFloor) / q;
   }
   // t Q / top: one correction of the quotient makes it exact where it is
-  // representable. |value| stays below the border of the largest, so neither
+  // representable, with what t Q loses to rounding (22 bits of fp16 products and
+  // 7 of Q). |value| stays below the border of the largest, so neither
   // type saturates.
   __device__ __forceinline__ float value(float t) const {
-    const float p = t * most, q = p * inv;
-    return fmaf(fmaf(-q, top, p), fix, q);
+    const float p = t * most, rest = fmaf(t, most, -p), q = p * inv;
+    return fmaf(fmaf(-q, top, p) + rest, fix, q);
   }
 };
 
