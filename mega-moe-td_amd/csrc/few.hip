@@ -303,7 +303,12 @@ __global__ __launch_bounds__(W * 64) void few_fc1_kernel(FewArgs p) {
 // y crosses the XCDs' L2 caches inside the launch: it is written and read with
 // agent-scope accesses, which go past them. A release fence would write back
 // the whole L2 of the XCD for every workgroup (8 experts, 2048 columns: 41 us
-// against 10).
+// against 10). What orders the hand-over instead: an agent-scope store writes
+// through to memory and counts as outstanding (vmcnt) until it is there; a wave
+// waits for its own, the barrier for the workgroup's waves, and only then does
+// the workgroup arrive. The last to arrive reads y behind that, and no cache of
+// its XCD can hold an older copy of a line: within the launch nobody has read y,
+// and a route's columns of a tile, whole lines, are written by one workgroup.
 __device__ __forceinline__ void put_y(float* p, const f32x4& v) {
   const uint64_t* w = reinterpret_cast<const uint64_t*>(&v);
   uint64_t* d = reinterpret_cast<uint64_t*>(p);

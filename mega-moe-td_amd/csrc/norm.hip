@@ -594,7 +594,9 @@ struct LaunchFwd {
 // (8192 x 2048, one vector: 26 + 4 us, with half as many 31 + 4; 16384 x 1024,
 // two: 26 + 4, with twice as many 30 + 4). All take equally many rows, so that
 // none leaves a partial row for fewer (1021 x 2305: 511 workgroups of 2 rows
-// 10.2 + 4.0 us, 819 of 1 or 2 rows 10.9 + 4.9).
+// 10.2 + 4.0 us, 819 of 1 or 2 rows 10.9 + 4.9). Workgroups of 8 waves and more
+// then leave CUs idle: 128 of them at 16384 columns, 64 at 32768 (2048 x 16384
+// with a residual 63 us, 4.2 TB/s; 1024 x 32768 431, with spilled registers).
 template <int NV, bool WAVE>
 int bwd_groups(int64_t rows, int threads) {
   const int rpb = WAVE ? kWaveRows : 1, waves = (WAVE ? kWaveThreads : threads) / 64;

@@ -413,6 +413,12 @@ class FusedMoEForward(torch.nn.Module):
         (``MegaMoEFunction`` has one); no workspace of the operator is used and its
         routing generation does not move: calls may run on any stream, between a
         forward and its backward, and captured. No counterpart in the reference.
+
+        It is the faster call for one token whose experts hold up to about 150 MB
+        (hidden 2048, inter 768, 8 of 128 experts: 27 us against ``forward``'s 36;
+        4096, 1536, 4 of 32: 47 against 61). ``forward`` streams weights faster
+        and wins beyond (two tokens of these layers: 44 against 42, 88 against 72;
+        7168, 2048, 8 of 64: 159 against 129 for one token, 888 against 821 for 32).
         """
         ops, layer = self._few_layer(hidden_states)
         out = ops.few_forward(layer, hidden_states, selected_experts, gate_up_weight, down_weight, routing_weights)
