@@ -490,6 +490,87 @@ int mm_int8_matmul(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb,
                    int32_t bias_type, int64_t m, int64_t n, int64_t k, void* out,
                    int64_t ldo, int32_t out_type, mm_stream_t stream);
 
+/* --------------------------------- E4M3 with a scale for each block of 128 */
+
+/* Columns of a block, and rows of a square one. */
+#define MM_FP8_BLOCK 128
+
+/*
+ * Blocks of x [batch, rows, cols] (BF16, FP16 or FP32; unit column stride, row
+ * stride ldx, matrix stride x_batch, any alignment) in E4M3 with a power-of-two
+ * scale each: blocks are 128 columns of a row (block_rows = 1) or 128 x 128
+ * (block_rows = 128), the last ones of an axis what is left of it.
+ *   a = max |x| of the block, scale = 2^k, k the smallest integer >= -126 with
+ *   a <= 448 2^k (k = 0 where a = 0), q = round_to_even(x / 2^k)
+ * scale holds k + 127 in a byte (E8M0). A block with a NaN or an infinity has
+ * scale 255 (NaN) and bytes 0. q [batch, rows, ldq] with cols <= ldq <= cols
+ * rounded up to 128, bytes from cols on 0; scale [batch, ceil(rows /
+ * block_rows), ceil(cols / 128)]. No counterpart in the reference, here and in
+ * the entries below.
+ */
+int mm_quantize_blocks(const void* x, int64_t ldx, int64_t x_batch, int32_t x_type,
+                       int64_t batch, int64_t rows, int64_t cols, int32_t block_rows,
+                       uint8_t* q, int64_t ldq, uint8_t* scale, mm_stream_t stream);
+
+/*
+ * The forms of x [rows, cols] that a product's gradients read, with ceil(rows /
+ * 128) = rb, ceil(cols / 128) = cb:
+ *   q   [rows, 128 cb]  as mm_quantize_blocks (NULL: not wanted)
+ *   qt  [cols, 128 rb]  the transpose. block_rows = 1: in blocks of 128 rows of
+ *                       x each, scale_t [cols, rb]; 128: the bytes of q with
+ *                       their blocks' scales, scale_t [cb, rb]. Bytes from rows
+ *                       on are 0.
+ * x_type may also be E4M3 with x_scale [rows, cb], rows as block_rows = 1 makes
+ * them; then block_rows is 128 and q NULL.
+ */
+int mm_quantize_blocks_t(const void* x, int64_t ldx, int32_t x_type, const uint8_t* x_scale,
+                         int64_t rows, int64_t cols, int32_t block_rows, uint8_t* q,
+                         uint8_t* scale, uint8_t* qt, uint8_t* scale_t, mm_stream_t stream);
+
+/*
+ * mm_rms_norm with y in E4M3 and a scale for each 128 columns, as
+ * mm_quantize_blocks of the unrounded y: q [rows, hidden], scale [rows,
+ * ceil(hidden / 128)].
+ */
+int mm_rms_norm_blocks(const void* x, int64_t ldx, int32_t x_type, const void* residual,
+                       int64_t ldr, int32_t h_type, const void* weight, int32_t weight_type,
+                       int64_t rows, int32_t hidden, float eps, void* h_out, uint8_t* q,
+                       uint8_t* scale, mm_stream_t stream);
+
+/*
+ * out[i, j] = sum_k a[i, k] a_scale[i, k / 128] b[j, k] b_scale[j / 128, k / 128] + bias[j]
+ * for E4M3 a [m, k] and b [n, k], unit column strides, row strides lda and ldb
+ * from k to 2^23 at any alignment, and E8M0 scales, contiguous: a_scale [m,
+ * ceil(k / 128)], b_scale [ceil(n / 128), ceil(k / 128)]. Sums and bias (NULL:
+ * none; BF16, FP16 or FP32) are fp32 and rounded once to out_type (the same
+ * three; row stride ldo).
+ */
+int mm_fp8_matmul(const uint8_t* a, int64_t lda, const uint8_t* a_scale, const uint8_t* b,
+                  int64_t ldb, const uint8_t* b_scale, const void* bias, int32_t bias_type,
+                  int64_t m, int64_t n, int64_t k, void* out, int64_t ldo, int32_t out_type,
+                  mm_stream_t stream);
+
+/*
+ * The forward of the layer on E4M3 rows and experts: x [tokens, hidden] with
+ * x_scale [tokens, hidden / 128]; w1 [E, 2 inter, hidden] (gate rows, then up
+ * rows) and w2 [E, hidden, inter] with scales for each 128 x 128; all
+ * contiguous, hidden and inter multiples of 128. The activation (fp32, times
+ * the routing weight) goes to FC2 in E4M3 with a scale for each 128 columns, the
+ * experts' outputs to the sum over the slots in bf16. Routing as mm_route; a
+ * NaN scale of a row makes that row's output NaN where any slot of it has an
+ * expert. Scratch of mm_moe_fp8_scratch_bytes (0 for sizes out of range), 16-byte
+ * aligned like out, free again when the stream has passed the call.
+ */
+size_t mm_moe_fp8_scratch_bytes(int64_t tokens, int32_t top_k, int32_t num_experts,
+                                int32_t hidden, int32_t inter);
+
+int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_t* selected,
+               const float* routing_weights, const uint8_t* w1, const uint8_t* w1_scale,
+               const uint8_t* w2, const uint8_t* w2_scale, int64_t tokens, int32_t top_k,
+               int32_t num_experts, int32_t hidden, int32_t inter, int32_t act_kind,
+               float situ_beta, float situ_linear_beta, float clamp_limit, uint16_t* out,
+               void* scratch, size_t scratch_bytes, mm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,305 @@
+// Product of E4M3 rows with a power-of-two scale for each block of 128 (fp8.h).
+//
+//   out[m, n] = sum_k a[m, k] sa[m, k / 128] b[n, k] sb[n / 128, k / 128]  (+ bias[n])
+//
+// a [M, K] and b [N, K] with K contiguous. The scales are the matrix
+// instruction's own operands, so sums over the whole of K stay in its fp32
+// accumulators and are rounded once, behind the bias. (Results in 32 bits: see
+// Op16Wide.)
+#include "fp8_tile.h"
+
+namespace {
+
+constexpr int64_t kMaxStride = int64_t(1) << 23;        // 256 rows of a tile in 32-bit offsets
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 512;  // a tile's last row stays in 32 bits
+
+struct Fp8Args {
+  const uint8_t* a;
+  const uint8_t* b;
+  const uint8_t* sa;  // [M, kb]
+  const uint8_t* sb;  // [N / 128, kb]
+  const void* bias;
+  void* out;
+  int64_t lda, ldb, ldo;
+  int32_t m, n, k, kb, out_type, bias_type;
+};
+
+// Columns col .. col + 3 of a row, from their sums.
+__device__ __forceinline__ void store4(const Fp8Args& p, int row, int col, f32x4 f) {
+  const int left = p.n - col;
+  if (p.bias) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] += load_any(p.bias, p.bias_type, min(col + r, p.n - 1));
+  }
+  const int64_t at = row * p.ldo + col;
+  if (p.out_type == MM_T_FP32) {
+    float* out = static_cast<float*>(p.out) + at;
+    if (left >= 4) {
+      *reinterpret_cast<Out4*>(out) = __builtin_bit_cast(i32x4, f);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 3; ++r)
+        if (r < left) out[r] = f[r];
+    }
+    return;
+  }
+  const uint2 h = pack4(f, p.out_type);
+  uint16_t* out = static_cast<uint16_t*>(p.out) + at;
+  if (left >= 4) {
+    *reinterpret_cast<Out2*>(out) = Out2{static_cast<int>(h.x), static_cast<int>(h.y)};
+  } else {
+    if (left > 0) out[0] = static_cast<uint16_t>(h.x);
+    if (left > 1) out[1] = static_cast<uint16_t>(h.x >> 16);
+    if (left > 2) out[2] = static_cast<uint16_t>(h.y);
+  }
+}
+
+// ------------------------------------------------------------------ operands from memory
+// Tile of 16 G channels x 16 NT tokens. Channels are the rows of the matrix
+// instruction and tokens its columns; the lane's 32 bytes of a block are two
+// runs of 16, 64 apart, so that four lanes read 64 neighbouring bytes. The W
+// waves share the sum's blocks (wave w takes w, w + W, ...), U of them in
+// flight, and join through LDS in wave order.
+template <class OP, int G, int NT, int W, int U, bool SHIFT>
+__global__ __launch_bounds__(W * 64) void fp8_direct_kernel(Fp8Args p) {
+  __shared__ f32x4 red[W * G * NT * 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, q = lane >> 4;
+  // every XCD gets a run of channels with all their tokens
+  const int total = gridDim.x, per = (total + 7) / 8, tiles_m = (p.m + NT * 16 - 1) / (NT * 16);
+  int tile = blockIdx.x;
+  if (total % 8 == 0) tile = (tile & 7) * per + (tile >> 3);
+  const int n0 = tile / tiles_m * (G * 16), m0 = tile % tiles_m * (NT * 16);
+  uint32_t b_off[G], a_off[NT], rest_a, rest_b;
+  const char* a = aligned_base(p.a + m0 * p.lda, rest_a);
+  const char* b = aligned_base(p.b + n0 * p.ldb, rest_b);
+  const uint8_t* sa[NT];
+  const uint8_t* sb[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const int row = min(g * 16 + j, p.n - 1 - n0);
+    b_off[g] = static_cast<uint32_t>(row) * static_cast<uint32_t>(p.ldb) + rest_b + 16 * q;
+    sb[g] = p.sb + static_cast<int64_t>((n0 + row) / kBlock) * p.kb;
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = min(n * 16 + j, p.m - 1 - m0);
+    a_off[n] = static_cast<uint32_t>(row) * static_cast<uint32_t>(p.lda) + rest_a + 16 * q;
+    sa[n] = p.sa + static_cast<int64_t>(m0 + row) * p.kb;
+  }
+  f32x4 acc[G][NT];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[g][n] = f32x4{0, 0, 0, 0};
+  const int full = p.k / kBlock;
+  auto steps = [&](auto count, int s) {
+    constexpr int C = decltype(count)::value;
+    i32x4 bv[C][G][2], av[C][NT][2];
+    uint32_t bs[C][G], as[C][NT];
+#pragma unroll
+    for (int u = 0; u < C; ++u) {
+      const int block = s + u * W, at = block * kBlock;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        bs[u][g] = sb[g][block];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) bv[u][g][h] = load16<SHIFT>(b + at + h * 64, b_off[g]);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        as[u][n] = sa[n][block];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) av[u][n][h] = load16<SHIFT>(a + at + h * 64, a_off[n]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < C; ++u)
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          acc[g][n] = OP::mac(OP::frag(bv[u][g][0], bv[u][g][1]), OP::frag(av[u][n][0], av[u][n][1]), acc[g][n], bs[u][g],
+                              as[u][n]);
+  };
+  int s = wave;
+  for (; s + (U - 1) * W < full; s += U * W) steps(std::integral_constant<int, U>{}, s);
+  for (; s < full; s += W) steps(std::integral_constant<int, 1>{}, s);
+  if (p.k % kBlock && s == full) {  // the last block of the sum, cut at K
+    const int at = full * kBlock;
+    i32x4 bv[G][2], av[NT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int left = p.k - at - h * 64 - 16 * q;
+#pragma unroll
+      for (int g = 0; g < G; ++g) bv[g][h] = load16_cut(b + at + h * 64, b_off[g], left);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) av[n][h] = load16_cut(a + at + h * 64, a_off[n], left);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        acc[g][n] = OP::mac(OP::frag(bv[g][0], bv[g][1]), OP::frag(av[n][0], av[n][1]), acc[g][n], sb[g][full], sa[n][full]);
+  }
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) red[(wave * G * NT + n * G + g) * 64 + lane] = acc[g][n];
+  __syncthreads();
+  for (int op = wave; op < G * NT; op += W) {
+    f32x4 v = red[op * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v += red[(w * G * NT + op) * 64 + lane];
+    const int row = m0 + op / G * 16 + j;
+    if (row < p.m) store4(p, row, n0 + op % G * 16 + 4 * q, v);
+  }
+}
+
+// ------------------------------------------------------------------ tiles through LDS
+// BM x BN tile of tile_sums; the KS groups' sums are joined in order, and 32 (or
+// 16) rows of a wave at a time go through its own LDS, padded to spread a pass
+// over the banks, so that neighbouring lanes store neighbouring 16 bytes.
+template <class OP, int BM, int BN, int WM, int WN, int KS, int PRE, bool SHIFT>
+__global__ __launch_bounds__(WM * WN * KS * 64) void fp8_tile_kernel(Fp8Args p) {
+  constexpr int NT = WM * WN * KS * 64, STEP = KS * BK, R = OP::R, MI = BM / WM / R, NI = BN / WN / R;
+  __shared__ __attribute__((aligned(1024))) int8_t smem[2][(BM + BN) * STEP];
+  const int num_m = (p.m + BM - 1) / BM, num_n = (p.n + BN - 1) / BN;
+  int mt, nt;
+  tile_of(num_m, num_n, mt, nt);
+  const int m0 = mt * BM, n0 = nt * BN;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ks = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
+  Panel<BM, NT, KS, SHIFT> pa;
+  Panel<BN, NT, KS, SHIFT> pb;
+  pa.init(p.a, p.lda, m0, p.m);
+  pb.init(p.b, p.ldb, n0, p.n);
+  const uint8_t* const sa0 = p.sa + static_cast<int64_t>(m0) * p.kb;
+  uint32_t sa_off[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+    sa_off[i] = static_cast<uint32_t>(min(wm * (BM / WM) + i * R + OP::token(lane), p.m - 1 - m0)) * static_cast<uint32_t>(p.kb);
+  auto sa = [&](int i, int block) -> uint32_t { return sa0[sa_off[i] + block]; };
+  static_assert(kBlock % (BN / WN) == 0, "a wave's channels share a scale");
+  const uint8_t* const sb0 = p.sb + static_cast<int64_t>(min(n0 + wn * (BN / WN), p.n - 1) / kBlock) * p.kb;
+  auto sb = [&](int, int block) -> uint32_t { return sb0[block]; };
+  typename OP::Acc acc[MI][NI];
+  tile_sums<OP, BM, BN, WM, WN, KS, PRE, 1>(smem, pa, pb, p.k, sa, sb, acc);
+
+  constexpr int COLS = BN / WN, PITCH = COLS * 4 + 16, PITCH16 = COLS * 2 + 16;  // bytes of a staged row
+  static_assert(WM * WN * R * PITCH <= sizeof(smem), "epilogue staging");
+  __syncthreads();
+  if constexpr (KS > 1) {  // group 0 adds the others' sums, one group at a time
+    static_assert(BM * BN * 4 <= sizeof(smem), "a group's sums");
+    f32x4* red = reinterpret_cast<f32x4*>(&smem[0][0]) + (wm * WN + wn) * (MI * NI * OP::QUADS * 64) + lane;
+    for (int k = 1; k < KS; ++k) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int g = 0; g < OP::QUADS; ++g)
+            if (ks == k)
+              red[((i * NI + j) * OP::QUADS + g) * 64] =
+                  f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int g = 0; g < OP::QUADS; ++g)
+            if (ks == 0) {
+              const f32x4 v = red[((i * NI + j) * OP::QUADS + g) * 64];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[i][j][4 * g + r] += v[r];
+            }
+      __syncthreads();
+    }
+    if (ks) return;
+  }
+  int8_t* const staged = &smem[0][0] + wave * (R * PITCH);
+  const int c0 = n0 + wn * COLS, lane_row = OP::token(lane);
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int r0 = m0 + wm * (BM / WM) + i * R;
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int g = 0; g < OP::QUADS; ++g) {
+        const int c = j * R + OP::channel(lane, g);
+        f32x4 f = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        if (p.bias) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) f[r] += load_any(p.bias, p.bias_type, min(c0 + c + r, p.n - 1));
+        }
+        if (p.out_type == MM_T_FP32)
+          *reinterpret_cast<f32x4*>(staged + lane_row * PITCH + c * 4) = f;
+        else
+          *reinterpret_cast<uint2*>(staged + lane_row * PITCH16 + c * 2) = pack4(f, p.out_type);
+      }
+    if (p.out_type == MM_T_FP32)
+      store_rows<R, COLS, PITCH, float>(p, staged, r0, c0);
+    else
+      store_rows<R, COLS, PITCH16, uint16_t>(p, staged, r0, c0);
+  }
+}
+
+// ------------------------------------------------------------------ choice
+int launch(void (*kernel)(Fp8Args), int64_t tiles, int threads, const Fp8Args& p, hipStream_t s) {
+  MM_CHECK_ARG(tiles * threads < (int64_t(1) << 32), "mm_fp8_matmul: too many tiles");
+  kernel<<<static_cast<uint32_t>(tiles), threads, 0, s>>>(p);
+  return mm_check_launch("fp8_matmul");
+}
+
+int64_t tiles_of(const Fp8Args& p, int bm, int bn) {
+  return ((static_cast<int64_t>(p.m) + bm - 1) / bm) * ((static_cast<int64_t>(p.n) + bn - 1) / bn);
+}
+
+template <class OP, int G, int NT, int W, int U>
+int launch_direct(const Fp8Args& p, bool shift, hipStream_t s) {
+  return launch(shift ? fp8_direct_kernel<OP, G, NT, W, U, true> : fp8_direct_kernel<OP, G, NT, W, U, false>,
+                tiles_of(p, NT * 16, G * 16), W * 64, p, s);
+}
+
+template <class OP, int BM, int BN, int WM, int WN, int KS, int PRE, bool SHIFT>
+int launch_tiles(const Fp8Args& p, hipStream_t s) {
+  return launch(fp8_tile_kernel<OP, BM, BN, WM, WN, KS, PRE, SHIFT>, tiles_of(p, BM, BN), WM * WN * KS * 64, p, s);
+}
+
+int launch_best(const Fp8Args& p, hipStream_t s) {
+  const bool shift = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.lda | p.ldb) & 3) != 0;
+  if (p.out_type == MM_T_FP32) {
+    if (p.m <= 16) return launch_direct<Op16Wide, 1, 1, 16, 2>(p, shift, s);
+    if (p.k < BK) return launch_direct<Op16Wide, 2, 2, 1, 1>(p, shift, s);
+    return launch_tiles<Op16Wide, 128, 128, 2, 2, 1, 1, false>(p, s);
+  }
+  if (p.m <= 16) return launch_direct<Op16, 1, 1, 16, 4>(p, shift, s);
+  if (p.k < BK) return launch_direct<Op16, 4, 4, 1, 1>(p, shift, s);  // not one whole stage
+  if (tiles_of(p, 256, 256) >= 256) return launch_tiles<Op32, 256, 256, 2, 2, 1, 1, false>(p, s);
+  return launch_tiles<Op32, 128, 128, 2, 2, 1, 2, false>(p, s);
+}
+
+bool is_float_type(int t) { return t == MM_T_BF16 || t == MM_T_FP16 || t == MM_T_FP32; }
+
+}  // namespace
+
+extern "C" int mm_fp8_matmul(const uint8_t* a, int64_t lda, const uint8_t* a_scale, const uint8_t* b, int64_t ldb,
+                             const uint8_t* b_scale, const void* bias, int32_t bias_type, int64_t m, int64_t n,
+                             int64_t k, void* out, int64_t ldo, int32_t out_type, mm_stream_t stream) {
+  MM_CHECK_ARG(m >= 0 && n > 0 && k > 0 && k <= kMaxStride && m < kMaxRows && n < kMaxRows,
+               "mm_fp8_matmul: bad sizes (%lld x %lld x %lld; K at most %lld)", static_cast<long long>(m),
+               static_cast<long long>(n), static_cast<long long>(k), static_cast<long long>(kMaxStride));
+  MM_CHECK_ARG(is_float_type(out_type) && (!bias || is_float_type(bias_type)), "mm_fp8_matmul: bad types");
+  MM_CHECK_ARG((m <= 1 || (lda >= k && lda <= kMaxStride)) && (n <= 1 || (ldb >= k && ldb <= kMaxStride)) &&
+                   (m <= 1 || ldo >= n),
+               "mm_fp8_matmul: bad strides (rows of a and b at least K and at most %lld apart)",
+               static_cast<long long>(kMaxStride));
+  if (m == 0) return MM_OK;
+  MM_CHECK_ARG(a && b && a_scale && b_scale && out, "mm_fp8_matmul: null pointer");
+  // a single row's stride is never stepped over
+  if (m == 1) lda = k;
+  if (n == 1) ldb = k;
+  const Fp8Args p{a,   b,   a_scale, b_scale, bias, out, lda, ldb, ldo, static_cast<int32_t>(m), static_cast<int32_t>(n),
+                  static_cast<int32_t>(k), static_cast<int32_t>((k + kBlock - 1) / kBlock), out_type, bias_type};
+  return launch_best(p, mm_hip_stream(stream));
+}

@@ -339,7 +339,7 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) 
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<f32x4*>(staged + lane_row * PITCH + (j * 32 + g * 8 + lane_col) * 4) = results(j, g);
-      store_rows<COLS, PITCH, float>(p, staged, m0 + r0, n0 + c0);
+      store_rows<32, COLS, PITCH, float>(p, staged, m0 + r0, n0 + c0);
     } else {
 #pragma unroll
       for (int j = 0; j < NI; ++j)
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void int8_tile_kernel(I8Args p) 
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<uint2*>(staged + lane_row * PITCH16 + (j * 32 + g * 8 + lane_col) * 2) =
               pack4(results(j, g), p.out_type);
-      store_rows<COLS, PITCH16, uint16_t>(p, staged, m0 + r0, n0 + c0);
+      store_rows<32, COLS, PITCH16, uint16_t>(p, staged, m0 + r0, n0 + c0);
     }
   }
 }

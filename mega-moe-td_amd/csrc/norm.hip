@@ -5,6 +5,7 @@
 //   y = h * r * w,  r = 1 / sqrt(mean(h^2) + eps)
 //   8 bits: s = max(a, 1e-30) / Q with a = max |y| over the row (s = 1 where
 //           a = 0), q = round(y / s) of the unrounded y; Q = 127 (int8) or 448 (E4M3)
+//   8 bits with a scale for each 128 columns: fp8.h's blocks of the unrounded y
 //   backward, with n = h r: dx = dh + r (w dy - n mean(w dy n)),  dw = sum_rows dy n
 //           (n is near 1 whatever the row's size; r^3 would leave fp32 from rows
 //           of 1e13 on)
@@ -16,7 +17,7 @@
 // Memory bound: every element is read once and written once. A row stays in
 // the registers of its TPR threads (NV vectors of 8 columns each) between the
 // sum of squares, the maximum and the output.
-#include "common.h"
+#include "fp8.h"
 
 namespace {
 
@@ -27,6 +28,7 @@ struct NormArgs {
   void* h;             // stored sum, given with res
   void* y;
   float* scale;        // per row, 8-bit outputs
+  uint8_t* block_scale;  // or per 128 columns (E4M3)
   float* rstd;         // per row, or NULL
   int64_t ldx, ldr, rows;
   int32_t hidden, w_type, y_type, norm;
@@ -216,7 +218,8 @@ __device__ __forceinline__ uint2 quantize8(const float* v, const Quantizer& z, b
 
 // Two vectors of 16 bits a thread fit the registers of six waves, which the
 // compiler misses by two of them by itself (8192 x 7168: 94 us, 87 so).
-template <class TX, class TH, int NV, bool WAVE>
+// BLOCKS: E4M3 with a scale for each 128 columns, which 16 neighbouring threads hold.
+template <class TX, class TH, int NV, bool WAVE, bool BLOCKS>
 __global__ __launch_bounds__(WAVE ? kWaveThreads : 1024)
 __attribute__((amdgpu_waves_per_eu(!WAVE && NV == 2 && sizeof(TX) + sizeof(TH) == 4 ? 6 : 4))) void rms_norm_kernel(NormArgs p) {
   __shared__ float sums[16];
@@ -253,7 +256,7 @@ __attribute__((amdgpu_waves_per_eu(!WAVE && NV == 2 && sizeof(TX) + sizeof(TH) =
         h.to_f32(v[u]);
       }
     }
-    const bool eight = p.y_type == MM_T_INT8 || p.y_type == MM_T_E4M3;
+    const bool eight = !BLOCKS && (p.y_type == MM_T_INT8 || p.y_type == MM_T_E4M3);
     float mant = 1.0f;
     if (p.norm) {
       float mean, k = 1.0f;
@@ -290,6 +293,29 @@ __attribute__((amdgpu_waves_per_eu(!WAVE && NV == 2 && sizeof(TX) + sizeof(TH) =
         for (int i = 0; i < 8; ++i) v[u][i] *= p.w ? r * w[i] : r;
       }
     }
+    if constexpr (BLOCKS) {
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        const int i0 = u * threads + t;
+        const Columns c(i0, H);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, c.counts(i) ? abs_bits(v[u][i]) : 0u);
+        const BlockScale s(max16(top));
+        if (!c.any()) continue;
+        if (i0 % 16 == 0) p.block_scale[row * ((H + kBlock - 1) / kBlock) + i0 / 16] = static_cast<uint8_t>(s.byte);
+        const uint2 q = make_uint2(s.pack4(v[u][0], v[u][1], v[u][2], v[u][3]), s.pack4(v[u][4], v[u][5], v[u][6], v[u][7]));
+        uint8_t* const y = static_cast<uint8_t*>(p.y) + row * H + c.at;
+        if (c.own <= 0) {
+          __builtin_memcpy(y, &q, 8);
+        } else {  // the columns before may belong to another block
+#pragma unroll
+          for (int i = 1; i < 8; ++i)
+            if (c.counts(i)) y[i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+        }
+      }
+      continue;
+    }
     if (!eight) {
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
@@ -316,7 +342,7 @@ __attribute__((amdgpu_waves_per_eu(!WAVE && NV == 2 && sizeof(TX) + sizeof(TH) =
 }
 
 // Rows of fewer than 8 columns: a thread has a row.
-template <class TX, class TH>
+template <class TX, class TH, bool BLOCKS>
 __global__ __launch_bounds__(256) void rms_norm_short_kernel(NormArgs p) {
   const int H = p.hidden;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; row < p.rows;
@@ -331,7 +357,7 @@ __global__ __launch_bounds__(256) void rms_norm_short_kernel(NormArgs p) {
       }
       ss += v[i] * v[i];
     }
-    const bool eight = p.y_type == MM_T_INT8 || p.y_type == MM_T_E4M3;
+    const bool eight = !BLOCKS && (p.y_type == MM_T_INT8 || p.y_type == MM_T_E4M3);
     float mant = 1.0f;
     if (p.norm) {
       float mean = ss / static_cast<float>(H) + p.eps, k = 1.0f;
@@ -352,6 +378,19 @@ __global__ __launch_bounds__(256) void rms_norm_short_kernel(NormArgs p) {
         r = split.pow2;
       }
       for (int i = 0; i < H; ++i) v[i] *= p.w ? r * load_any(p.w, p.w_type, i) : r;
+    }
+    if constexpr (BLOCKS) {
+      uint32_t top = 0;
+      for (int i = 0; i < 8; ++i) {
+        if (i >= H) v[i] = 0.0f;
+        top = max(top, abs_bits(v[i]));
+      }
+      const BlockScale s(top);
+      p.block_scale[row] = static_cast<uint8_t>(s.byte);
+      const uint2 q = make_uint2(s.pack4(v[0], v[1], v[2], v[3]), s.pack4(v[4], v[5], v[6], v[7]));
+      for (int i = 0; i < H; ++i)
+        static_cast<uint8_t*>(p.y)[row * H + i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+      continue;
     }
     if (!eight) {
       for (int i = 0; i < H; ++i) static_cast<TX*>(p.y)[row * H + i] = static_cast<TX>(v[i]);
@@ -579,12 +618,14 @@ struct LaunchFwd {
   int operator()(int threads) const {
     const int size = WAVE ? kWaveThreads : threads, rpb = WAVE ? kWaveRows : 1;
     const int64_t need = (p.rows + rpb - 1) / rpb, most = (int64_t(1) << 31) / size;
-    rms_norm_kernel<TX, TH, NV, WAVE><<<static_cast<uint32_t>(need < most ? need : most), size, 0, s>>>(p);
+    const auto kernel = p.block_scale ? rms_norm_kernel<TX, TH, NV, WAVE, true> : rms_norm_kernel<TX, TH, NV, WAVE, false>;
+    kernel<<<static_cast<uint32_t>(need < most ? need : most), size, 0, s>>>(p);
     return mm_check_launch("rms_norm_kernel");
   }
   int short_rows() const {
     const int64_t need = (p.rows + 255) / 256;
-    rms_norm_short_kernel<TX, TH><<<static_cast<uint32_t>(need < 65536 ? need : 65536), 256, 0, s>>>(p);
+    const auto kernel = p.block_scale ? rms_norm_short_kernel<TX, TH, true> : rms_norm_short_kernel<TX, TH, false>;
+    kernel<<<static_cast<uint32_t>(need < 65536 ? need : 65536), 256, 0, s>>>(p);
     return mm_check_launch("rms_norm_short_kernel");
   }
 };
@@ -666,7 +707,21 @@ extern "C" int mm_rms_norm(const void* x, int64_t ldx, int32_t x_type, const voi
   MM_CHECK_ARG(eight || y_type == x_type, "mm_rms_norm: the output has the input's type or 8 bits");
   if (rows == 0) return MM_OK;
   MM_CHECK_ARG(x && y && (!residual || h_out) && (!eight || scale), "mm_rms_norm: null pointer");
-  const NormArgs p{x, residual, weight, h_out, y, scale, rstd, ldx, ldr, rows, hidden, weight_type, y_type, 1, eps};
+  const NormArgs p{x, residual, weight, h_out, y, scale, nullptr, rstd, ldx, ldr, rows, hidden, weight_type, y_type, 1, eps};
+  return by_types<false, LaunchFwd>(x_type, residual ? h_type : x_type, hidden, p, mm_hip_stream(stream));
+}
+
+extern "C" int mm_rms_norm_blocks(const void* x, int64_t ldx, int32_t x_type, const void* residual, int64_t ldr,
+                                  int32_t h_type, const void* weight, int32_t weight_type, int64_t rows, int32_t hidden,
+                                  float eps, void* h_out, uint8_t* q, uint8_t* scale, mm_stream_t stream) {
+  MM_CHECK_ARG(rows_ok(rows) && hidden > 0 && hidden <= kMaxHidden, "mm_rms_norm_blocks: bad sizes (rows %lld, hidden %d)",
+               static_cast<long long>(rows), hidden);
+  MM_CHECK_ARG(is_float_type(x_type) && (h_type == x_type || h_type == MM_T_FP32) && (!weight || is_float_type(weight_type)),
+               "mm_rms_norm_blocks: bad types");
+  if (rows == 0) return MM_OK;
+  MM_CHECK_ARG(x && q && scale && (!residual || h_out), "mm_rms_norm_blocks: null pointer");
+  const NormArgs p{x,   residual, weight, h_out, q,           nullptr,     scale, nullptr,
+                   ldx, ldr,      rows,   hidden, weight_type, MM_T_E4M3, 1,     eps};
   return by_types<false, LaunchFwd>(x_type, residual ? h_type : x_type, hidden, p, mm_hip_stream(stream));
 }
 
@@ -677,7 +732,7 @@ extern "C" int mm_quantize_rows(const void* x, int64_t ldx, int32_t x_type, int6
   MM_CHECK_ARG(is_float_type(x_type) && (q_type == MM_T_INT8 || q_type == MM_T_E4M3), "mm_quantize_rows: bad types");
   if (rows == 0) return MM_OK;
   MM_CHECK_ARG(x && q && scale, "mm_quantize_rows: null pointer");
-  const NormArgs p{x, nullptr, nullptr, nullptr, q, scale, nullptr, ldx, 0, rows, cols, 0, q_type, 0, 0.0f};
+  const NormArgs p{x, nullptr, nullptr, nullptr, q, scale, nullptr, nullptr, ldx, 0, rows, cols, 0, q_type, 0, 0.0f};
   return by_types<false, LaunchFwd>(x_type, x_type, cols, p, mm_hip_stream(stream));
 }
 

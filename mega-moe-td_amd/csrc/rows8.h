@@ -2,6 +2,8 @@
 // stages in LDS and the way of results to memory.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -104,6 +106,7 @@ template <int ROWS, int NT, int KS, bool SHIFT>
 struct Panel {
   static constexpr int VPR = 8 * KS, PER = ROWS * VPR / NT;  // 16-byte vectors a row, a thread
   static_assert(PER * NT == ROWS * VPR && NT % VPR == 0, "whole vectors");
+  static constexpr bool CUTS = true;  // has put_cut
   // A run: consecutive lanes with consecutive vectors of a row, within the 16
   // lanes that exchange words.
   static constexpr int LAST = VPR < 16 ? VPR - 1 : 15;
@@ -167,15 +170,15 @@ struct Panel {
   }
 };
 
-// 32 staged rows of a wave to memory, 16 bytes a lane.
-template <int COLS, int PITCH, class T, class Args>
+// ROWS staged rows of a wave to memory, 16 bytes a lane.
+template <int ROWS, int COLS, int PITCH, class T, class Args>
 __device__ __forceinline__ void store_rows(const Args& p, const int8_t* staged, int row0, int col0) {
   constexpr int PER = 16 / sizeof(T), LANES = COLS / PER;  // columns a lane, lanes a row
   const int lane = threadIdx.x & 63, r0 = lane / LANES, c = lane % LANES * PER, left = p.n - col0 - c;
   T* out = static_cast<T*>(p.out) + (row0 + r0) * p.ldo + col0 + c;
   const int64_t step = 64 / LANES * p.ldo;
 #pragma unroll
-  for (int r = 0; r < 32; r += 64 / LANES, out += step) {
+  for (int r = 0; r < ROWS; r += 64 / LANES, out += step) {
     if (row0 + r0 + r >= p.m) break;
     const int8_t* from = staged + (r0 + r) * PITCH + c * sizeof(T);
     if (left >= PER) {

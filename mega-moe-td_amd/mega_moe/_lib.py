@@ -80,6 +80,13 @@ SIGNATURES = {
     "mm_rms_norm_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I32, _P, _I32, _I32, _I64, _I32, _P, _P, _P,
                                        _P, _SZ, _P]),
     "mm_quantize_rows": (ctypes.c_int, [_P, _I64, _I32, _I64, _I32, _P, _I32, _P, _P]),
+    "mm_quantize_blocks": (ctypes.c_int, [_P, _I64, _I64, _I32, _I64, _I64, _I64, _I32, _P, _I64, _P, _P]),
+    "mm_quantize_blocks_t": (ctypes.c_int, [_P, _I64, _I32, _P, _I64, _I64, _I32, _P, _P, _P, _P, _P]),
+    "mm_rms_norm_blocks": (ctypes.c_int, [_P, _I64, _I32, _P, _I64, _I32, _P, _I32, _I64, _I32, _F32, _P, _P, _P, _P]),
+    "mm_fp8_matmul": (ctypes.c_int, [_P, _I64, _P, _P, _I64, _P, _P, _I32, _I64, _I64, _I64, _P, _I64, _I32, _P]),
+    "mm_moe_fp8_scratch_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32]),
+    "mm_moe_fp8": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F32, _F32, _F32,
+                                  _P, _P, _SZ, _P]),
     "mm_int8_matmul": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _I32, _I64, _I64, _I64, _P, _I64, _I32, _P]),
 }
 

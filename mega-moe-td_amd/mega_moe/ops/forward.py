@@ -35,6 +35,7 @@ from ._saved import MoESaved
 from ..runtime.timing import StageTimer
 from .. import _lib
 from . import _kernels as K
+from .fp8 import Fp8Experts
 from .int8 import Int8Experts
 
 # Device-kernel limits (csrc/routing.hip kMaxExperts, csrc/rowops.hip combine slots).
@@ -389,7 +390,7 @@ class FusedMoEForward(torch.nn.Module):
         of the first call."""
         ops = _lib.torch_ops()
         lbeta = self.situ_linear_beta
-        of = (min(MAX_FEW_TOKENS, self.max_tokens_per_rank), self.top_k, self.experts_per_rank, self.hidden_size,
+        of = (self.max_tokens_per_rank, self.top_k, self.experts_per_rank, self.hidden_size,
               _lib.ACT_KINDS[self.activation], self.situ_beta, 0.0 if lbeta is None else lbeta, self.clamp_limit)
         if of != self._few_of:  # the attributes may change between calls, as forward reads them at each
             self._few, self._few_of = ops.Layer(*of), of
@@ -469,6 +470,51 @@ class FusedMoEForward(torch.nn.Module):
         self._validate_few_sizes(two_inter)
         if hidden >= MAX_INT8_SUM:
             raise ValueError(f"hidden_size must be below {MAX_INT8_SUM} for exact int32 sums, got {hidden}")
+        device = selected_experts.device
+        if tokens.device != device or token_scale.device != device or experts.gate_up.device != device:
+            raise ValueError("tokens, token_scale, selected_experts and experts must be on the same device")
+        raise ValueError("the operands do not fit the operator")
+
+    # ------------------------------------------------------------ E4M3 rows and experts
+    def forward_fp8(self, tokens, token_scale, selected_experts, experts: Fp8Experts, routing_weights):
+        """The forward on E4M3 rows and E4M3 experts with a scale for each block of
+        128, for one token to ``max_tokens_per_rank``.
+
+        ``tokens`` float8_e4m3fn [T, H] with float8_e8m0fnu ``token_scale``
+        [T, H / 128], as ``rms_norm`` (``scale_columns=128``) and
+        ``quantize_blocks`` make them; returns bf16 [T, H]. Sums are fp32; the
+        activation (times the routing weight) goes to FC2 in E4M3 with a scale for
+        each 128 columns, and the experts' outputs to the sum over the slots in
+        bf16. A NaN scale makes its own token's output NaN (where any slot of the
+        token has an expert) and no other's. Nothing is saved for a backward and
+        operands that ask for a gradient are refused; no workspace of the operator
+        is used, so calls may run on any stream and captured. No counterpart in
+        the reference.
+        """
+        if not isinstance(experts, Fp8Experts):
+            raise TypeError("experts must be an Fp8Experts")
+        ops, layer = self._few_layer(tokens)
+        out = ops.layer_forward_fp8(layer, tokens, token_scale, selected_experts, experts.gate_up,
+                                    experts.gate_up_scale, experts.down, experts.down_scale, routing_weights)
+        if out is not None:
+            return out
+        # the operands do not fit the layer: one of these checks says why
+        self._validate_topk_indices(selected_experts)
+        expected = (selected_experts.shape[0], self.hidden_size)
+        if tokens.dtype != torch.float8_e4m3fn:
+            raise TypeError(f"tokens must use torch.float8_e4m3fn, got {tokens.dtype}")
+        if tuple(tokens.shape) != expected or not tokens.is_contiguous():
+            raise ValueError(f"tokens must be contiguous with shape {expected}, got {tuple(tokens.shape)}")
+        scales = (expected[0], self.hidden_size // 128)
+        if (token_scale.dtype != torch.float8_e8m0fnu or tuple(token_scale.shape) != scales
+                or not token_scale.is_contiguous()):
+            raise ValueError(f"token_scale must be contiguous float8_e8m0fnu with shape {scales}")
+        self._validate_routing_weights(routing_weights, selected_experts)
+        num_experts, two_inter, hidden = experts.gate_up.shape
+        if num_experts != self.experts_per_rank or hidden != self.hidden_size:
+            raise ValueError(f"experts hold {num_experts} experts of hidden size {hidden}, expected "
+                             f"{self.experts_per_rank} of {self.hidden_size}")
+        self._validate_few_sizes(two_inter)
         device = selected_experts.device
         if tokens.device != device or token_scale.device != device or experts.gate_up.device != device:
             raise ValueError("tokens, token_scale, selected_experts and experts must be on the same device")

@@ -20,7 +20,7 @@ MAX_HIDDEN = 32768  # columns of a row (csrc/norm.hip)
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
-             eps: float = 1e-6, out_dtype: Optional[torch.dtype] = None):
+             eps: float = 1e-6, out_dtype: Optional[torch.dtype] = None, scale_columns: Optional[int] = None):
     """``h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, with
     ``h = x + residual`` (rounded to the residual's type) or ``h = x``.
 
@@ -34,14 +34,17 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
     ``out_dtype`` int8 or float8_e4m3fn ``y`` is replaced by ``q, scale``:
     ``y`` = ``q * scale[..., None]``, one fp32 scale a row (largest ``|y|`` /
     127 or 448; 1 for a row of zeros; NaN, with bytes of zero, for a row that
-    holds a NaN or an infinity).
+    holds a NaN or an infinity). With float8_e4m3fn and ``scale_columns`` = 128
+    there is one float8_e8m0fnu scale for each 128 columns instead, ``scale``
+    [..., ceil(H / 128)], as ``quantize_blocks`` makes them of the unrounded
+    ``y``: what ``fp8_matmul`` and ``FusedMoEForward.forward_fp8`` take.
 
     Differentiable in ``x``, ``weight`` and ``residual`` (once) where the output
     is floating; 8-bit outputs carry no gradient and refuse inputs that ask for
     one. A captured backward raises while a graph built on the default stream
     still uses the same leaves.
     """
-    return _lib.torch_ops().rms_norm(x, weight, residual, eps, out_dtype)
+    return _lib.torch_ops().rms_norm(x, weight, residual, eps, out_dtype, scale_columns)
 
 
 def quantize_rows(x: torch.Tensor, dtype: torch.dtype = torch.int8):
