@@ -556,7 +556,7 @@ int mm_fp8_matmul(const uint8_t* a, int64_t lda, const uint8_t* a_scale, const u
  * rows) and w2 [E, hidden, inter] with scales for each 128 x 128; all
  * contiguous, hidden and inter multiples of 128. The activation (fp32, times
  * the routing weight) goes to FC2 in E4M3 with a scale for each 128 columns, the
- * experts' outputs to the sum over the slots in bf16. Routing as mm_route; a
+ * experts' outputs to the sum over the slots in fp32. Routing as mm_route; a
  * NaN scale of a row makes that row's output NaN where any slot of it has an
  * expert. Scratch of mm_moe_fp8_scratch_bytes (0 for sizes out of range), 16-byte
  * aligned like out, free again when the stream has passed the call.

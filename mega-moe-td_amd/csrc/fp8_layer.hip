@@ -3,10 +3,12 @@
 //
 //   gu[i, :]  = x[token(i), :] W1[e]^T                 (fp32, e = expert of expert-major row i)
 //   act[i, :] = act_fn(gate, up) * w[i], then E4M3 with a scale for each 128 columns
-//   y[i, :]   = act[i, :] W2[e]^T                      (bf16)
+//   y[i, :]   = act[i, :] W2[e]^T                      (fp32)
 //   out[t, :] = sum_j y[route_to_send[t k + j], :]     (fp32, slot order)
 //
-// Routing tables, tile lists and the top-k sum are those of the bf16 layer.
+// Routing tables and tile lists are those of the bf16 layer. The experts' outputs
+// stay in fp32 until the slots are summed: in bf16 each would be off by as much
+// as the result is by its own rounding.
 #include "fp8_tile.h"
 
 namespace {
@@ -18,7 +20,7 @@ struct LayerArgs {
   const uint8_t* w;     // [E, C, K]
   const uint8_t* ws;    // [E, C / 128, K / 128]
   const float* weight;  // routing weight of row i (FC1)
-  void* out;            // E4M3 [R, I] (FC1) or bf16 [R, C]
+  void* out;            // E4M3 [R, I] (FC1) or fp32 [R, C]
   uint8_t* out_scale;   // [R, I / 128] (FC1)
   const TileList* tl;
   int32_t k, c, inter, act_kind;
@@ -135,10 +137,193 @@ __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(LayerArgs p) {
         if (i >= t.z) continue;
 #pragma unroll
         for (int g = 0; g < 2; ++g)
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + static_cast<int64_t>(i) * p.c + c0 + g * 16 + 4 * q) =
-              make_uint2(pack_bf16x2(acc[g][n][0], acc[g][n][1]), pack_bf16x2(acc[g][n][2], acc[g][n][3]));
+          *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + static_cast<int64_t>(i) * p.c + c0 + g * 16 + 4 * q) = acc[g][n];
       }
     }
+  }
+}
+
+// ------------------------------------------------------------------ many rows an expert
+// Rows of K bytes, K a multiple of 128: 16-byte vectors of a stage, NT threads.
+template <int ROWS, int NT>
+struct RowPanel {
+  static constexpr int PER = ROWS * 8 / NT;
+  static constexpr bool CUTS = false;
+  static_assert(PER * NT == ROWS * 8, "whole vectors");
+  struct Stage {
+    i32x4 d[PER];
+  };
+  const uint8_t* base;
+  uint32_t off[PER];  // in 16 bytes, so that rows may lie 64 GB apart
+  // row(r): index of the panel's r-th row
+  template <class F>
+  __device__ __forceinline__ RowPanel(const uint8_t* p, int K, const F& row) : base(p) {
+#pragma unroll
+    for (int v = 0; v < PER; ++v) {
+      const int c = v * NT + threadIdx.x;
+      off[v] = static_cast<uint32_t>(row(c / 8)) * (static_cast<uint32_t>(K) / 16) + c % 8;
+    }
+  }
+  __device__ __forceinline__ void load(Stage& r, int k) const {
+#pragma unroll
+    for (int v = 0; v < PER; ++v) __builtin_memcpy(&r.d[v], base + k + (static_cast<uint64_t>(off[v]) << 4), 16);
+  }
+  __device__ __forceinline__ void put(int8_t* lds, const Stage& r) const {
+#pragma unroll
+    for (int v = 0; v < PER; ++v) {
+      const int c = v * NT + threadIdx.x;
+      *reinterpret_cast<i32x4*>(lds + slot_of(c / 8, c % 8)) = r.d[v];
+    }
+  }
+  __device__ __forceinline__ void put_cut(int8_t*, int, int) const {}
+};
+
+// One tile of 32 MI WM rows of an expert by 256 channels: with FC1 128 columns
+// of the activation, a wave's channels gate and up of the same columns.
+template <bool FC1, int MI, int WM, int WN, int PRE>
+__device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const int4& t, int r0, int cb) {
+  constexpr int BM = 32 * MI * WM, BN = 256, NT = WM * WN * 64, COLS = BN / WN, NI = COLS / 32, Q = Op32::QUADS;
+  constexpr int GATE = NI / 2;  // tiles of gate channels (FC1)
+  auto& smem = *reinterpret_cast<int8_t(*)[2][(BM + BN) * BK]>(lds);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  const int kb = p.k / kBlock;
+  const uint8_t* const ws = p.ws + static_cast<int64_t>(t.x) * (p.c / kBlock) * kb;
+  auto token = [&](int r) {
+    const int i = min(r0 + r, t.z - 1);
+    return p.rows ? p.rows[i] : i;
+  };
+  auto channel = [&](int r) {
+    if (!FC1) return min(cb * BN + r, p.c - 1);
+    const int w = r / COLS, c = r % COLS;
+    return cb * kBlock + w * (COLS / 2) + c % (COLS / 2) + (c < COLS / 2 ? 0 : p.inter);
+  };
+  // a tile's rows of x lie anywhere; those of act from its first one on
+  const RowPanel<BM, NT> pa(p.x, p.k, token);
+  const RowPanel<BN, NT> pb(p.w + static_cast<int64_t>(t.x) * p.c * p.k, p.k, channel);
+  const uint8_t* xs[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) xs[i] = p.xs + static_cast<int64_t>(token(wm * 32 * MI + i * 32 + Op32::token(lane))) * kb;
+  auto sa = [&](int i, int block) -> uint32_t { return xs[i][block]; };
+  constexpr int NB = FC1 ? 2 : 1;
+  const int sb0 = FC1 ? cb : min(cb * BN + wn * COLS, p.c - 1) / kBlock, sb1 = FC1 ? p.inter / kBlock + cb : 0;
+  auto sb = [&](int h, int block) -> uint32_t { return ws[static_cast<int64_t>(h ? sb1 : sb0) * kb + block]; };
+  f32x16 acc[MI][NI];
+  tile_sums<Op32, BM, BN, WM, WN, 1, PRE, NB>(smem, pa, pb, p.k, sa, sb, acc);
+  __syncthreads();  // the stages are read
+
+  if constexpr (FC1) {
+    constexpr int PITCH = kBlock + 16;
+    static_assert(BM * PITCH + WN * BM * 4 <= sizeof(smem), "epilogue staging");
+    int8_t* const staged = lds;
+    uint32_t* const tops = reinterpret_cast<uint32_t*>(lds + BM * PITCH);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int r = wm * 32 * MI + i * 32 + Op32::token(lane);
+      const float weight = p.weight[min(r0 + r, t.z - 1)];
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < GATE; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float a = gated_act(p.act_kind, acc[i][j][v], acc[i][j + GATE][v], p.beta, p.lbeta, p.limit) * weight;
+          acc[i][j][v] = a;
+          top = max(top, abs_bits(a));
+        }
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+      if (lane < 32) tops[wn * BM + r] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int r = wm * 32 * MI + i * 32 + Op32::token(lane);
+      uint32_t top = 0;
+#pragma unroll
+      for (int w = 0; w < WN; ++w) top = max(top, tops[w * BM + r]);
+      const BlockScale s(top);
+      if (wn == 0 && lane < 32 && r0 + r < t.z)
+        p.out_scale[static_cast<int64_t>(r0 + r) * (p.inter / kBlock) + cb] = static_cast<uint8_t>(s.byte);
+#pragma unroll
+      for (int j = 0; j < GATE; ++j)
+#pragma unroll
+        for (int g = 0; g < Q; ++g)
+          *reinterpret_cast<uint32_t*>(staged + r * PITCH + wn * (COLS / 2) + j * 32 + Op32::channel(lane, g)) =
+              s.pack4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+    }
+    __syncthreads();
+    for (int v = threadIdx.x; v < BM * 8; v += NT) {
+      const int r = v / 8, c = v % 8 * 16;
+      if (r0 + r < t.z)
+        *reinterpret_cast<i32x4*>(static_cast<uint8_t*>(p.out) + static_cast<int64_t>(r0 + r) * p.inter + cb * kBlock + c) =
+            *reinterpret_cast<const i32x4*>(staged + r * PITCH + c);
+    }
+  } else {
+    constexpr int PITCH = COLS * 4 + 16;
+    static_assert(WM * WN * 32 * PITCH <= sizeof(smem), "epilogue staging");
+    int8_t* const staged = lds + wave * (32 * PITCH);
+    struct {
+      void* out;
+      int64_t ldo;
+      int32_t m, n;
+    } to{p.out, p.c, t.z, p.c};
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int g = 0; g < Q; ++g)
+          *reinterpret_cast<f32x4*>(staged + Op32::token(lane) * PITCH + (j * 32 + Op32::channel(lane, g)) * 4) =
+              f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+      store_rows<32, COLS, PITCH, float>(to, staged, r0 + wm * 32 * MI + i * 32, cb * BN + wn * COLS);
+    }
+  }
+}
+
+// A tile list's tile and a run of 256 channels (128 columns of the activation)
+// a workgroup. Tile m runs on XCD m % 8 with all its channels, so that its rows
+// come from one L2. The instructions fit the tile's rows: tiles of experts with
+// fewer do not multiply what is not there.
+template <bool FC1, int ROWS>
+__global__ __launch_bounds__(256) void fp8_rows_kernel(LayerArgs p) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds[2 * (ROWS + 256) * BK];
+  const int cblocks = FC1 ? p.inter / kBlock : (p.c + 255) / 256;
+  const int slot = blockIdx.x >> 3, tile = slot / cblocks * 8 + (blockIdx.x & 7), cb = slot % cblocks;
+  if (tile >= p.tl->count) return;
+  const int4 t = p.tl->tiles[tile];
+  const int rows = t.z - t.y;
+  if constexpr (ROWS == kStreamRows) {
+    if (rows <= 32) return rows_tile<FC1, 1, 1, 4, 1>(p, lds, t, t.y, cb);
+    if (rows <= 64) return rows_tile<FC1, 2, 1, 4, 1>(p, lds, t, t.y, cb);
+    if (rows <= 96) return rows_tile<FC1, 3, 1, 4, 1>(p, lds, t, t.y, cb);
+    if (rows <= 128) return rows_tile<FC1, 4, 1, 4, 1>(p, lds, t, t.y, cb);
+    rows_tile<FC1, 5, 1, 4, 1>(p, lds, t, t.y, cb);
+  } else {
+    if (rows <= 128) return rows_tile<FC1, 2, 2, 2, 1>(p, lds, t, t.y, cb);
+    rows_tile<FC1, 4, 2, 2, 1>(p, lds, t, t.y, cb);
+  }
+}
+
+// out[t, :] = sum of the token's slots in slot order; a thread has 8 columns.
+__global__ __launch_bounds__(256) void fp8_combine_kernel(const float* y, const int32_t* route_to_send, int64_t tokens,
+                                                          int32_t top_k, int32_t hidden, uint16_t* out) {
+  const int chunks = hidden / 8;
+  const int64_t total = tokens * chunks;
+  for (int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; v < total; v += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t token = v / chunks;
+    const int c = static_cast<int>(v - token * chunks) * 8;
+    float sum[8] = {};
+    for (int j = 0; j < top_k; ++j) {
+      const int32_t row = route_to_send[token * top_k + j];
+      if (row < 0) continue;
+      const f32x4* from = reinterpret_cast<const f32x4*>(y + static_cast<int64_t>(row) * hidden + c);
+      const f32x4 a = from[0], b = from[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum[i] += a[i];
+        sum[4 + i] += b[i];
+      }
+    }
+    *reinterpret_cast<uint4*>(out + token * hidden + c) =
+        make_uint4(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]), pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7]));
   }
 }
 
@@ -159,7 +344,7 @@ struct Scratch {
   float* weight_perm;
   void *tiles, *route_ws;
   uint8_t *act, *act_scale;
-  uint16_t* y;
+  float* y;
   size_t tiles_bytes, route_ws_bytes, bytes;
 
   Scratch(void* base, int64_t R, int E, int hidden, int inter) {
@@ -167,7 +352,7 @@ struct Scratch {
     const size_t r = static_cast<size_t>(R);
     tiles_bytes = mm_tile_lists_bytes(R, E);
     route_ws_bytes = mm_route_workspace_bytes(R, E);
-    y = c.take<uint16_t>(r * hidden * 2);
+    y = c.take<float>(r * hidden * 4);
     act = c.take<uint8_t>(r * inter);
     act_scale = c.take<uint8_t>(r * (inter / kBlock));
     route_ws = c.take<void>(route_ws_bytes);
@@ -184,10 +369,13 @@ struct Scratch {
 
 constexpr int kMaxDim = 1 << 20;
 
+// Rows of x and act, and an expert's weights, in 32-bit offsets of 16 bytes.
 bool layer_sizes_ok(int64_t tokens, int32_t top_k, int32_t E, int32_t hidden, int32_t inter) {
+  constexpr int64_t most = int64_t(1) << 32;
   return tokens >= 0 && top_k > 0 && top_k <= 64 && E > 0 && E <= 32768 && hidden > 0 && inter > 0 &&
          hidden <= kMaxDim && inter <= kMaxDim && hidden % kBlock == 0 && inter % kBlock == 0 &&
-         tokens < (int64_t(1) << 31) / top_k;
+         tokens < (int64_t(1) << 31) / top_k && tokens * (hidden / 16) < most && tokens * top_k * (inter / 16) < most &&
+         static_cast<int64_t>(inter) * (hidden / 8) < most;
 }
 
 int launch(void (*kernel)(LayerArgs), int64_t blocks, int threads, const LayerArgs& p, hipStream_t s) {
@@ -227,14 +415,27 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
                           s.route_to_send, s.weight_perm, s.tiles, s.tiles_bytes, s.route_ws, s.route_ws_bytes, stream);
   if (rc) return rc;
   const hipStream_t hs = mm_hip_stream(stream);
-  const TileList* tl = mm_tile_list_of(s.tiles, R, E, kStreamRows);
-  const int64_t tiles = mm_max_m_tiles(R, E, kStreamRows);
+  // rows an expert on average
+  const int64_t mean = (R + E - 1) / E;
+  const int height = mean > kStreamRows ? 256 : kStreamRows;
+  const TileList* tl = mm_tile_list_of(s.tiles, R, E, height);
+  const int64_t tiles = mm_max_m_tiles(R, E, height), tiles8 = (tiles + 7) / 8 * 8;
   const LayerArgs fc1{x, x_scale, s.send_token, w1, w1_scale, s.weight_perm, s.act, s.act_scale, tl, hidden, 2 * inter, inter,
                       act_kind, situ_beta, situ_linear_beta, clamp_limit};
-  rc = launch(fp8_stream_kernel<true, 2, 8, 2>, tiles * (inter / kBlock), 512, fc1, hs);
-  if (rc) return rc;
   const LayerArgs fc2{s.act, s.act_scale, nullptr, w2, w2_scale, nullptr, s.y, nullptr, tl, inter, hidden, inter, 0, 0, 0, 0};
-  rc = launch(fp8_stream_kernel<false, 2, 4, 2>, tiles * (hidden / 128), 256, fc2, hs);
+  if (mean <= 16) {
+    rc = launch(fp8_stream_kernel<true, 1, 8, 2>, tiles * (inter / kBlock), 512, fc1, hs);
+    if (!rc) rc = launch(fp8_stream_kernel<false, 1, 4, 2>, tiles * (hidden / kBlock), 256, fc2, hs);
+  } else {
+    rc = launch(height == 256 ? fp8_rows_kernel<true, 256> : fp8_rows_kernel<true, kStreamRows>, tiles8 * (inter / kBlock),
+                256, fc1, hs);
+    if (!rc)
+      rc = launch(height == 256 ? fp8_rows_kernel<false, 256> : fp8_rows_kernel<false, kStreamRows>,
+                  tiles8 * ((hidden + 255) / 256), 256, fc2, hs);
+  }
   if (rc) return rc;
-  return mm_combine(s.y, hidden, s.route_to_send, tokens, top_k, hidden, out, hidden, stream);
+  const int64_t groups = (tokens * (hidden / 8) + 255) / 256;
+  fp8_combine_kernel<<<static_cast<uint32_t>(groups < 65536 ? groups : 65536), 256, 0, hs>>>(s.y, s.route_to_send, tokens, top_k,
+                                                                                             hidden, out);
+  return mm_check_launch("fp8_combine_kernel");
 }

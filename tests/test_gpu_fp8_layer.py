@@ -68,7 +68,7 @@ def reference(x, sx, sel, ex, w, act):
         y = av @ w2.t()
         dy = dq @ w2.abs().t() + R.sum_error(av, w2)
         out.index_add_(0, token, y)
-        bound.index_add_(0, token, dy + step * (y.abs() + dy))
+        bound.index_add_(0, token, dy)
     k = sel.shape[1]
     return out, bound + step * (out.abs() + bound) + k * 2.0 ** -23 * out.abs()
 
