@@ -156,12 +156,12 @@ __global__ __launch_bounds__(W * 64) void fp8_direct_kernel(Fp8Args p) {
 }
 
 // ------------------------------------------------------------------ tiles through LDS
-// BM x BN tile of tile_sums; the KS groups' sums are joined in order, and 32 (or
-// 16) rows of a wave at a time go through its own LDS, padded to spread a pass
+// BM x BN tile of tile_sums; the KS groups' sums are joined in order, and 16 rows
+// of a wave at a time go through its own LDS, padded to spread a pass
 // over the banks, so that neighbouring lanes store neighbouring 16 bytes.
 template <class OP, int BM, int BN, int WM, int WN, int KS, int PRE, bool SHIFT>
 __global__ __launch_bounds__(WM * WN * KS * 64) void fp8_tile_kernel(Fp8Args p) {
-  constexpr int NT = WM * WN * KS * 64, STEP = KS * BK, R = OP::R, MI = BM / WM / R, NI = BN / WN / R;
+  constexpr int NT = WM * WN * KS * 64, STEP = KS * BK, R = kTile, MI = BM / WM / R, NI = BN / WN / R;
   __shared__ __attribute__((aligned(1024))) int8_t smem[2][(BM + BN) * STEP];
   const int num_m = (p.m + BM - 1) / BM, num_n = (p.n + BN - 1) / BN;
   int mt, nt;
@@ -169,20 +169,20 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void fp8_tile_kernel(Fp8Args p) 
   const int m0 = mt * BM, n0 = nt * BN;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ks = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
-  Panel<BM, NT, KS, SHIFT> pa;
-  Panel<BN, NT, KS, SHIFT> pb;
+  Panel<BM, NT, KS, SHIFT, true> pa;
+  Panel<BN, NT, KS, SHIFT, true> pb;
   pa.init(p.a, p.lda, m0, p.m);
   pb.init(p.b, p.ldb, n0, p.n);
   const uint8_t* const sa0 = p.sa + static_cast<int64_t>(m0) * p.kb;
   uint32_t sa_off[MI];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
-    sa_off[i] = static_cast<uint32_t>(min(wm * (BM / WM) + i * R + OP::token(lane), p.m - 1 - m0)) * static_cast<uint32_t>(p.kb);
+    sa_off[i] = static_cast<uint32_t>(min(wm * (BM / WM) + i * R + token_of(lane), p.m - 1 - m0)) * static_cast<uint32_t>(p.kb);
   auto sa = [&](int i, int block) -> uint32_t { return sa0[sa_off[i] + block]; };
   static_assert(kBlock % (BN / WN) == 0, "a wave's channels share a scale");
   const uint8_t* const sb0 = p.sb + static_cast<int64_t>(min(n0 + wn * (BN / WN), p.n - 1) / kBlock) * p.kb;
   auto sb = [&](int, int block) -> uint32_t { return sb0[block]; };
-  typename OP::Acc acc[MI][NI];
+  f32x4 acc[MI][NI];
   tile_sums<OP, BM, BN, WM, WN, KS, PRE, 1>(smem, pa, pb, p.k, sa, sb, acc);
 
   constexpr int COLS = BN / WN, PITCH = COLS * 4 + 16, PITCH16 = COLS * 2 + 16;  // bytes of a staged row
@@ -190,53 +190,43 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void fp8_tile_kernel(Fp8Args p) 
   __syncthreads();
   if constexpr (KS > 1) {  // group 0 adds the others' sums, one group at a time
     static_assert(BM * BN * 4 <= sizeof(smem), "a group's sums");
-    f32x4* red = reinterpret_cast<f32x4*>(&smem[0][0]) + (wm * WN + wn) * (MI * NI * OP::QUADS * 64) + lane;
+    f32x4* red = reinterpret_cast<f32x4*>(&smem[0][0]) + (wm * WN + wn) * (MI * NI * 64) + lane;
     for (int k = 1; k < KS; ++k) {
+      if (ks == k) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
-#pragma unroll
-          for (int g = 0; g < OP::QUADS; ++g)
-            if (ks == k)
-              red[((i * NI + j) * OP::QUADS + g) * 64] =
-                  f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+          for (int j = 0; j < NI; ++j) red[(i * NI + j) * 64] = acc[i][j];
+      }
       __syncthreads();
+      if (ks == 0) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
-#pragma unroll
-          for (int g = 0; g < OP::QUADS; ++g)
-            if (ks == 0) {
-              const f32x4 v = red[((i * NI + j) * OP::QUADS + g) * 64];
-#pragma unroll
-              for (int r = 0; r < 4; ++r) acc[i][j][4 * g + r] += v[r];
-            }
+          for (int j = 0; j < NI; ++j) acc[i][j] += red[(i * NI + j) * 64];
+      }
       __syncthreads();
     }
     if (ks) return;
   }
   int8_t* const staged = &smem[0][0] + wave * (R * PITCH);
-  const int c0 = n0 + wn * COLS, lane_row = OP::token(lane);
+  const int c0 = n0 + wn * COLS, lane_row = token_of(lane);
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int r0 = m0 + wm * (BM / WM) + i * R;
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
+    for (int j = 0; j < NI; ++j) {
+      const int c = j * R + channel_of(lane);
+      f32x4 f = acc[i][j];
+      if (p.bias) {
 #pragma unroll
-      for (int g = 0; g < OP::QUADS; ++g) {
-        const int c = j * R + OP::channel(lane, g);
-        f32x4 f = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        if (p.bias) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) f[r] += load_any(p.bias, p.bias_type, min(c0 + c + r, p.n - 1));
-        }
-        if (p.out_type == MM_T_FP32)
-          *reinterpret_cast<f32x4*>(staged + lane_row * PITCH + c * 4) = f;
-        else
-          *reinterpret_cast<uint2*>(staged + lane_row * PITCH16 + c * 2) = pack4(f, p.out_type);
+        for (int r = 0; r < 4; ++r) f[r] += load_any(p.bias, p.bias_type, min(c0 + c + r, p.n - 1));
       }
+      if (p.out_type == MM_T_FP32)
+        *reinterpret_cast<f32x4*>(staged + lane_row * PITCH + c * 4) = f;
+      else
+        *reinterpret_cast<uint2*>(staged + lane_row * PITCH16 + c * 2) = pack4(f, p.out_type);
+    }
     if (p.out_type == MM_T_FP32)
       store_rows<R, COLS, PITCH, float>(p, staged, r0, c0);
     else
@@ -266,6 +256,30 @@ int launch_tiles(const Fp8Args& p, hipStream_t s) {
   return launch(fp8_tile_kernel<OP, BM, BN, WM, WN, KS, PRE, SHIFT>, tiles_of(p, BM, BN), WM * WN * KS * 64, p, s);
 }
 
+// Time of a product in us by its tiles: every 256 of them take `round` + `byte`
+// a byte of K, as measured on full rounds (and about 4 us in all).
+struct TileCost {
+  int bm, bn, step;  // step: K has to reach one whole stage
+  double round, byte;
+  int rounds = 1 << 30;  // for so many
+};
+constexpr TileCost kTileCosts[] = {
+    {256, 256, 128, 11.5, 13.3e-3}, {128, 128, 128, 3.3, 5.0e-3}, {128, 64, 256, 4.0, 2.9e-3, 1},
+    {64, 64, 128, 1.4, 1.75e-3},    {32, 64, 512, 1.8, 1.4e-3},   {32, 32, 1024, 1.8, 1.15e-3},
+};
+
+int best_tile(const Fp8Args& p) {
+  int best = 0;
+  double least = 1e300;
+  for (int i = 0; i < 6; ++i) {
+    const TileCost& c = kTileCosts[i];
+    const int64_t rounds = (tiles_of(p, c.bm, c.bn) + 255) / 256;
+    const double t = static_cast<double>(rounds) * (c.round + c.byte * p.k);
+    if (p.k >= c.step && rounds <= c.rounds && t < least) best = i, least = t;
+  }
+  return best;
+}
+
 int launch_best(const Fp8Args& p, hipStream_t s) {
   const bool shift = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.lda | p.ldb) & 3) != 0;
   if (p.out_type == MM_T_FP32) {
@@ -275,8 +289,20 @@ int launch_best(const Fp8Args& p, hipStream_t s) {
   }
   if (p.m <= 16) return launch_direct<Op16, 1, 1, 16, 4>(p, shift, s);
   if (p.k < BK) return launch_direct<Op16, 4, 4, 1, 1>(p, shift, s);  // not one whole stage
-  if (tiles_of(p, 256, 256) >= 256) return launch_tiles<Op32, 256, 256, 2, 2, 1, 1, false>(p, s);
-  return launch_tiles<Op32, 128, 128, 2, 2, 1, 2, false>(p, s);
+  switch (best_tile(p)) {
+    case 0: return launch_tiles<Op16, 256, 256, 4, 2, 1, 1, false>(p, s);
+    case 1: return launch_tiles<Op16, 128, 128, 2, 2, 1, 2, false>(p, s);
+    case 2:
+      return shift ? launch_tiles<Op16, 128, 64, 2, 2, 2, 2, true>(p, s) : launch_tiles<Op16, 128, 64, 2, 2, 2, 2, false>(p, s);
+    case 3:
+      if (p.k >= 2 * BK && tiles_of(p, 64, 64) <= 256)
+        return shift ? launch_tiles<Op16, 64, 64, 2, 2, 2, 2, true>(p, s) : launch_tiles<Op16, 64, 64, 2, 2, 2, 2, false>(p, s);
+      return shift ? launch_tiles<Op16, 64, 64, 2, 2, 1, 2, true>(p, s) : launch_tiles<Op16, 64, 64, 2, 2, 1, 2, false>(p, s);
+    case 4:
+      return shift ? launch_tiles<Op16, 32, 64, 1, 2, 4, 2, true>(p, s) : launch_tiles<Op16, 32, 64, 1, 2, 4, 2, false>(p, s);
+    default:
+      return shift ? launch_tiles<Op16, 32, 32, 1, 1, 8, 1, true>(p, s) : launch_tiles<Op16, 32, 32, 1, 1, 8, 1, false>(p, s);
+  }
 }
 
 bool is_float_type(int t) { return t == MM_T_BF16 || t == MM_T_FP16 || t == MM_T_FP32; }

@@ -147,68 +147,73 @@ __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(LayerArgs p) {
 // Rows of K bytes, K a multiple of 128: 16-byte vectors of a stage, NT threads.
 template <int ROWS, int NT>
 struct RowPanel {
-  static constexpr int PER = ROWS * 8 / NT;
+  // 32 rows of 8 waves: the upper half of the threads has a vector that the lower one has too
+  static constexpr int PER = (ROWS * 8 + NT - 1) / NT;
   static constexpr bool CUTS = false;
-  static_assert(PER * NT == ROWS * 8, "whole vectors");
   struct Stage {
     i32x4 d[PER];
   };
-  const uint8_t* base;
-  uint32_t off[PER];  // in 16 bytes, so that rows may lie 64 GB apart
+  const char* base;
+  uint32_t off[PER];
   // row(r): index of the panel's r-th row
   template <class F>
-  __device__ __forceinline__ RowPanel(const uint8_t* p, int K, const F& row) : base(p) {
+  __device__ __forceinline__ RowPanel(const uint8_t* p, int K, const F& row) : base(reinterpret_cast<const char*>(p)) {
 #pragma unroll
     for (int v = 0; v < PER; ++v) {
-      const int c = v * NT + threadIdx.x;
-      off[v] = static_cast<uint32_t>(row(c / 8)) * (static_cast<uint32_t>(K) / 16) + c % 8;
+      const int c = (v * NT + threadIdx.x) % (ROWS * 8);
+      off[v] = static_cast<uint32_t>(row(c / 8)) * static_cast<uint32_t>(K) + c % 8 * 16;
     }
+  }
+  __device__ __forceinline__ void load_one(Stage& r, int v, int k) const {
+    load_at(r.d[v], base + k, off[v]);
+  }
+  __device__ __forceinline__ void put_one(int8_t* lds, const Stage& r, int v) const {
+    const int c = (v * NT + threadIdx.x) % (ROWS * 8);
+    *reinterpret_cast<i32x4*>(lds + slot_of(c / 8, c % 8)) = r.d[v];
   }
   __device__ __forceinline__ void load(Stage& r, int k) const {
 #pragma unroll
-    for (int v = 0; v < PER; ++v) __builtin_memcpy(&r.d[v], base + k + (static_cast<uint64_t>(off[v]) << 4), 16);
+    for (int v = 0; v < PER; ++v) load_one(r, v, k);
   }
   __device__ __forceinline__ void put(int8_t* lds, const Stage& r) const {
 #pragma unroll
-    for (int v = 0; v < PER; ++v) {
-      const int c = v * NT + threadIdx.x;
-      *reinterpret_cast<i32x4*>(lds + slot_of(c / 8, c % 8)) = r.d[v];
-    }
+    for (int v = 0; v < PER; ++v) put_one(lds, r, v);
   }
   __device__ __forceinline__ void put_cut(int8_t*, int, int) const {}
 };
 
-// One tile of 32 MI WM rows of an expert by 256 channels: with FC1 128 columns
+// One tile of 16 MI WM rows of an expert by 256 channels: with FC1 128 columns
 // of the activation, a wave's channels gate and up of the same columns.
 template <bool FC1, int MI, int WM, int WN, int PRE>
-__device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const int4& t, int r0, int cb) {
-  constexpr int BM = 32 * MI * WM, BN = 256, NT = WM * WN * 64, COLS = BN / WN, NI = COLS / 32, Q = Op32::QUADS;
+__device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const int4& t, int cb) {
+  constexpr int ROWS = kTile * MI, BM = ROWS * WM, BN = 256, NT = WM * WN * 64, COLS = BN / WN, NI = COLS / kTile;
   constexpr int GATE = NI / 2;  // tiles of gate channels (FC1)
   auto& smem = *reinterpret_cast<int8_t(*)[2][(BM + BN) * BK]>(lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-  const int kb = p.k / kBlock;
+  const int kb = p.k / kBlock, r0 = t.y;
   const uint8_t* const ws = p.ws + static_cast<int64_t>(t.x) * (p.c / kBlock) * kb;
+  // rows of x lie anywhere, those of act from the tile's first one on
+  const int64_t base = FC1 ? 0 : r0;
   auto token = [&](int r) {
-    const int i = min(r0 + r, t.z - 1);
-    return p.rows ? p.rows[i] : i;
+    const int i = min(r, t.z - 1 - r0);
+    return FC1 ? p.rows[r0 + i] : i;
   };
   auto channel = [&](int r) {
     if (!FC1) return min(cb * BN + r, p.c - 1);
     const int w = r / COLS, c = r % COLS;
     return cb * kBlock + w * (COLS / 2) + c % (COLS / 2) + (c < COLS / 2 ? 0 : p.inter);
   };
-  // a tile's rows of x lie anywhere; those of act from its first one on
-  const RowPanel<BM, NT> pa(p.x, p.k, token);
+  const RowPanel<BM, NT> pa(p.x + base * p.k, p.k, token);
   const RowPanel<BN, NT> pb(p.w + static_cast<int64_t>(t.x) * p.c * p.k, p.k, channel);
   const uint8_t* xs[MI];
 #pragma unroll
-  for (int i = 0; i < MI; ++i) xs[i] = p.xs + static_cast<int64_t>(token(wm * 32 * MI + i * 32 + Op32::token(lane))) * kb;
+  for (int i = 0; i < MI; ++i) xs[i] = p.xs + (base + token(wm * ROWS + i * kTile + token_of(lane))) * kb;
   auto sa = [&](int i, int block) -> uint32_t { return xs[i][block]; };
-  constexpr int NB = FC1 ? 2 : 1;
-  const int sb0 = FC1 ? cb : min(cb * BN + wn * COLS, p.c - 1) / kBlock, sb1 = FC1 ? p.inter / kBlock + cb : 0;
-  auto sb = [&](int h, int block) -> uint32_t { return ws[static_cast<int64_t>(h ? sb1 : sb0) * kb + block]; };
-  f32x16 acc[MI][NI];
-  tile_sums<Op32, BM, BN, WM, WN, 1, PRE, NB>(smem, pa, pb, p.k, sa, sb, acc);
+  const uint8_t* const sb0 = ws + static_cast<int64_t>(FC1 ? cb : min(cb * BN + wn * COLS, p.c - 1) / kBlock) * kb;
+  const uint8_t* const sb1 = ws + static_cast<int64_t>(FC1 ? p.inter / kBlock + cb : 0) * kb;
+  auto sb = [&](int h, int block) -> uint32_t { return h ? sb1[block] : sb0[block]; };
+  f32x4 acc[MI][NI];
+  tile_sums<Op16, BM, BN, WM, WN, 1, PRE, FC1 ? 2 : 1>(smem, pa, pb, p.k, sa, sb, acc);
   __syncthreads();  // the stages are read
 
   if constexpr (FC1) {
@@ -218,36 +223,35 @@ __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const
     uint32_t* const tops = reinterpret_cast<uint32_t*>(lds + BM * PITCH);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const int r = wm * 32 * MI + i * 32 + Op32::token(lane);
+      const int r = wm * ROWS + i * kTile + token_of(lane);
       const float weight = p.weight[min(r0 + r, t.z - 1)];
       uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < GATE; ++j)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
+        for (int v = 0; v < 4; ++v) {
           const float a = gated_act(p.act_kind, acc[i][j][v], acc[i][j + GATE][v], p.beta, p.lbeta, p.limit) * weight;
           acc[i][j][v] = a;
           top = max(top, abs_bits(a));
         }
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
       top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-      if (lane < 32) tops[wn * BM + r] = top;
+      if (lane < 16) tops[wn * BM + r] = top;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const int r = wm * 32 * MI + i * 32 + Op32::token(lane);
+      const int r = wm * ROWS + i * kTile + token_of(lane);
       uint32_t top = 0;
 #pragma unroll
       for (int w = 0; w < WN; ++w) top = max(top, tops[w * BM + r]);
       const BlockScale s(top);
-      if (wn == 0 && lane < 32 && r0 + r < t.z)
+      if (wn == 0 && lane < 16 && r0 + r < t.z)
         p.out_scale[static_cast<int64_t>(r0 + r) * (p.inter / kBlock) + cb] = static_cast<uint8_t>(s.byte);
 #pragma unroll
       for (int j = 0; j < GATE; ++j)
-#pragma unroll
-        for (int g = 0; g < Q; ++g)
-          *reinterpret_cast<uint32_t*>(staged + r * PITCH + wn * (COLS / 2) + j * 32 + Op32::channel(lane, g)) =
-              s.pack4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+        *reinterpret_cast<uint32_t*>(staged + r * PITCH + wn * (COLS / 2) + j * kTile + channel_of(lane)) =
+            s.pack4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
     }
     __syncthreads();
     for (int v = threadIdx.x; v < BM * 8; v += NT) {
@@ -258,8 +262,8 @@ __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const
     }
   } else {
     constexpr int PITCH = COLS * 4 + 16;
-    static_assert(WM * WN * 32 * PITCH <= sizeof(smem), "epilogue staging");
-    int8_t* const staged = lds + wave * (32 * PITCH);
+    static_assert(WM * WN * kTile * PITCH <= sizeof(smem), "epilogue staging");
+    int8_t* const staged = lds + wave * (kTile * PITCH);
     struct {
       void* out;
       int64_t ldo;
@@ -269,11 +273,8 @@ __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const
     for (int i = 0; i < MI; ++i) {
 #pragma unroll
       for (int j = 0; j < NI; ++j)
-#pragma unroll
-        for (int g = 0; g < Q; ++g)
-          *reinterpret_cast<f32x4*>(staged + Op32::token(lane) * PITCH + (j * 32 + Op32::channel(lane, g)) * 4) =
-              f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-      store_rows<32, COLS, PITCH, float>(to, staged, r0 + wm * 32 * MI + i * 32, cb * BN + wn * COLS);
+        *reinterpret_cast<f32x4*>(staged + token_of(lane) * PITCH + (j * kTile + channel_of(lane)) * 4) = acc[i][j];
+      store_rows<kTile, COLS, PITCH, float>(to, staged, r0 + wm * ROWS + i * kTile, cb * BN + wn * COLS);
     }
   }
 }
@@ -283,7 +284,7 @@ __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const
 // come from one L2. The instructions fit the tile's rows: tiles of experts with
 // fewer do not multiply what is not there.
 template <bool FC1, int ROWS>
-__global__ __launch_bounds__(256) void fp8_rows_kernel(LayerArgs p) {
+__global__ __launch_bounds__(512) void fp8_rows_kernel(LayerArgs p) {
   __shared__ __attribute__((aligned(1024))) int8_t lds[2 * (ROWS + 256) * BK];
   const int cblocks = FC1 ? p.inter / kBlock : (p.c + 255) / 256;
   const int slot = blockIdx.x >> 3, tile = slot / cblocks * 8 + (blockIdx.x & 7), cb = slot % cblocks;
@@ -291,14 +292,14 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(LayerArgs p) {
   const int4 t = p.tl->tiles[tile];
   const int rows = t.z - t.y;
   if constexpr (ROWS == kStreamRows) {
-    if (rows <= 32) return rows_tile<FC1, 1, 1, 4, 1>(p, lds, t, t.y, cb);
-    if (rows <= 64) return rows_tile<FC1, 2, 1, 4, 1>(p, lds, t, t.y, cb);
-    if (rows <= 96) return rows_tile<FC1, 3, 1, 4, 1>(p, lds, t, t.y, cb);
-    if (rows <= 128) return rows_tile<FC1, 4, 1, 4, 1>(p, lds, t, t.y, cb);
-    rows_tile<FC1, 5, 1, 4, 1>(p, lds, t, t.y, cb);
+    if (rows <= 32) return rows_tile<FC1, 1, 2, 4, 1>(p, lds, t, cb);
+    if (rows <= 64) return rows_tile<FC1, 2, 2, 4, 1>(p, lds, t, cb);
+    if (rows <= 96) return rows_tile<FC1, 3, 2, 4, 1>(p, lds, t, cb);
+    if (rows <= 128) return rows_tile<FC1, 4, 2, 4, 1>(p, lds, t, cb);
+    rows_tile<FC1, 5, 2, 4, 1>(p, lds, t, cb);
   } else {
-    if (rows <= 128) return rows_tile<FC1, 2, 2, 2, 1>(p, lds, t, t.y, cb);
-    rows_tile<FC1, 4, 2, 2, 1>(p, lds, t, t.y, cb);
+    if (rows <= 128) return rows_tile<FC1, 2, 4, 2, 1>(p, lds, t, cb);
+    rows_tile<FC1, 4, 4, 2, 1>(p, lds, t, cb);
   }
 }
 
@@ -369,13 +370,13 @@ struct Scratch {
 
 constexpr int kMaxDim = 1 << 20;
 
-// Rows of x and act, and an expert's weights, in 32-bit offsets of 16 bytes.
+// The rows of x, and an expert's weights, have 32-bit offsets.
 bool layer_sizes_ok(int64_t tokens, int32_t top_k, int32_t E, int32_t hidden, int32_t inter) {
   constexpr int64_t most = int64_t(1) << 32;
   return tokens >= 0 && top_k > 0 && top_k <= 64 && E > 0 && E <= 32768 && hidden > 0 && inter > 0 &&
          hidden <= kMaxDim && inter <= kMaxDim && hidden % kBlock == 0 && inter % kBlock == 0 &&
-         tokens < (int64_t(1) << 31) / top_k && tokens * (hidden / 16) < most && tokens * top_k * (inter / 16) < most &&
-         static_cast<int64_t>(inter) * (hidden / 8) < most;
+         tokens < (int64_t(1) << 31) / top_k && tokens * hidden < most &&
+         int64_t(2) * inter * hidden < most;
 }
 
 int launch(void (*kernel)(LayerArgs), int64_t blocks, int threads, const LayerArgs& p, hipStream_t s) {
@@ -428,10 +429,10 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
     if (!rc) rc = launch(fp8_stream_kernel<false, 1, 4, 2>, tiles * (hidden / kBlock), 256, fc2, hs);
   } else {
     rc = launch(height == 256 ? fp8_rows_kernel<true, 256> : fp8_rows_kernel<true, kStreamRows>, tiles8 * (inter / kBlock),
-                256, fc1, hs);
+                512, fc1, hs);
     if (!rc)
       rc = launch(height == 256 ? fp8_rows_kernel<false, 256> : fp8_rows_kernel<false, kStreamRows>,
-                  tiles8 * ((hidden + 255) / 256), 256, fc2, hs);
+                  tiles8 * ((hidden + 255) / 256), 512, fc2, hs);
   }
   if (rc) return rc;
   const int64_t groups = (tokens * (hidden / 8) + 255) / 256;

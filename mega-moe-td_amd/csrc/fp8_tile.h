@@ -23,46 +23,28 @@ __device__ __forceinline__ i32x8 join32(const i32x4& lo, const i32x4& hi) {
   return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
-// R x R sums over 128 / SUB values with the scale byte of the lane's row (bits
-// 0-7 of sb, sa). A result's quad g of 4 channels begins at channel(g) of the
-// lane's token.
-struct Op32 {
-  static constexpr int R = 32, SUB = 2, QUADS = 4;
-  using Frag = i32x8;
-  using Acc = f32x16;
-  __device__ __forceinline__ static int token(int lane) { return lane & 31; }
-  __device__ __forceinline__ static int channel(int lane, int g) { return g * 8 + (lane >> 5) * 4; }
-  // the 16-byte slots of a row's 128 bytes that a lane holds
-  __device__ __forceinline__ static int slot(int lane, int kk, int h) { return kk * 4 + h * 2 + (lane >> 5); }
-  __device__ __forceinline__ static Frag frag(const i32x4& lo, const i32x4& hi) { return join32(lo, hi); }
-  __device__ __forceinline__ static Acc mac(const Frag& b, const Frag& a, const Acc& c, uint32_t sb, uint32_t sa) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b, a, c, 0, 0, 0, static_cast<int>(sb), 0, static_cast<int>(sa));
-  }
-};
+// 16 x 16 sums over a block of 128 values with the scale byte of the lane's row
+// (bits 0-7 of sb, sa): a result is 4 channels from channel(lane) on of the lane's
+// token. (32 x 32 x 64 instructions move half as many operand bytes and twice as
+// many sums; on registers alone, random values, they reach 3460 TFLOP/s and
+// these 3900: the chip is bound by power.)
+constexpr int kTile = 16;
+__device__ __forceinline__ int token_of(int lane) { return lane & 15; }
+__device__ __forceinline__ int channel_of(int lane) { return (lane >> 4) * 4; }
 
 struct Op16 {
-  static constexpr int R = 16, SUB = 1, QUADS = 1;
   using Frag = i32x8;
-  using Acc = f32x4;
-  __device__ __forceinline__ static int token(int lane) { return lane & 15; }
-  __device__ __forceinline__ static int channel(int lane, int) { return (lane >> 4) * 4; }
-  __device__ __forceinline__ static int slot(int lane, int, int h) { return h * 4 + (lane >> 4); }
   __device__ __forceinline__ static Frag frag(const i32x4& lo, const i32x4& hi) { return join32(lo, hi); }
-  __device__ __forceinline__ static Acc mac(const Frag& b, const Frag& a, const Acc& c, uint32_t sb, uint32_t sa) {
+  __device__ __forceinline__ static f32x4 mac(const Frag& b, const Frag& a, const f32x4& c, uint32_t sb, uint32_t sa) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, static_cast<int>(sb), 0, static_cast<int>(sa));
   }
 };
 
 // Op16 with sums in fp32: values in bf16, a block's sum times its power of two.
 struct Op16Wide {
-  static constexpr int R = 16, SUB = 1, QUADS = 1;
   struct Frag {
     bf16x8 v[4];
   };
-  using Acc = f32x4;
-  __device__ __forceinline__ static int token(int lane) { return lane & 15; }
-  __device__ __forceinline__ static int channel(int lane, int) { return (lane >> 4) * 4; }
-  __device__ __forceinline__ static int slot(int lane, int, int h) { return h * 4 + (lane >> 4); }
   __device__ __forceinline__ static bf16x8 wide(int w0, int w1) {
     uint32_t d[4];
 #pragma unroll
@@ -76,7 +58,7 @@ struct Op16Wide {
   __device__ __forceinline__ static Frag frag(const i32x4& lo, const i32x4& hi) {
     return Frag{{wide(lo[0], lo[1]), wide(lo[2], lo[3]), wide(hi[0], hi[1]), wide(hi[2], hi[3])}};
   }
-  __device__ __forceinline__ static Acc mac(const Frag& b, const Frag& a, Acc c, uint32_t sb, uint32_t sa) {
+  __device__ __forceinline__ static f32x4 mac(const Frag& b, const Frag& a, f32x4 c, uint32_t sb, uint32_t sa) {
     const float z = sb == kScaleNan || sa == kScaleNan ? __uint_as_float(0x7fc00000u) : 0.0f;
     f32x4 t = {z, z, z, z};
 #pragma unroll
@@ -97,15 +79,14 @@ struct Op16Wide {
 // Group ks has the sums of its blocks, ks, ks + KS, ...
 template <class OP, int BM, int BN, int WM, int WN, int KS, int PRE, int NB, class PA, class PB, class SA, class SB>
 __device__ __forceinline__ void tile_sums(int8_t (&smem)[2][(BM + BN) * KS * BK], const PA& pa, const PB& pb, int K,
-                                          const SA& sa, const SB& sb,
-                                          typename OP::Acc (&acc)[BM / WM / OP::R][BN / WN / OP::R]) {
-  constexpr int STEP = KS * BK, MI = BM / WM / OP::R, NI = BN / WN / OP::R, SUB = OP::SUB;
+                                          const SA& sa, const SB& sb, f32x4 (&acc)[BM / WM / kTile][BN / WN / kTile]) {
+  constexpr int STEP = KS * BK, MI = BM / WM / kTile, NI = BN / WN / kTile;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ks = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < NI; ++j) acc[i][j] = typename OP::Acc{};
+    for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{};
   const int cut = K % STEP, stages = (K + STEP - 1) / STEP, last_block = (K + BK - 1) / BK - 1;
   typename PA::Stage ra[PRE];
   typename PB::Stage rb[PRE];
@@ -138,74 +119,77 @@ __device__ __forceinline__ void tile_sums(int8_t (&smem)[2][(BM + BN) * KS * BK]
     pb.load(rb[u], at(u + 1));
   }
   __syncthreads();
-  auto frag = [&](const int8_t* panel, int row, int kk) __attribute__((always_inline)) {
-    return OP::frag(*reinterpret_cast<const i32x4*>(panel + slot_of(row, OP::slot(lane, kk, 0))),
-                    *reinterpret_cast<const i32x4*>(panel + slot_of(row, OP::slot(lane, kk, 1))));
+  // a lane's bytes of a row: 16 from 16 q on, and 64 behind them
+  auto frag = [&](const int8_t* panel, int row) __attribute__((always_inline)) {
+    return OP::frag(*reinterpret_cast<const i32x4*>(panel + slot_of(row, lane >> 4)),
+                    *reinterpret_cast<const i32x4*>(panel + slot_of(row, 4 + (lane >> 4))));
   };
-  auto frag_a = [&](const int8_t* buf, int i, int kk) __attribute__((always_inline)) {
-    return frag(buf + ks * BM * BK, wm * (BM / WM) + i * OP::R + OP::token(lane), kk);
+  auto frag_a = [&](const int8_t* buf, int i) __attribute__((always_inline)) {
+    return frag(buf + ks * BM * BK, wm * (BM / WM) + i * kTile + token_of(lane));
   };
-  auto frag_b = [&](const int8_t* buf, int j, int kk) __attribute__((always_inline)) {
-    return frag(buf + BM * STEP + ks * BN * BK, wn * (BN / WN) + j * OP::R + OP::token(lane), kk);
-  };
-  // LDS and memory instructions between the matrix instructions of a stage
-  auto schedule = [&](auto count) __attribute__((always_inline)) {
-    constexpr int MACS = decltype(count)::value;
-    if constexpr (SUB > 1 && MACS > 0) {
-      constexpr int READS = (2 * (SUB * NI + (SUB - 1) * MI) + MACS - 1) / MACS, MOVES = (PA::PER + PB::PER + MACS - 1) / MACS;
-#pragma unroll
-      for (int g = 0; g < MACS; ++g) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // MFMA
-        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);  // LDS read
-        __builtin_amdgcn_sched_group_barrier(0x200, MOVES, 0);  // LDS write
-        __builtin_amdgcn_sched_group_barrier(0x020, MOVES, 0);  // global load
-      }
-    }
+  auto frag_b = [&](const int8_t* buf, int j) __attribute__((always_inline)) {
+    return frag(buf + BM * STEP + ks * BN * BK, wn * (BN / WN) + j * kTile + token_of(lane));
   };
   typename OP::Frag fa[MI], fb;
 #pragma unroll
-  for (int i = 0; i < MI; ++i) fa[i] = frag_a(smem[0], i, 0);
-  fb = frag_b(smem[0], 0, 0);
-  // A sub-step takes one tile of channels after the other and reads the next
-  // one's fragment, and the next sub-step's of the tokens, meanwhile. Stage s + 1
-  // goes from its registers to LDS first, and its registers take stage s + 1 +
-  // PRE. The barrier stands behind the stage's last read and before the first of
-  // the next: from there on `nxt` is whole and `cur` free. Past the last stage
-  // the writes land where nobody reads any more.
+  for (int i = 0; i < MI; ++i) fa[i] = frag_a(smem[0], i);
+  fb = frag_b(smem[0], 0);
+  // A stage goes tile of channels by tile of channels. Meanwhile the next one's
+  // fragment is read, and stage s + 1 goes, a share at a time, from its registers
+  // to LDS, where it is followed by stage s + 1 + PRE. (Reads stand before
+  // writes: the compiler keeps their order.) The barrier stands behind the
+  // stage's last read and before the first of the next: from there on `nxt` is
+  // whole and `cur` free, and the last tile of channels hands its token fragments
+  // over one by one. Past the last stage the writes land where nobody reads any
+  // more.
   auto stage = [&](int s, auto reg) __attribute__((always_inline)) {
-    constexpr int R = decltype(reg)::value;
+    constexpr int R = decltype(reg)::value, MOVES = PA::PER + PB::PER;
+    constexpr int SHARE = NI > 1 ? (MOVES + NI - 2) / (NI - 1) : MOVES;  // moves a step
     const int8_t* cur = smem[s & 1];
     int8_t* nxt = smem[(s + 1) & 1];
+    const int ahead = at(s + 1 + PRE);
     uint32_t as_next[MI], bs_next[NB];
-    scales(s + 1, as_next, bs_next);
-    pa.put(nxt, ra[R]);
-    pa.load(ra[R], at(s + 1 + PRE));
-    pb.put(nxt + BM * STEP, rb[R]);
-    pb.load(rb[R], at(s + 1 + PRE));
+    auto moves = [&](int first) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kk = 0; kk < SUB; ++kk) {
-      typename OP::Frag fa_next[MI];
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const bool last = kk == SUB - 1, tail = last && j == NI - 1;
-        if (tail) {
-          schedule(std::integral_constant<int, (SUB * NI - 1) * MI>{});
-          __syncthreads();
+      for (int v = first; v < first + SHARE; ++v) {
+        if (v < PA::PER) {
+          pa.put_one(nxt, ra[R], v);
+          pa.load_one(ra[R], v, ahead);
+        } else if (v < MOVES) {
+          pb.put_one(nxt + BM * STEP, rb[R], v - PA::PER);
+          pb.load_one(rb[R], v - PA::PER, ahead);
         }
-        const typename OP::Frag fb_next = tail         ? frag_b(nxt, 0, 0)
-                                          : j < NI - 1 ? frag_b(cur, j + 1, kk)
-                                                       : frag_b(cur, 0, kk + 1);
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          if (tail) fa_next[i] = frag_a(nxt, i, 0);
-          if (!last && i * NI / MI == j) fa_next[i] = frag_a(cur, i, kk + 1);
-        }
-#pragma unroll
-        for (int i = 0; i < MI; ++i) acc[i][j] = OP::mac(fb, fa[i], acc[i][j], bs[j * NB / NI], as[i]);
-        fb = fb_next;
       }
+    };
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fa[i] = fa_next[i];
+    for (int j = 0; j < NI; ++j) {
+      const bool tail = j == NI - 1;
+      if (tail) {
+        if (NI == 1) moves(0);
+        __syncthreads();
+      }
+      const typename OP::Frag fb_next = tail ? frag_b(nxt, 0) : frag_b(cur, j + 1);
+      if (j == 0) scales(s + 1, as_next, bs_next);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        acc[i][j] = OP::mac(fb, fa[i], acc[i][j], bs[j * NB / NI], as[i]);
+        if (tail) fa[i] = frag_a(nxt, i);
+      }
+      if (!tail) moves(j * SHARE);
+      // reads first, the rest between the matrix instructions, and no step's into another's
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS read
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+        if (tail) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        } else if (i % (MI / (SHARE < MI ? SHARE : MI)) == 0) {
+          __builtin_amdgcn_sched_group_barrier(0x200, (SHARE + MI - 1) / MI, 0);  // LDS write
+          __builtin_amdgcn_sched_group_barrier(0x020, (SHARE + MI - 1) / MI, 0);  // global load
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      fb = fb_next;
     }
 #pragma unroll
     for (int i = 0; i < MI; ++i) as[i] = as_next[i];

@@ -84,11 +84,21 @@ __device__ __forceinline__ i32x4 load16_cut(const char* base, uint32_t off, int 
   return v;
 }
 
-// Address of a row as an aligned base and what is left of it.
+// Address of a row as an aligned base and what is left of it. The base is the
+// pointer less the rest, not a number made a pointer again, whose loads the
+// compiler cannot tell from LDS (it then waits for both kinds at once).
 __device__ __forceinline__ const char* aligned_base(const void* p, uint32_t& rest) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-  rest = a & 3;
-  return reinterpret_cast<const char*>(a - rest);
+  rest = reinterpret_cast<uintptr_t>(p) & 3;
+  return static_cast<const char*>(p) - rest;
+}
+
+// Sixteen bytes at a base that is the same for the wave plus a lane's offset. The
+// empty instruction keeps the offset's extension to 64 bits in place: in front
+// of a loop it is kept there in two registers and the sum is made of vector adds.
+template <class T>
+__device__ __forceinline__ void load_at(T& to, const char* base, uint32_t off) {
+  asm volatile("" : "+v"(off));
+  __builtin_memcpy(&to, base + off, 16);
 }
 
 // ------------------------------------------------------------------ stages in LDS
@@ -102,7 +112,8 @@ __device__ __forceinline__ int slot_of(int r, int s) { return r * BK + ((s ^ ((r
 // SHIFT a vector's fifth word is the first of the next lane's vector; only the
 // last lane of a run loads it, and words are joined on their way to LDS (128 x
 // 7169 x 4096 in 32 x 64 tiles: 21 us, 23 with five words loaded by every lane).
-template <int ROWS, int NT, int KS, bool SHIFT>
+// PIN: load_at's loads.
+template <int ROWS, int NT, int KS, bool SHIFT, bool PIN = false>
 struct Panel {
   static constexpr int VPR = 8 * KS, PER = ROWS * VPR / NT;  // 16-byte vectors a row, a thread
   static_assert(PER * NT == ROWS * VPR && NT % VPR == 0, "whole vectors");
@@ -127,32 +138,37 @@ struct Panel {
   __device__ __forceinline__ static bool last_of_run() { return (threadIdx.x & LAST) == LAST; }
   __device__ __forceinline__ void load(Stage& r, int k) const {
 #pragma unroll
-    for (int v = 0; v < PER; ++v) {
-      if constexpr (SHIFT) {
-        const uint32_t sh = off[v] & 3;
-        const char* p = base + k + (off[v] - sh);
-        __builtin_memcpy(r.d[v], __builtin_assume_aligned(p, 4), 16);
-        if (last_of_run()) __builtin_memcpy(r.d[v] + 4, __builtin_assume_aligned(p + (sh ? 16 : 12), 4), 4);
-      } else {
+    for (int v = 0; v < PER; ++v) load_one(r, v, k);
+  }
+  __device__ __forceinline__ void load_one(Stage& r, int v, int k) const {
+    if constexpr (SHIFT) {
+      const uint32_t sh = off[v] & 3;
+      const char* p = base + k + (off[v] - sh);
+      __builtin_memcpy(r.d[v], __builtin_assume_aligned(p, 4), 16);
+      if (last_of_run()) __builtin_memcpy(r.d[v] + 4, __builtin_assume_aligned(p + (sh ? 16 : 12), 4), 4);
+    } else {
+      if constexpr (PIN)
+        load_at(r.d[v], base + k, off[v]);
+      else
         __builtin_memcpy(r.d[v], base + k + off[v], 16);
-      }
     }
   }
   __device__ __forceinline__ void put(int8_t* lds, const Stage& r) const {
 #pragma unroll
-    for (int v = 0; v < PER; ++v) {
-      if constexpr (SHIFT) {
-        uint32_t d[5];
+    for (int v = 0; v < PER; ++v) put_one(lds, r, v);
+  }
+  __device__ __forceinline__ void put_one(int8_t* lds, const Stage& r, int v) const {
+    if constexpr (SHIFT) {
+      uint32_t d[5];
 #pragma unroll
-        for (int i = 0; i < 5; ++i) d[i] = r.d[v][i];
-        const uint32_t next = __builtin_amdgcn_update_dpp(d[4], d[0], 0x101, 0xf, 0xf, false);  // of lane + 1
-        if (!last_of_run()) d[4] = next;
-        put(lds, v, join16(d, off[v] & 3));
-      } else {
-        i32x4 x;
-        __builtin_memcpy(&x, r.d[v], 16);
-        put(lds, v, x);
-      }
+      for (int i = 0; i < 5; ++i) d[i] = r.d[v][i];
+      const uint32_t next = __builtin_amdgcn_update_dpp(d[4], d[0], 0x101, 0xf, 0xf, false);  // of lane + 1
+      if (!last_of_run()) d[4] = next;
+      put(lds, v, join16(d, off[v] & 3));
+    } else {
+      i32x4 x;
+      __builtin_memcpy(&x, r.d[v], 16);
+      put(lds, v, x);
     }
   }
   // The stage that K cuts, from memory to LDS.
