@@ -6,6 +6,8 @@
 // instruction's own operands, so sums over the whole of K stay in its fp32
 // accumulators and are rounded once, behind the bias. (Results in 32 bits: see
 // Op16Wide.)
+#include <algorithm>
+
 #include "fp8_tile.h"
 
 namespace {
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(W * 64) void fp8_direct_kernel(Fp8Args p) {
       for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-          acc[g][n] = OP::mac(OP::frag(bv[u][g][0], bv[u][g][1]), OP::frag(av[u][n][0], av[u][n][1]), acc[g][n], bs[u][g],
+          acc[g][n] = OP::mac(OP::frag(join32(bv[u][g][0], bv[u][g][1])), OP::frag(join32(av[u][n][0], av[u][n][1])), acc[g][n], bs[u][g],
                               as[u][n]);
   };
   int s = wave;
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(W * 64) void fp8_direct_kernel(Fp8Args p) {
     for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
-        acc[g][n] = OP::mac(OP::frag(bv[g][0], bv[g][1]), OP::frag(av[n][0], av[n][1]), acc[g][n], sb[g][full], sa[n][full]);
+        acc[g][n] = OP::mac(OP::frag(join32(bv[g][0], bv[g][1])), OP::frag(join32(av[n][0], av[n][1])), acc[g][n], sb[g][full], sa[n][full]);
   }
 #pragma unroll
   for (int g = 0; g < G; ++g)
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(W * 64) void fp8_direct_kernel(Fp8Args p) {
 // of a wave at a time go through its own LDS, padded to spread a pass
 // over the banks, so that neighbouring lanes store neighbouring 16 bytes.
 template <class OP, int BM, int BN, int WM, int WN, int KS, int PRE, bool SHIFT>
-__global__ __launch_bounds__(WM * WN * KS * 64) void fp8_tile_kernel(Fp8Args p) {
+__global__ __launch_bounds__(WM * WN * KS * 64, OP::WAVES) void fp8_tile_kernel(Fp8Args p) {
   constexpr int NT = WM * WN * KS * 64, STEP = KS * BK, R = kTile, MI = BM / WM / R, NI = BN / WN / R;
   __shared__ __attribute__((aligned(1024))) int8_t smem[2][(BM + BN) * STEP];
   const int num_m = (p.m + BM - 1) / BM, num_n = (p.n + BN - 1) / BN;
@@ -256,26 +258,31 @@ int launch_tiles(const Fp8Args& p, hipStream_t s) {
   return launch(fp8_tile_kernel<OP, BM, BN, WM, WN, KS, PRE, SHIFT>, tiles_of(p, BM, BN), WM * WN * KS * 64, p, s);
 }
 
-// Time of a product in us by its tiles: every 256 of them take `round` + `byte`
-// a byte of K, as measured on full rounds (and about 4 us in all).
+// Time of a product in us by its tiles, about 4 us in all and `tile` and `byte` a
+// byte of K for every 256 of them, as measured on full rounds (2048 x 2048 x 1024
+// and 8192 in 128 x 128 tiles, 256 of them: 11.5 and 55 us). Where a CU holds
+// several tiles a part of a round costs what its share is, or 0.42 of a round
+// (968 x 4992 x 6016, 312 such tiles: 58 us, 42 for up to 256).
 struct TileCost {
   int bm, bn, step;  // step: K has to reach one whole stage
-  double round, byte;
-  int rounds = 1 << 30;  // for so many
+  double tile, byte;
+  bool several;
 };
 constexpr TileCost kTileCosts[] = {
-    {256, 256, 128, 11.5, 13.3e-3}, {128, 128, 128, 3.3, 5.0e-3}, {128, 64, 256, 4.0, 2.9e-3, 1},
-    {64, 64, 128, 1.4, 1.75e-3},    {32, 64, 512, 1.8, 1.4e-3},   {32, 32, 1024, 1.8, 1.15e-3},
+    {256, 256, 128, 6.0, 13.2e-3, false}, {128, 128, 128, 1.3, 6.1e-3, true}, {64, 64, 128, 0.2, 2.85e-3, true},
+    {32, 64, 512, 1.0, 1.67e-3, false},   {32, 32, 1024, 1.4, 1.0e-3, false},
 };
 
 int best_tile(const Fp8Args& p) {
   int best = 0;
   double least = 1e300;
-  for (int i = 0; i < 6; ++i) {
+  for (int i = 0; i < 5; ++i) {
     const TileCost& c = kTileCosts[i];
-    const int64_t rounds = (tiles_of(p, c.bm, c.bn) + 255) / 256;
-    const double t = static_cast<double>(rounds) * (c.round + c.byte * p.k);
-    if (p.k >= c.step && rounds <= c.rounds && t < least) best = i, least = t;
+    const int64_t tiles = tiles_of(p, c.bm, c.bn), full = (tiles + 255) / 256;
+    double rounds = static_cast<double>(full);
+    if (c.several && full > 1) rounds = std::max(rounds - 0.58, static_cast<double>(tiles) / 256);
+    const double t = rounds * (c.tile + c.byte * p.k);
+    if (p.k >= c.step && t < least) best = i, least = t;
   }
   return best;
 }
@@ -293,12 +300,10 @@ int launch_best(const Fp8Args& p, hipStream_t s) {
     case 0: return launch_tiles<Op16, 256, 256, 4, 2, 1, 1, false>(p, s);
     case 1: return launch_tiles<Op16, 128, 128, 2, 2, 1, 2, false>(p, s);
     case 2:
-      return shift ? launch_tiles<Op16, 128, 64, 2, 2, 2, 2, true>(p, s) : launch_tiles<Op16, 128, 64, 2, 2, 2, 2, false>(p, s);
-    case 3:
       if (p.k >= 2 * BK && tiles_of(p, 64, 64) <= 256)
         return shift ? launch_tiles<Op16, 64, 64, 2, 2, 2, 2, true>(p, s) : launch_tiles<Op16, 64, 64, 2, 2, 2, 2, false>(p, s);
       return shift ? launch_tiles<Op16, 64, 64, 2, 2, 1, 2, true>(p, s) : launch_tiles<Op16, 64, 64, 2, 2, 1, 2, false>(p, s);
-    case 4:
+    case 3:
       return shift ? launch_tiles<Op16, 32, 64, 1, 2, 4, 2, true>(p, s) : launch_tiles<Op16, 32, 64, 1, 2, 4, 2, false>(p, s);
     default:
       return shift ? launch_tiles<Op16, 32, 32, 1, 1, 8, 1, true>(p, s) : launch_tiles<Op16, 32, 32, 1, 1, 8, 1, false>(p, s);

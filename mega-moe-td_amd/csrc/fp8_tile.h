@@ -33,8 +33,9 @@ __device__ __forceinline__ int token_of(int lane) { return lane & 15; }
 __device__ __forceinline__ int channel_of(int lane) { return (lane >> 4) * 4; }
 
 struct Op16 {
+  static constexpr int WAVES = 1;  // of a SIMD, at least
   using Frag = i32x8;
-  __device__ __forceinline__ static Frag frag(const i32x4& lo, const i32x4& hi) { return join32(lo, hi); }
+  __device__ __forceinline__ static Frag frag(const i32x8& bytes) { return bytes; }
   __device__ __forceinline__ static f32x4 mac(const Frag& b, const Frag& a, const f32x4& c, uint32_t sb, uint32_t sa) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, static_cast<int>(sb), 0, static_cast<int>(sa));
   }
@@ -42,21 +43,21 @@ struct Op16 {
 
 // Op16 with sums in fp32: values in bf16, a block's sum times its power of two.
 struct Op16Wide {
+  static constexpr int WAVES = 2;  // one converts while the other multiplies
   struct Frag {
     bf16x8 v[4];
   };
   __device__ __forceinline__ static bf16x8 wide(int w0, int w1) {
-    uint32_t d[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int w = i < 2 ? w0 : w1;
-      const auto f = i & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8(w, true) : __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
-      d[i] = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u);  // the low halves are 0
-    }
-    return __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3]));
+    const bf16x2_t d[4] = {
+        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<uint32_t>(w0), 1.0f, false),
+        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<uint32_t>(w0), 1.0f, true),
+        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<uint32_t>(w1), 1.0f, false),
+        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<uint32_t>(w1), 1.0f, true),
+    };
+    return __builtin_bit_cast(bf16x8, d);
   }
-  __device__ __forceinline__ static Frag frag(const i32x4& lo, const i32x4& hi) {
-    return Frag{{wide(lo[0], lo[1]), wide(lo[2], lo[3]), wide(hi[0], hi[1]), wide(hi[2], hi[3])}};
+  __device__ __forceinline__ static Frag frag(const i32x8& b) {
+    return Frag{{wide(b[0], b[1]), wide(b[2], b[3]), wide(b[4], b[5]), wide(b[6], b[7])}};
   }
   __device__ __forceinline__ static f32x4 mac(const Frag& b, const Frag& a, f32x4 c, uint32_t sb, uint32_t sa) {
     const float z = sb == kScaleNan || sa == kScaleNan ? __uint_as_float(0x7fc00000u) : 0.0f;
@@ -80,7 +81,7 @@ struct Op16Wide {
 template <class OP, int BM, int BN, int WM, int WN, int KS, int PRE, int NB, class PA, class PB, class SA, class SB>
 __device__ __forceinline__ void tile_sums(int8_t (&smem)[2][(BM + BN) * KS * BK], const PA& pa, const PB& pb, int K,
                                           const SA& sa, const SB& sb, f32x4 (&acc)[BM / WM / kTile][BN / WN / kTile]) {
-  constexpr int STEP = KS * BK, MI = BM / WM / kTile, NI = BN / WN / kTile;
+  constexpr int STEP = KS * BK, MI = BM / WM / kTile, NI = BN / WN / kTile, MOVES = PA::PER + PB::PER;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ks = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
 #pragma unroll
@@ -104,7 +105,6 @@ __device__ __forceinline__ void tile_sums(int8_t (&smem)[2][(BM + BN) * KS * BK]
     pa.put(smem[0], ra[0]);
     pb.put(smem[0] + BM * STEP, rb[0]);
   }
-  uint32_t as[MI], bs[NB];
   auto scales = [&](int s, uint32_t (&a)[MI], uint32_t (&b)[NB]) __attribute__((always_inline)) {
     const int at_block = block(s);
 #pragma unroll
@@ -112,70 +112,72 @@ __device__ __forceinline__ void tile_sums(int8_t (&smem)[2][(BM + BN) * KS * BK]
 #pragma unroll
     for (int h = 0; h < NB; ++h) b[h] = sb(h, at_block);
   };
-  scales(0, as, bs);
+  // before the loads of stages: a loop's first wait counts what is outstanding in
+  // front of it too, and scales behind them would wait for all of those
+  uint32_t as[2][MI], bs[2][NB];
+  scales(0, as[0], bs[0]);
 #pragma unroll
   for (int u = 0; u < PRE; ++u) {
     pa.load(ra[u], at(u + 1));
     pb.load(rb[u], at(u + 1));
   }
-  __syncthreads();
-  // a lane's bytes of a row: 16 from 16 q on, and 64 behind them
-  auto frag = [&](const int8_t* panel, int row) __attribute__((always_inline)) {
-    return OP::frag(*reinterpret_cast<const i32x4*>(panel + slot_of(row, lane >> 4)),
-                    *reinterpret_cast<const i32x4*>(panel + slot_of(row, 4 + (lane >> 4))));
-  };
-  auto frag_a = [&](const int8_t* buf, int i) __attribute__((always_inline)) {
-    return frag(buf + ks * BM * BK, wm * (BM / WM) + i * kTile + token_of(lane));
-  };
-  auto frag_b = [&](const int8_t* buf, int j) __attribute__((always_inline)) {
-    return frag(buf + BM * STEP + ks * BN * BK, wn * (BN / WN) + j * kTile + token_of(lane));
-  };
-  typename OP::Frag fa[MI], fb;
+  // vectors first .. first + count - 1 of the stage in registers R to `buf`, and
+  // the stage at byte `ahead` into the registers
+  auto moves = [&](auto reg, int8_t* buf, int ahead, int first, int count) __attribute__((always_inline)) {
+    constexpr int R = decltype(reg)::value;
 #pragma unroll
-  for (int i = 0; i < MI; ++i) fa[i] = frag_a(smem[0], i);
-  fb = frag_b(smem[0], 0);
+    for (int v = first; v < first + count; ++v) {
+      if (v < PA::PER) {
+        pa.put_one(buf, ra[R], v);
+        pa.load_one(ra[R], v, ahead);
+      } else if (v < MOVES) {
+        pb.put_one(buf + BM * STEP, rb[R], v - PA::PER);
+        pb.load_one(rb[R], v - PA::PER, ahead);
+      }
+    }
+  };
+  // a lane's bytes of a row: 16 from 16 q on, and 64 behind them
+  auto bytes = [&](const int8_t* panel, int row) __attribute__((always_inline)) {
+    return join32(*reinterpret_cast<const i32x4*>(panel + slot_of(row, lane >> 4)),
+                  *reinterpret_cast<const i32x4*>(panel + slot_of(row, 4 + (lane >> 4))));
+  };
+  auto bytes_a = [&](const int8_t* buf, int i) __attribute__((always_inline)) {
+    return bytes(buf + ks * BM * BK, wm * (BM / WM) + i * kTile + token_of(lane));
+  };
+  auto bytes_b = [&](const int8_t* buf, int j) __attribute__((always_inline)) {
+    return bytes(buf + BM * STEP + ks * BN * BK, wn * (BN / WN) + j * kTile + token_of(lane));
+  };
   // A stage goes tile of channels by tile of channels. Meanwhile the next one's
   // fragment is read, and stage s + 1 goes, a share at a time, from its registers
   // to LDS, where it is followed by stage s + 1 + PRE. (Reads stand before
   // writes: the compiler keeps their order.) The barrier stands behind the
   // stage's last read and before the first of the next: from there on `nxt` is
   // whole and `cur` free, and the last tile of channels hands its token fragments
-  // over one by one. Past the last stage the writes land where nobody reads any
-  // more.
+  // over one by one. (All fragments of a stage read ahead in one go take the
+  // registers of a second workgroup: 128 x 128 tiles, 4096^3, 113 us so, 136.)
+  static_assert(NI > 1, "moves stand between tiles of channels");
+  constexpr int SHARE = (MOVES + NI - 2) / (NI - 1);  // moves a step
+  typename OP::Frag fa[MI], fb;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MI; ++i) fa[i] = OP::frag(bytes_a(smem[0], i));
+  fb = OP::frag(bytes_b(smem[0], 0));
   auto stage = [&](int s, auto reg) __attribute__((always_inline)) {
-    constexpr int R = decltype(reg)::value, MOVES = PA::PER + PB::PER;
-    constexpr int SHARE = NI > 1 ? (MOVES + NI - 2) / (NI - 1) : MOVES;  // moves a step
     const int8_t* cur = smem[s & 1];
     int8_t* nxt = smem[(s + 1) & 1];
     const int ahead = at(s + 1 + PRE);
-    uint32_t as_next[MI], bs_next[NB];
-    auto moves = [&](int first) __attribute__((always_inline)) {
-#pragma unroll
-      for (int v = first; v < first + SHARE; ++v) {
-        if (v < PA::PER) {
-          pa.put_one(nxt, ra[R], v);
-          pa.load_one(ra[R], v, ahead);
-        } else if (v < MOVES) {
-          pb.put_one(nxt + BM * STEP, rb[R], v - PA::PER);
-          pb.load_one(rb[R], v - PA::PER, ahead);
-        }
-      }
-    };
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const bool tail = j == NI - 1;
-      if (tail) {
-        if (NI == 1) moves(0);
-        __syncthreads();
-      }
-      const typename OP::Frag fb_next = tail ? frag_b(nxt, 0) : frag_b(cur, j + 1);
-      if (j == 0) scales(s + 1, as_next, bs_next);
+      if (tail) __syncthreads();
+      const i32x8 next = tail ? bytes_b(nxt, 0) : bytes_b(cur, j + 1);
+      if (j == 0) scales(s + 1, as[1], bs[1]);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
-        acc[i][j] = OP::mac(fb, fa[i], acc[i][j], bs[j * NB / NI], as[i]);
-        if (tail) fa[i] = frag_a(nxt, i);
+        acc[i][j] = OP::mac(fb, fa[i], acc[i][j], bs[0][j * NB / NI], as[0][i]);
+        if (tail) fa[i] = OP::frag(bytes_a(nxt, i));
       }
-      if (!tail) moves(j * SHARE);
+      if (!tail) moves(reg, nxt, ahead, j * SHARE, SHARE);
       // reads first, the rest between the matrix instructions, and no step's into another's
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS read
 #pragma unroll
@@ -189,12 +191,12 @@ __device__ __forceinline__ void tile_sums(int8_t (&smem)[2][(BM + BN) * KS * BK]
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      fb = fb_next;
+      fb = OP::frag(next);
     }
 #pragma unroll
-    for (int i = 0; i < MI; ++i) as[i] = as_next[i];
+    for (int i = 0; i < MI; ++i) as[0][i] = as[1][i];
 #pragma unroll
-    for (int h = 0; h < NB; ++h) bs[h] = bs_next[h];
+    for (int h = 0; h < NB; ++h) bs[0][h] = bs[1][h];
   };
   for (int s = 0; s < stages; s += PRE) {
     stage(s, std::integral_constant<int, 0>{});
