@@ -272,12 +272,17 @@ constexpr TileCost kTileCosts[] = {
     {256, 256, 128, 6.0, 13.2e-3, false}, {128, 128, 128, 1.3, 6.1e-3, true}, {64, 64, 128, 0.2, 2.85e-3, true},
     {32, 64, 512, 1.0, 1.67e-3, false},   {32, 32, 1024, 1.4, 1.0e-3, false},
 };
+// Results in 32 bits (2048 x 2048 x 4096 in 128 x 128 tiles: 62 us; 1024 x 1024 x
+// 4096 in 64 x 64: 24; 64 x 4096 x 7168 in 32 x 64: 22).
+constexpr TileCost kWideCosts[] = {
+    {128, 128, 128, 0.5, 14.1e-3, true}, {64, 64, 128, 0.2, 4.8e-3, true}, {32, 64, 512, 0.5, 2.6e-3, false}};
 
-int best_tile(const Fp8Args& p) {
+template <int N>
+int best_tile(const TileCost (&costs)[N], const Fp8Args& p) {
   int best = 0;
   double least = 1e300;
-  for (int i = 0; i < 5; ++i) {
-    const TileCost& c = kTileCosts[i];
+  for (int i = 0; i < N; ++i) {
+    const TileCost& c = costs[i];
     const int64_t tiles = tiles_of(p, c.bm, c.bn), full = (tiles + 255) / 256;
     double rounds = static_cast<double>(full);
     if (c.several && full > 1) rounds = std::max(rounds - 0.58, static_cast<double>(tiles) / 256);
@@ -287,26 +292,37 @@ int best_tile(const Fp8Args& p) {
   return best;
 }
 
+// Tiles whose rows may begin anywhere: shifted into place on their way to LDS
+// where they do not on 4-byte borders.
+template <class OP, int BM, int BN, int WM, int WN, int KS, int PRE>
+int launch_any(const Fp8Args& p, bool shift, hipStream_t s) {
+  return shift ? launch_tiles<OP, BM, BN, WM, WN, KS, PRE, true>(p, s) : launch_tiles<OP, BM, BN, WM, WN, KS, PRE, false>(p, s);
+}
+
 int launch_best(const Fp8Args& p, hipStream_t s) {
+  // the two largest tiles leave odd addresses to the memory pipe
   const bool shift = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.lda | p.ldb) & 3) != 0;
-  if (p.out_type == MM_T_FP32) {
-    if (p.m <= 16) return launch_direct<Op16Wide, 1, 1, 16, 2>(p, shift, s);
-    if (p.k < BK) return launch_direct<Op16Wide, 2, 2, 1, 1>(p, shift, s);
-    return launch_tiles<Op16Wide, 128, 128, 2, 2, 1, 1, false>(p, s);
+  const bool wide = p.out_type == MM_T_FP32;
+  // 16 rows at most: a run of channels for each workgroup, its waves sharing K
+  if (p.m <= 16) return wide ? launch_direct<Op16Wide, 1, 1, 16, 2>(p, shift, s) : launch_direct<Op16, 1, 1, 16, 4>(p, shift, s);
+  // not one whole stage
+  if (p.k < BK) return wide ? launch_direct<Op16Wide, 2, 2, 1, 1>(p, shift, s) : launch_direct<Op16, 4, 4, 1, 1>(p, shift, s);
+  // 64 x 64: the sum shared by two groups of waves until the chip is full
+  const bool shared = p.k >= 2 * BK && tiles_of(p, 64, 64) <= 256;
+  if (wide) {
+    switch (best_tile(kWideCosts, p)) {
+      case 0: return launch_tiles<Op16Wide, 128, 128, 2, 2, 1, 1, false>(p, s);
+      case 1:
+        return shared ? launch_any<Op16Wide, 64, 64, 2, 2, 2, 1>(p, shift, s) : launch_any<Op16Wide, 64, 64, 2, 2, 1, 1>(p, shift, s);
+      default: return launch_any<Op16Wide, 32, 64, 1, 2, 4, 1>(p, shift, s);
+    }
   }
-  if (p.m <= 16) return launch_direct<Op16, 1, 1, 16, 4>(p, shift, s);
-  if (p.k < BK) return launch_direct<Op16, 4, 4, 1, 1>(p, shift, s);  // not one whole stage
-  switch (best_tile(p)) {
+  switch (best_tile(kTileCosts, p)) {
     case 0: return launch_tiles<Op16, 256, 256, 4, 2, 1, 1, false>(p, s);
     case 1: return launch_tiles<Op16, 128, 128, 2, 2, 1, 2, false>(p, s);
-    case 2:
-      if (p.k >= 2 * BK && tiles_of(p, 64, 64) <= 256)
-        return shift ? launch_tiles<Op16, 64, 64, 2, 2, 2, 2, true>(p, s) : launch_tiles<Op16, 64, 64, 2, 2, 2, 2, false>(p, s);
-      return shift ? launch_tiles<Op16, 64, 64, 2, 2, 1, 2, true>(p, s) : launch_tiles<Op16, 64, 64, 2, 2, 1, 2, false>(p, s);
-    case 3:
-      return shift ? launch_tiles<Op16, 32, 64, 1, 2, 4, 2, true>(p, s) : launch_tiles<Op16, 32, 64, 1, 2, 4, 2, false>(p, s);
-    default:
-      return shift ? launch_tiles<Op16, 32, 32, 1, 1, 8, 1, true>(p, s) : launch_tiles<Op16, 32, 32, 1, 1, 8, 1, false>(p, s);
+    case 2: return shared ? launch_any<Op16, 64, 64, 2, 2, 2, 2>(p, shift, s) : launch_any<Op16, 64, 64, 2, 2, 1, 2>(p, shift, s);
+    case 3: return launch_any<Op16, 32, 64, 1, 2, 4, 2>(p, shift, s);
+    default: return launch_any<Op16, 32, 32, 1, 1, 8, 1>(p, shift, s);
   }
 }
 
