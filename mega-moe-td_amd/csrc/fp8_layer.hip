@@ -9,6 +9,8 @@
 // Routing tables and tile lists are those of the bf16 layer. The experts' outputs
 // stay in fp32 until the slots are summed: in bf16 each would be off by as much
 // as the result is by its own rounding.
+#include <algorithm>
+
 #include "fp8_tile.h"
 
 namespace {
@@ -26,122 +28,6 @@ struct LayerArgs {
   int32_t k, c, inter, act_kind;
   float beta, lbeta, limit;
 };
-
-// 32 bytes of a row's block, at any alignment: 16 and the 16 that lie 64 behind.
-__device__ __forceinline__ i32x8 load32(const uint8_t* p) {
-  i32x4 lo, hi;
-  __builtin_memcpy(&lo, p, 16);
-  __builtin_memcpy(&hi, p + 64, 16);
-  return join32(lo, hi);
-}
-
-// ------------------------------------------------------------------ few rows an expert
-// An expert's rows against 128 columns of the activation (FC1: 8 waves, each 16
-// gate and the 16 up channels of the same columns) or 32 W channels (FC2).
-// Weights and rows go straight from memory into the matrix instruction: weights
-// are its rows, 16 NT tokens at a time its columns. Every wave sums the whole
-// of K, U blocks in flight.
-template <bool FC1, int NT, int W, int U>
-__global__ __launch_bounds__(W * 64) void fp8_stream_kernel(LayerArgs p) {
-  static_assert(W == (FC1 ? 8 : 4), "a workgroup has 128 columns");
-  __shared__ uint32_t tops[FC1 ? W : 1][NT * 16];
-  const int cblocks = FC1 ? p.inter / kBlock : p.c / (32 * W);
-  const int tile = blockIdx.x / cblocks, cb = blockIdx.x % cblocks;
-  if (tile >= p.tl->count) return;
-  const int4 t = p.tl->tiles[tile];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, q = lane >> 4;
-  const int kb = p.k / kBlock;
-  // the wave's first channel in either group of 16
-  const int c0 = FC1 ? cb * kBlock + wave * 16 : (cb * W + wave) * 32;
-  const int c1 = FC1 ? p.inter + c0 : c0 + 16;
-  const uint8_t* const w = p.w + static_cast<int64_t>(t.x) * p.c * p.k;
-  const uint8_t* const ws = p.ws + static_cast<int64_t>(t.x) * (p.c / kBlock) * kb;
-  const uint8_t* const w0 = w + static_cast<int64_t>(c0 + j) * p.k + 16 * q;
-  const uint8_t* const w1 = w + static_cast<int64_t>(c1 + j) * p.k + 16 * q;
-  const uint8_t* const s0 = ws + static_cast<int64_t>(c0 / kBlock) * kb;
-  const uint8_t* const s1 = ws + static_cast<int64_t>(c1 / kBlock) * kb;
-  for (int r = t.y; r < t.z; r += NT * 16) {
-    const uint8_t* x[NT];
-    const uint8_t* xs[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int i = min(r + n * 16 + j, t.z - 1);
-      const int64_t row = p.rows ? p.rows[i] : i;
-      x[n] = p.x + row * p.k + 16 * q;
-      xs[n] = p.xs + row * kb;
-    }
-    f32x4 acc[2][NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[0][n] = acc[1][n] = f32x4{0, 0, 0, 0};
-    auto steps = [&](auto count, int b) {
-      constexpr int N = decltype(count)::value;
-      i32x8 wv[N][2], xv[N][NT];
-      uint32_t sv[N][2], sx[N][NT];
-#pragma unroll
-      for (int u = 0; u < N; ++u) {
-        const int at = (b + u) * kBlock;
-        wv[u][0] = load32(w0 + at);
-        wv[u][1] = load32(w1 + at);
-        sv[u][0] = s0[b + u];
-        sv[u][1] = s1[b + u];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          xv[u][n] = load32(x[n] + at);
-          sx[u][n] = xs[n][b + u];
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < N; ++u)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int g = 0; g < 2; ++g) acc[g][n] = Op16::mac(wv[u][g], xv[u][n], acc[g][n], sv[u][g], sx[u][n]);
-    };
-    int b = 0;
-    for (; b + U <= kb; b += U) steps(std::integral_constant<int, U>{}, b);
-    for (; b < kb; ++b) steps(std::integral_constant<int, 1>{}, b);
-
-    if constexpr (FC1) {
-      float act[NT][4];
-      __syncthreads();  // the chunk before has read `tops`
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float weight = p.weight[min(r + n * 16 + j, t.z - 1)];
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          act[n][i] = gated_act(p.act_kind, acc[0][n][i], acc[1][n][i], p.beta, p.lbeta, p.limit) * weight;
-          top = max(top, abs_bits(act[n][i]));
-        }
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-        if (q == 0) tops[wave][n * 16 + j] = top;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int i = r + n * 16 + j;
-        uint32_t top = 0;
-#pragma unroll
-        for (int k = 0; k < W; ++k) top = max(top, tops[k][n * 16 + j]);
-        const BlockScale s(top);
-        if (i >= t.z) continue;
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + static_cast<int64_t>(i) * p.inter + c0 + 4 * q) =
-            s.pack4(act[n][0], act[n][1], act[n][2], act[n][3]);
-        if (wave == 0 && q == 0) p.out_scale[static_cast<int64_t>(i) * (p.inter / kBlock) + cb] = static_cast<uint8_t>(s.byte);
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int i = r + n * 16 + j;
-        if (i >= t.z) continue;
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-          *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + static_cast<int64_t>(i) * p.c + c0 + g * 16 + 4 * q) = acc[g][n];
-      }
-    }
-  }
-}
 
 // ------------------------------------------------------------------ many rows an expert
 // Rows of K bytes, K a multiple of 128: 16-byte vectors of a stage, NT threads.
@@ -184,7 +70,7 @@ struct RowPanel {
 
 // One tile of 16 MI WM rows of an expert by 256 channels: with FC1 128 columns
 // of the activation, a wave's channels gate and up of the same columns.
-template <bool FC1, int MI, int WM, int WN, int PRE>
+template <bool FC1, int MI, int WM, int WN>
 __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const int4& t, int cb) {
   constexpr int ROWS = kTile * MI, BM = ROWS * WM, BN = 256, NT = WM * WN * 64, COLS = BN / WN, NI = COLS / kTile;
   constexpr int GATE = NI / 2;  // tiles of gate channels (FC1)
@@ -213,7 +99,7 @@ __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const
   const uint8_t* const sb1 = ws + static_cast<int64_t>(FC1 ? p.inter / kBlock + cb : 0) * kb;
   auto sb = [&](int h, int block) -> uint32_t { return h ? sb1[block] : sb0[block]; };
   f32x4 acc[MI][NI];
-  tile_sums<Op16, BM, BN, WM, WN, 1, PRE, FC1 ? 2 : 1>(smem, pa, pb, p.k, sa, sb, acc);
+  tile_sums<Op16, BM, BN, WM, WN, 1, 1, FC1 ? 2 : 1>(smem, pa, pb, p.k, sa, sb, acc);
   __syncthreads();  // the stages are read
 
   if constexpr (FC1) {
@@ -279,28 +165,385 @@ __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const
   }
 }
 
-// A tile list's tile and a run of 256 channels (128 columns of the activation)
-// a workgroup. Tile m runs on XCD m % 8 with all its channels, so that its rows
-// come from one L2. The instructions fit the tile's rows: tiles of experts with
-// fewer do not multiply what is not there.
-template <bool FC1, int ROWS>
+// ------------------------------------------------------------------ weights streamed once
+// Items of up to 160 rows of an expert (the 160-row tile list) by 256 channels, one
+// after another in each of the chip's CUs. A stage is a block of K: the weights'
+// and the rows' bytes are copied straight to LDS, with their scale bytes, into a
+// ring of three; 2 x 4 waves multiply. A buffer is copied into again as soon as its
+// last fragment is read, and the copies run on into the next item: with a
+// workgroup for each item, alone on its CU by its LDS, the memory idled for 8 us in
+// front of an item, 7 behind it and 8 between workgroups, of 110 (4096 tokens, H
+// 7168, E 256 top-8). There FC1 has 7.5 GB of weights and takes 1.62 ms, 4.6 TB/s,
+// with LDS and the matrix unit each busy for 40% of it; 64 experts of 4 rows take
+// 277 us for 1.9 GB, 6.8 TB/s.
+//
+// The compiler does not know of the copies, so it waits for none by itself:
+// wait_copies and a barrier stand in front of what reads them. Loads that it knows
+// would wait for all of them: row numbers and tiles come through the scalar cache,
+// routing weights by a copy.
+typedef __attribute__((address_space(3))) void lds_void;
+__device__ __forceinline__ uint32_t lds_offset(const int8_t* p) {
+  return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)(p))));
+}
+// A wave's copy of 16 bytes a lane, lane l's to `lds` + 16 l.
+__device__ __forceinline__ void copy_lines(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
+}
+// The same of bytes that no other workgroup reads soon: they are the first that the caches let go.
+__device__ __forceinline__ void copy_lines_once(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "s"(lds) : "memory");
+}
+// Of a byte each in the first 26 lanes, lane l's to the word at `lds` + 4 l; every lane is active around it.
+__device__ __forceinline__ void copy_scales(const uint8_t* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 exec, 0x3ffffff\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off\n\ts_mov_b64 exec, -1"
+               ::"v"(p), "s"(lds) : "memory");
+}
+// Of a float a lane.
+__device__ __forceinline__ void copy_float(const float* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_copies() {  // until N of the wave's are left
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+}
+
+typedef int i32x8s __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ i32x4 scalar_load4(const void* p) {
+  i32x4 v;
+  asm volatile("s_load_dwordx4 %0, %1, 0x0\n\ts_waitcnt lgkmcnt(0)" : "=s"(v) : "s"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ i32x8s scalar_load8(const void* p) {
+  i32x8s v;
+  asm volatile("s_load_dwordx8 %0, %1, 0x0\n\ts_waitcnt lgkmcnt(0)" : "=s"(v) : "s"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ int pick(const i32x8s& v, int i) {
+  int r = v[0];
+#pragma unroll
+  for (int k = 1; k < 8; ++k) r = i == k ? v[k] : r;
+  return r;
+}
+
+namespace ring {
+constexpr int kRows = kStreamRows, kChannels = 256, kDepth = 3;
+constexpr int kPanels = (kRows + kChannels) * BK;  // bytes of a stage's rows and weights, in copies of 8 rows (1 KB)
+constexpr int kWaveScales = 32;                    // words of a wave's scales: its 24 rows', then the channels' two
+constexpr int kStage = kPanels + 8 * kWaveScales * 4;
+constexpr int kWeights = kDepth * kStage;  // routing weights of 192 rows
+constexpr int kBytes = kWeights + 192 * 4;
+constexpr int kCopies = 4 + 3 + 1;  // a wave and stage: of weights, of rows, of scales
+static_assert(kBytes <= 160 * 1024, "fits LDS");
+// where the scale of row r is: the wave that copies the row copies it too
+__device__ __forceinline__ int scale_slot(int r) { return (r >> 3 & 7) * kWaveScales + (r >> 6) * 8 + (r & 7); }
+}  // namespace ring
+
+template <bool FC1, bool ONCE>
+struct Ring {
+  struct Item {
+    const char* w;      // its first channel's weights
+    const char* x;      // the rows' base
+    int r0, rows, c0;   // expert-major rows from r0 on; first channel (FC1: column of the activation)
+    uint32_t off[3];    // the lane's bytes of the wave's copies of rows
+    const uint8_t* scale;  // the lane's scale, of block 0
+  };
+  const LayerArgs& p;
+  int8_t* const lds;
+  const uint32_t lds0;
+  const int lane, wave, wm, wn, kb, stages, cblocks, step, count;
+  uint32_t w_off[4];
+  Item cur, next;
+  int buf;
+
+  __device__ __forceinline__ Ring(const LayerArgs& args, int8_t* l)
+      : p(args), lds(l), lds0(lds_offset(l)), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
+        wm(wave / 4), wn(wave % 4), kb(args.k / kBlock),
+        stages(max(kb, ring::kDepth)),  // so that no item is passed over; a stage past K is not multiplied
+        cblocks(FC1 ? args.inter / kBlock : (args.c + 255) / 256), step(gridDim.x / 8),
+        count(__builtin_amdgcn_readfirstlane(args.tl->count)), buf(0) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int r = (v * 8 + wave) * 8 + lane / 8, in = r % 64;
+      // a wave's 64 channels: 32 of gate and the 32 of up for the same columns (FC1)
+      const int c = FC1 ? r / 64 * 32 + in % 32 + (in < 32 ? 0 : p.inter) : min(r, p.c - 1);
+      w_off[v] = static_cast<uint32_t>(c) * static_cast<uint32_t>(p.k) + slot(r);
+    }
+  }
+  // what slot_of keeps where this lane's 16 bytes of row r go
+  __device__ __forceinline__ uint32_t slot(int r) const { return ((lane & 7) ^ (r >> 1 & 7)) << 4; }
+  // XCD x takes the tiles x, x + 8, ... with all their channels, so that an expert's
+  // rows come from one L2; its workgroups take them in turn
+  __device__ __forceinline__ int tile_of(int n) const { return n / cblocks * 8 + static_cast<int>(blockIdx.x & 7); }
+
+  __device__ __forceinline__ void take(Item& it, int n) const {
+    const i32x4 t = scalar_load4(p.tl->tiles + tile_of(n));
+    const int cb = n % cblocks;
+    it.r0 = t[1];
+    it.rows = t[2] - t[1];
+    // the last 256 channels again where they are not a whole run
+    it.c0 = FC1 ? cb * kBlock : min(cb * 256, max(p.c - 256, 0));
+    it.w = reinterpret_cast<const char*>(p.w) + (static_cast<int64_t>(t[0]) * p.c + it.c0) * p.k;
+    it.x = reinterpret_cast<const char*>(p.x) + (FC1 ? 0 : static_cast<int64_t>(it.r0) * p.k);
+    int scale_row = 0;
+#pragma unroll
+    for (int v = 0; v < 3; ++v) {
+      const int r = min(v * 8 + wave, ring::kRows / 8 - 1) * 8;  // first row of the copy
+      // eight row numbers that hold it (those past the last row are the scratch's next bytes, and not picked)
+      const int first = min(r, (it.rows - 1) & ~7);
+      const i32x8s ids = FC1 ? scalar_load8(p.rows + it.r0 + first) : i32x8s{0, 1, 2, 3, 4, 5, 6, 7} + first;
+      it.off[v] = static_cast<uint32_t>(pick(ids, min(r + lane / 8, it.rows - 1) - first)) * static_cast<uint32_t>(p.k) +
+                  slot(r + lane / 8);
+      const int row = pick(ids, min(r + lane % 8, it.rows - 1) - first);
+      if (lane / 8 == v) scale_row = row;
+    }
+    const int h = lane - 24;  // 0 and 1: of gate and up, or of the run's two blocks of channels
+    const uint8_t* const ws = p.ws + static_cast<int64_t>(t[0]) * (p.c / kBlock) * kb;
+    const int channels = FC1 ? cb + (h & 1) * (p.inter / kBlock) : min(it.c0 / kBlock + (h & 1), p.c / kBlock - 1);
+    it.scale = h < 0 ? p.xs + ((FC1 ? 0 : static_cast<int64_t>(it.r0)) + scale_row) * kb : ws + static_cast<int64_t>(channels) * kb;
+  }
+
+  // Copies stage s of the current item, or of the next one behind its last.
+  __device__ __forceinline__ void copy(int s, int to_buf) const {
+    const bool in = s < stages;
+    const int block = min(in ? s : s - stages, kb - 1);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + to_buf * ring::kStage);
+    const char* const w = (in ? cur.w : next.w) + block * BK;
+    const char* const x = (in ? cur.x : next.x) + block * BK;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const uint32_t panel = to + ring::kRows * BK + (v * 8 + wave) * 1024;
+      if constexpr (ONCE)
+        copy_lines_once(w, w_off[v], panel);
+      else
+        copy_lines(w, w_off[v], panel);
+    }
+#pragma unroll
+    for (int v = 0; v < 3; ++v)
+      copy_lines(x, in ? cur.off[v] : next.off[v], to + min(v * 8 + wave, ring::kRows / 8 - 1) * 1024);
+    copy_scales((in ? cur.scale : next.scale) + block, to + ring::kPanels + wave * (ring::kWaveScales * 4));
+  }
+  __device__ __forceinline__ void copy_weights() const {  // of the current item's rows
+    const int w = wave % 3;
+    if constexpr (FC1) copy_float(p.weight + cur.r0 + min(w * 64 + lane, cur.rows - 1), lds0 + ring::kWeights + w * 256);
+  }
+
+  // The current item's sums for up to 32 MI rows, and what becomes of them. Leaves
+  // the last stage's buffer to be copied into.
+  template <int MI>
+  __device__ __forceinline__ void run() {
+    constexpr int NI = 4, ROWS = kTile * MI;
+    int id = lane;  // kept from the other heights' addresses, which would all be held in registers
+    asm volatile("" : "+v"(id));
+    const int j = id & 15, q = id >> 4;
+    auto bytes = [&](const int8_t* panel, int row) __attribute__((always_inline)) {
+      return join32(*reinterpret_cast<const i32x4*>(panel + slot_of(row, q)),
+                    *reinterpret_cast<const i32x4*>(panel + slot_of(row, 4 + q)));
+    };
+    auto bytes_a = [&](const int8_t* b, int i) __attribute__((always_inline)) { return bytes(b, wm * ROWS + i * kTile + j); };
+    auto bytes_b = [&](const int8_t* b, int c) __attribute__((always_inline)) {
+      return bytes(b + ring::kRows * BK, (wn * NI + c) * kTile + j);
+    };
+    int at[MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) at[i] = ring::scale_slot(wm * ROWS + i * kTile + j);
+    i32x8 fa[MI], fb;
+    uint32_t as[MI], bs[2], as_next[MI], bs_next[2];
+    auto scales = [&](const int8_t* b, uint32_t (&a)[MI], uint32_t (&c)[2]) __attribute__((always_inline)) {
+      const uint32_t* const from = reinterpret_cast<const uint32_t*>(b + ring::kPanels);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) a[i] = from[at[i]];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) c[h] = from[wave * ring::kWaveScales + 24 + h];
+    };
+    f32x4 acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int c = 0; c < NI; ++c) acc[i][c] = f32x4{0, 0, 0, 0};
+    const int8_t* b = lds + buf * ring::kStage;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) fa[i] = bytes_a(b, i);
+    fb = bytes_b(b, 0);
+    scales(b, as, bs);
+    auto stage = [&](int s, auto last) __attribute__((always_inline)) {
+      constexpr bool LAST = decltype(last)::value;
+      const int next_buf = buf + 1 == ring::kDepth ? 0 : buf + 1;
+      const int8_t* const now = lds + buf * ring::kStage;
+      const int8_t* const nxt = lds + next_buf * ring::kStage;
+#pragma unroll
+      for (int c = 0; c < NI; ++c) {
+        const bool tail = c == NI - 1;
+        if (tail) {  // every wave has read this stage, and its copies of the next have arrived
+          wait_copies<(ring::kDepth - 2) * ring::kCopies>();
+          __syncthreads();
+          if constexpr (!LAST) {
+            copy(s + ring::kDepth, buf);
+            scales(nxt, as_next, bs_next);
+          }
+        }
+        i32x8 fb_next = fb;
+        if (!(tail && LAST)) fb_next = tail ? bytes_b(nxt, 0) : bytes_b(now, c + 1);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          acc[i][c] = Op16::mac(fb, fa[i], acc[i][c], bs[FC1 ? c / 2 : wn / 2], as[i]);
+          if (tail && !LAST) fa[i] = bytes_a(nxt, i);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS read
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+          if (tail) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        fb = fb_next;
+      }
+      if constexpr (!LAST) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) as[i] = as_next[i];
+        bs[0] = bs_next[0];
+        bs[1] = bs_next[1];
+        buf = next_buf;
+      }
+    };
+    for (int s = 0; s + 1 < kb; ++s) stage(s, std::false_type{});
+    if (kb == stages) {
+      stage(kb - 1, std::true_type{});
+    } else {  // stages past K: their copies are waited for, and the next ones begun
+      stage(kb - 1, std::false_type{});
+      for (int s = kb; s < stages; ++s) {
+        wait_copies<(ring::kDepth - 2) * ring::kCopies>();
+        __syncthreads();
+        if (s + 1 < stages) {
+          copy(s + ring::kDepth, buf);
+          buf = buf + 1 == ring::kDepth ? 0 : buf + 1;
+        }
+      }
+    }
+    finish<MI>(acc, lds + buf * ring::kStage);
+  }
+
+  // `free`: a stage's bytes of LDS that nothing is copied into
+  template <int MI>
+  __device__ __forceinline__ void finish(f32x4 (&acc)[MI][4], int8_t* free) {
+    constexpr int ROWS = kTile * MI, BM = 2 * ROWS, NI = 4;
+    int lane = this->lane;
+    asm volatile("" : "+v"(lane));
+    if constexpr (FC1) {
+      constexpr int PITCH = kBlock + 16;
+      static_assert(BM * PITCH + 4 * BM * 4 <= ring::kStage, "epilogue staging");
+      const float* const weights = reinterpret_cast<const float*>(lds + ring::kWeights);
+      uint32_t* const tops = reinterpret_cast<uint32_t*>(free + BM * PITCH);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int r = wm * ROWS + i * kTile + token_of(lane);
+        const float weight = weights[r];
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float a = gated_act(p.act_kind, acc[i][c][v], acc[i][c + 2][v], p.beta, p.lbeta, p.limit) * weight;
+            acc[i][c][v] = a;
+            top = max(top, abs_bits(a));
+          }
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+        if (lane < 16) tops[wn * BM + r] = top;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int r = wm * ROWS + i * kTile + token_of(lane);
+        uint32_t top = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = max(top, tops[w * BM + r]);
+        const BlockScale s(top);
+        if (wn == 0 && lane < 16 && r < cur.rows)
+          p.out_scale[static_cast<int64_t>(cur.r0 + r) * (p.inter / kBlock) + cur.c0 / kBlock] = static_cast<uint8_t>(s.byte);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          *reinterpret_cast<uint32_t*>(free + r * PITCH + wn * 32 + c * kTile + channel_of(lane)) =
+              s.pack4(acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]);
+      }
+      __syncthreads();
+      for (int v = wave * 64 + lane; v < BM * 8; v += 512) {
+        const int r = v / 8, c = v % 8 * 16;
+        if (r < cur.rows)
+          *reinterpret_cast<i32x4*>(static_cast<uint8_t*>(p.out) + static_cast<int64_t>(cur.r0 + r) * p.inter + cur.c0 + c) =
+              *reinterpret_cast<const i32x4*>(free + r * PITCH + c);
+      }
+    } else {
+      constexpr int COLS = NI * kTile, PITCH = COLS * 4 + 16;
+      static_assert(8 * kTile * PITCH <= ring::kStage, "epilogue staging");
+      int8_t* const staged = free + wave * (kTile * PITCH);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+#pragma unroll
+        for (int c = 0; c < NI; ++c)
+          *reinterpret_cast<f32x4*>(staged + token_of(lane) * PITCH + (c * kTile + channel_of(lane)) * 4) = acc[i][c];
+        const int first = wm * ROWS + i * kTile, col = cur.c0 + wn * COLS + (lane & 15) * 4;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {  // 4 rows a wave at a time
+          const int r = v * 4 + (lane >> 4);
+          const f32x4 sum = *reinterpret_cast<const f32x4*>(staged + r * PITCH + (lane & 15) * 16);
+          if (first + r < cur.rows && col < p.c)
+            *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + static_cast<int64_t>(cur.r0 + first + r) * p.c + col) = sum;
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void all() {
+    int n = blockIdx.x >> 3;
+    if (tile_of(n) >= count) return;
+    take(cur, n);
+    for (int s = 0; s < ring::kDepth; ++s) copy(s, s);
+    copy_weights();
+    wait_copies<(ring::kDepth - 1) * ring::kCopies>();
+    __syncthreads();
+    for (;;) {
+      const bool more = tile_of(n + step) < count;
+      take(next, more ? n + step : n);
+      if (cur.rows <= 32)
+        run<1>();
+      else if (cur.rows <= 64)
+        run<2>();
+      else if (cur.rows <= 128)
+        run<4>();
+      else
+        run<5>();
+      if (!more) break;
+      __syncthreads();  // the buffer that the epilogue used
+      copy(stages - 1 + ring::kDepth, buf);
+      buf = buf + 1 == ring::kDepth ? 0 : buf + 1;
+      cur = next;
+      copy_weights();
+      n += step;
+    }
+    wait_copies<0>();  // nothing is copied into LDS that another workgroup has by then
+  }
+};
+
+template <bool FC1, bool ONCE>
+__global__ __launch_bounds__(512) void fp8_ring_kernel(LayerArgs p) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds[ring::kBytes];
+  Ring<FC1, ONCE>(p, lds).all();
+}
+
+// Experts of many rows, whose weights several tiles of the 256-row list read: tile
+// m runs on XCD m % 8 with all its channels, so that its rows come from one L2.
+template <bool FC1>
 __global__ __launch_bounds__(512) void fp8_rows_kernel(LayerArgs p) {
-  __shared__ __attribute__((aligned(1024))) int8_t lds[2 * (ROWS + 256) * BK];
+  __shared__ __attribute__((aligned(1024))) int8_t lds[2 * (256 + 256) * BK];
   const int cblocks = FC1 ? p.inter / kBlock : (p.c + 255) / 256;
   const int slot = blockIdx.x >> 3, tile = slot / cblocks * 8 + (blockIdx.x & 7), cb = slot % cblocks;
   if (tile >= p.tl->count) return;
   const int4 t = p.tl->tiles[tile];
-  const int rows = t.z - t.y;
-  if constexpr (ROWS == kStreamRows) {
-    if (rows <= 32) return rows_tile<FC1, 1, 2, 4, 1>(p, lds, t, cb);
-    if (rows <= 64) return rows_tile<FC1, 2, 2, 4, 1>(p, lds, t, cb);
-    if (rows <= 96) return rows_tile<FC1, 3, 2, 4, 1>(p, lds, t, cb);
-    if (rows <= 128) return rows_tile<FC1, 4, 2, 4, 1>(p, lds, t, cb);
-    rows_tile<FC1, 5, 2, 4, 1>(p, lds, t, cb);
-  } else {
-    if (rows <= 128) return rows_tile<FC1, 2, 4, 2, 1>(p, lds, t, cb);
-    rows_tile<FC1, 4, 4, 2, 1>(p, lds, t, cb);
-  }
+  if (t.z - t.y <= 128)
+    rows_tile<FC1, 2, 4, 2>(p, lds, t, cb);
+  else
+    rows_tile<FC1, 4, 4, 2>(p, lds, t, cb);
 }
 
 // out[t, :] = sum of the token's slots in slot order; a thread has 8 columns.
@@ -406,8 +649,9 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
   const Scratch s(scratch, R, E, hidden, inter);
   MM_CHECK_ARG(x && x_scale && selected && routing_weights && w1 && w1_scale && w2 && w2_scale && out,
                "mm_moe_fp8: null pointer");
-  MM_CHECK_ARG(((reinterpret_cast<uintptr_t>(scratch) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
-               "mm_moe_fp8: scratch and out must be 16-byte aligned");
+  MM_CHECK_ARG(((reinterpret_cast<uintptr_t>(scratch) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(x) |
+                 reinterpret_cast<uintptr_t>(w1) | reinterpret_cast<uintptr_t>(w2)) & 15) == 0,
+               "mm_moe_fp8: x, w1, w2, out and scratch must be 16-byte aligned");
   if (!scratch || scratch_bytes < s.bytes) {
     mm_set_error("mm_moe_fp8: scratch needs %zu bytes", s.bytes);
     return MM_E_WS;
@@ -424,15 +668,18 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
   const LayerArgs fc1{x, x_scale, s.send_token, w1, w1_scale, s.weight_perm, s.act, s.act_scale, tl, hidden, 2 * inter, inter,
                       act_kind, situ_beta, situ_linear_beta, clamp_limit};
   const LayerArgs fc2{s.act, s.act_scale, nullptr, w2, w2_scale, nullptr, s.y, nullptr, tl, inter, hidden, inter, 0, 0, 0, 0};
-  if (mean <= 16) {
-    rc = launch(fp8_stream_kernel<true, 1, 8, 2>, tiles * (inter / kBlock), 512, fc1, hs);
-    if (!rc) rc = launch(fp8_stream_kernel<false, 1, 4, 2>, tiles * (hidden / kBlock), 256, fc2, hs);
+  const int64_t fc1_items = tiles8 * (inter / kBlock), fc2_items = tiles8 * ((hidden + 255) / 256);
+  if (height == 256) {
+    rc = launch(fp8_rows_kernel<true>, fc1_items, 512, fc1, hs);
+    if (!rc) rc = launch(fp8_rows_kernel<false>, fc2_items, 512, fc2, hs);
   } else {
-    rc = launch(height == 256 ? fp8_rows_kernel<true, 256> : fp8_rows_kernel<true, kStreamRows>, tiles8 * (inter / kBlock),
-                512, fc1, hs);
-    if (!rc)
-      rc = launch(height == 256 ? fp8_rows_kernel<false, 256> : fp8_rows_kernel<false, kStreamRows>,
-                  tiles8 * ((hidden + 255) / 256), 512, fc2, hs);
+    const int64_t fc1_blocks = std::min<int64_t>(fc1_items, 256), fc2_blocks = std::min<int64_t>(fc2_items, 256);
+    // Weights that the last-level cache (256 MB) cannot hold from one call to the
+    // next pass it by: 604 MB of them in 75 us instead of 84 (FC1), 2.8 GB in 277
+    // instead of 306, but 38 MB in 19 instead of 16.
+    const bool once = std::min<int64_t>(R, E) * 3 * inter * hidden > (int64_t(192) << 20);
+    rc = launch(once ? fp8_ring_kernel<true, true> : fp8_ring_kernel<true, false>, fc1_blocks, 512, fc1, hs);
+    if (!rc) rc = launch(once ? fp8_ring_kernel<false, true> : fp8_ring_kernel<false, false>, fc2_blocks, 512, fc2, hs);
   }
   if (rc) return rc;
   const int64_t groups = (tokens * (hidden / 8) + 255) / 256;
