@@ -17,17 +17,134 @@ namespace {
 
 struct LayerArgs {
   const uint8_t* x;     // rows [., K]
+  const float* act;     // or, of a few rows' activation, in fp32
   const uint8_t* xs;    // their scales [., K / 128]
   const int32_t* rows;  // row of x of expert-major row i, or NULL: i
   const uint8_t* w;     // [E, C, K]
   const uint8_t* ws;    // [E, C / 128, K / 128]
   const float* weight;  // routing weight of row i (FC1)
-  void* out;            // E4M3 [R, I] (FC1) or fp32 [R, C]
+  void* out;            // E4M3 [R, I] (FC1; a few rows: fp32) or fp32 [R, C]
   uint8_t* out_scale;   // [R, I / 128] (FC1)
   const TileList* tl;
   int32_t k, c, inter, act_kind;
   float beta, lbeta, limit;
 };
+
+// 32 bytes of a row's block, at any alignment: 16 and the 16 that lie 64 behind.
+__device__ __forceinline__ i32x8 load32(const uint8_t* p) {
+  i32x4 lo, hi;
+  __builtin_memcpy(&lo, p, 16);
+  __builtin_memcpy(&hi, p + 64, 16);
+  return join32(lo, hi);
+}
+
+// ------------------------------------------------------------------ a few rows in all
+// Where the ring's tiles below would leave most CUs idle: an expert's rows against
+// 16 columns of the activation (the 16 gate and the 16 up channels) or 32 channels
+// of the result. The 4 waves share the blocks of K, 4 of them in flight in each, and
+// join their sums in LDS; weights are the matrix instruction's rows, 16 of the
+// expert's rows its columns. The activation passes in fp32: its 128 columns are in 8
+// workgroups, and each reader makes the same bytes of them in registers.
+// One token, H 2048, 8 experts of I 768: FC1 8.6 us for 25 MB, FC2 5.4 us for 13 MB,
+// which the ring's tiles take 16 and 9 for.
+template <bool FC1>
+__global__ __launch_bounds__(256) void fp8_few_kernel(LayerArgs p) {
+  constexpr int W = 4;
+  __shared__ f32x4 sums[W - 1][2][64];
+  const int groups = FC1 ? p.inter / 16 : p.c / 32;
+  const int tile = blockIdx.x / groups, c0 = blockIdx.x % groups * (FC1 ? 16 : 32);
+  if (tile >= p.tl->count) return;
+  const int4 t = p.tl->tiles[tile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, q = lane >> 4;
+  const int kb = p.k / kBlock, c1 = FC1 ? p.inter + c0 : c0 + 16;
+  const uint8_t* const w = p.w + static_cast<int64_t>(t.x) * p.c * p.k;
+  const uint8_t* const ws = p.ws + static_cast<int64_t>(t.x) * (p.c / kBlock) * kb;
+  const uint8_t* const w0 = w + static_cast<int64_t>(c0 + j) * p.k + 16 * q;
+  const uint8_t* const w1 = w + static_cast<int64_t>(c1 + j) * p.k + 16 * q;
+  const uint8_t* const s0 = ws + static_cast<int64_t>(c0 / kBlock) * kb;
+  const uint8_t* const s1 = ws + static_cast<int64_t>(c1 / kBlock) * kb;
+  for (int r = t.y; r < t.z; r += 16) {
+    const int at = min(r + j, t.z - 1);
+    const int64_t row = FC1 ? p.rows[at] : at;
+    const uint8_t* const x = p.x + row * p.k + 16 * q;
+    const uint8_t* const xs = p.xs + row * kb;
+    const float* const a = p.act + row * p.k + 16 * q;
+    f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    auto steps = [&](auto count, int b) {
+      constexpr int N = decltype(count)::value;
+      i32x8 wv[N][2], xv[N];
+      uint32_t sv[N][2], sx[N];
+      f32x4 av[N][8];
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const int block = b + u * W;
+        wv[u][0] = load32(w0 + block * kBlock);
+        wv[u][1] = load32(w1 + block * kBlock);
+        sv[u][0] = s0[block];
+        sv[u][1] = s1[block];
+        if constexpr (FC1) {
+          xv[u] = load32(x + block * kBlock);
+          sx[u] = xs[block];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            av[u][i] = *reinterpret_cast<const f32x4*>(a + block * kBlock + i / 4 * 64 + i % 4 * 4);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        if constexpr (!FC1) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) top = max(top, abs_bits(av[u][i][v]));
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+          const BlockScale s(top);
+          sx[u] = s.byte;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            xv[u][i] = static_cast<int>(s.pack4(av[u][i][0], av[u][i][1], av[u][i][2], av[u][i][3]));
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) acc[g] = Op16::mac(wv[u][g], xv[u], acc[g], sv[u][g], sx[u]);
+      }
+    };
+    int b = wave;
+    for (; b + 3 * W < kb; b += 4 * W) steps(std::integral_constant<int, 4>{}, b);
+    if (b + W < kb) {
+      steps(std::integral_constant<int, 2>{}, b);
+      b += 2 * W;
+    }
+    if (b < kb) steps(std::integral_constant<int, 1>{}, b);
+    if (wave) {
+      sums[wave - 1][0][lane] = acc[0];
+      sums[wave - 1][1][lane] = acc[1];
+    }
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int v = 0; v < W - 1; ++v) acc[g] += sums[v][g][lane];
+      const int i = r + j;
+      float* const out = static_cast<float*>(p.out) + static_cast<int64_t>(i) * (FC1 ? p.inter : p.c) + c0 + 4 * q;
+      if (i >= t.z) {
+      } else if constexpr (FC1) {
+        const float weight = p.weight[i];
+        f32x4 v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = gated_act(p.act_kind, acc[0][k], acc[1][k], p.beta, p.lbeta, p.limit) * weight;
+        *reinterpret_cast<f32x4*>(out) = v;
+      } else {
+        *reinterpret_cast<f32x4*>(out) = acc[0];
+        *reinterpret_cast<f32x4*>(out + 16) = acc[1];
+      }
+    }
+    __syncthreads();  // the sums are read
+  }
+}
 
 // ------------------------------------------------------------------ many rows an expert
 // Rows of K bytes, K a multiple of 128: 16-byte vectors of a stage, NT threads.
@@ -546,27 +663,40 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(LayerArgs p) {
     rows_tile<FC1, 4, 4, 2>(p, lds, t, cb);
 }
 
-// out[t, :] = sum of the token's slots in slot order; a thread has 8 columns.
-__global__ __launch_bounds__(256) void fp8_combine_kernel(const float* y, const int32_t* route_to_send, int64_t tokens,
+// out[t, :] = sum of the token's slots in slot order; a thread has 8 columns and
+// loads 4 slots at once. (8 slots one behind another took one token 5.6 us.)
+__global__ __launch_bounds__(256) void fp8_combine_kernel(const float* y, const int32_t* route_to_send, uint32_t tokens,
                                                           int32_t top_k, int32_t hidden, uint16_t* out) {
-  const int chunks = hidden / 8;
-  const int64_t total = tokens * chunks;
-  for (int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; v < total; v += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t token = v / chunks;
-    const int c = static_cast<int>(v - token * chunks) * 8;
+  const uint32_t chunks = hidden / 8, total = tokens * chunks;  // below 2^29
+  for (uint32_t v = blockIdx.x * 256 + threadIdx.x; v < total; v += gridDim.x * 256) {
+    const uint32_t token = v / chunks, c = (v - token * chunks) * 8;
+    const int32_t* const rows = route_to_send + static_cast<int64_t>(token) * top_k;
     float sum[8] = {};
-    for (int j = 0; j < top_k; ++j) {
-      const int32_t row = route_to_send[token * top_k + j];
-      if (row < 0) continue;
-      const f32x4* from = reinterpret_cast<const f32x4*>(y + static_cast<int64_t>(row) * hidden + c);
-      const f32x4 a = from[0], b = from[1];
+    auto slots = [&](auto count, int j) __attribute__((always_inline)) {
+      constexpr int N = decltype(count)::value;
+      int32_t row[N];
+      f32x4 a[N], b[N];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sum[i] += a[i];
-        sum[4 + i] += b[i];
+      for (int n = 0; n < N; ++n) row[n] = rows[j + n];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {  // a slot of no expert: a row that is not added
+        const f32x4* from = reinterpret_cast<const f32x4*>(y + static_cast<int64_t>(max(row[n], 0)) * hidden + c);
+        a[n] = from[0];
+        b[n] = from[1];
       }
-    }
-    *reinterpret_cast<uint4*>(out + token * hidden + c) =
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sum[i] = row[n] < 0 ? sum[i] : sum[i] + a[n][i];
+          sum[4 + i] = row[n] < 0 ? sum[4 + i] : sum[4 + i] + b[n][i];
+        }
+      }
+    };
+    int j = 0;
+    for (; j + 4 <= top_k; j += 4) slots(std::integral_constant<int, 4>{}, j);
+    for (; j < top_k; ++j) slots(std::integral_constant<int, 1>{}, j);
+    *reinterpret_cast<uint4*>(out + static_cast<int64_t>(token) * hidden + c) =
         make_uint4(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]), pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7]));
   }
 }
@@ -583,11 +713,23 @@ struct Carver {
   }
 };
 
+// Bytes of the weights that R rows read at most.
+int64_t weight_bytes(int64_t R, int E, int hidden, int inter) { return std::min<int64_t>(R, E) * 3 * inter * hidden; }
+
+// Up to 16 rows an expert that read up to 512 MB of weights are better off in
+// fp8_few_kernel, whose workgroups are many and short: one token takes 25 us with
+// it and 36 with the ring (38 MB), 4 tokens 46 and 50 (151 MB), 8 tokens 66 and 75
+// (302 MB), and with H 7168 one token 85 and 90 (352 MB), but 2 tokens 140 and 126
+// (705 MB).
+bool few_rows(int64_t R, int E, int hidden, int inter) {
+  return R <= int64_t(16) * E && weight_bytes(R, E, hidden, inter) <= int64_t(512) << 20;
+}
+
 struct Scratch {
   int32_t *counts, *offsets, *send_route, *send_token, *route_to_send;
   float* weight_perm;
   void *tiles, *route_ws;
-  uint8_t *act, *act_scale;
+  uint8_t *act, *act_scale;  // of a few rows in fp32
   float* y;
   size_t tiles_bytes, route_ws_bytes, bytes;
 
@@ -597,7 +739,7 @@ struct Scratch {
     tiles_bytes = mm_tile_lists_bytes(R, E);
     route_ws_bytes = mm_route_workspace_bytes(R, E);
     y = c.take<float>(r * hidden * 4);
-    act = c.take<uint8_t>(r * inter);
+    act = c.take<uint8_t>(r * inter * (few_rows(R, E, hidden, inter) ? 4 : 1));
     act_scale = c.take<uint8_t>(r * (inter / kBlock));
     route_ws = c.take<void>(route_ws_bytes);
     tiles = c.take<void>(tiles_bytes);
@@ -665,11 +807,14 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
   const int height = mean > kStreamRows ? 256 : kStreamRows;
   const TileList* tl = mm_tile_list_of(s.tiles, R, E, height);
   const int64_t tiles = mm_max_m_tiles(R, E, height), tiles8 = (tiles + 7) / 8 * 8;
-  const LayerArgs fc1{x, x_scale, s.send_token, w1, w1_scale, s.weight_perm, s.act, s.act_scale, tl, hidden, 2 * inter, inter,
+  const LayerArgs fc1{x, nullptr, x_scale, s.send_token, w1, w1_scale, s.weight_perm, s.act, s.act_scale, tl, hidden, 2 * inter, inter,
                       act_kind, situ_beta, situ_linear_beta, clamp_limit};
-  const LayerArgs fc2{s.act, s.act_scale, nullptr, w2, w2_scale, nullptr, s.y, nullptr, tl, inter, hidden, inter, 0, 0, 0, 0};
+  const LayerArgs fc2{s.act, reinterpret_cast<const float*>(s.act), s.act_scale, nullptr, w2, w2_scale, nullptr, s.y, nullptr, tl, inter, hidden, inter, 0, 0, 0, 0};
   const int64_t fc1_items = tiles8 * (inter / kBlock), fc2_items = tiles8 * ((hidden + 255) / 256);
-  if (height == 256) {
+  if (few_rows(R, E, hidden, inter)) {
+    rc = launch(fp8_few_kernel<true>, tiles * (inter / 16), 256, fc1, hs);
+    if (!rc) rc = launch(fp8_few_kernel<false>, tiles * (hidden / 32), 256, fc2, hs);
+  } else if (height == 256) {
     rc = launch(fp8_rows_kernel<true>, fc1_items, 512, fc1, hs);
     if (!rc) rc = launch(fp8_rows_kernel<false>, fc2_items, 512, fc2, hs);
   } else {
@@ -677,13 +822,13 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
     // Weights that the last-level cache (256 MB) cannot hold from one call to the
     // next pass it by: 604 MB of them in 75 us instead of 84 (FC1), 2.8 GB in 277
     // instead of 306, but 38 MB in 19 instead of 16.
-    const bool once = std::min<int64_t>(R, E) * 3 * inter * hidden > (int64_t(192) << 20);
+    const bool once = weight_bytes(R, E, hidden, inter) > int64_t(192) << 20;
     rc = launch(once ? fp8_ring_kernel<true, true> : fp8_ring_kernel<true, false>, fc1_blocks, 512, fc1, hs);
     if (!rc) rc = launch(once ? fp8_ring_kernel<false, true> : fp8_ring_kernel<false, false>, fc2_blocks, 512, fc2, hs);
   }
   if (rc) return rc;
   const int64_t groups = (tokens * (hidden / 8) + 255) / 256;
-  fp8_combine_kernel<<<static_cast<uint32_t>(groups < 65536 ? groups : 65536), 256, 0, hs>>>(s.y, s.route_to_send, tokens, top_k,
+  fp8_combine_kernel<<<static_cast<uint32_t>(groups < 65536 ? groups : 65536), 256, 0, hs>>>(s.y, s.route_to_send, static_cast<uint32_t>(tokens), top_k,
                                                                                              hidden, out);
   return mm_check_launch("fp8_combine_kernel");
 }
