@@ -558,8 +558,9 @@ int mm_fp8_matmul(const uint8_t* a, int64_t lda, const uint8_t* a_scale, const u
  * the routing weight) goes to FC2 in E4M3 with a scale for each 128 columns, the
  * experts' outputs to the sum over the slots in fp32. Routing as mm_route; a
  * NaN scale of a row makes that row's output NaN where any slot of it has an
- * expert. Scratch of mm_moe_fp8_scratch_bytes (0 for sizes out of range), 16-byte
- * aligned like out, free again when the stream has passed the call.
+ * expert. Scratch of mm_moe_fp8_scratch_bytes (0 for sizes out of range), free
+ * again when the stream has passed the call. x, w1, w2, out and scratch are
+ * 16-byte aligned; tokens * hidden and 2 * inter * hidden are below 2^32.
  */
 size_t mm_moe_fp8_scratch_bytes(int64_t tokens, int32_t top_k, int32_t num_experts,
                                 int32_t hidden, int32_t inter);

@@ -753,6 +753,9 @@ std::optional<Tensor> layer_forward_fp8(const Layer* layer, const Tensor& x, con
   if (tokens < 0 || !is_whole(x_scale, kE8m0, {tokens, l.hidden / kBlock}, x) ||
       !is_whole(gate_up, kE4m3, {l.experts, 2 * inter, l.hidden}, x))
     return std::nullopt;
+  for (const Tensor* t : {&x, &gate_up, &down})
+    CHECK_VALUE(reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0,
+                "tokens, gate_up and down must be aligned to 16 bytes");
   Tensor out = at::empty({tokens, l.hidden}, x.options().dtype(at::kBFloat16));
   if (!tokens) return out;
   const size_t bytes = entry.moe_fp8_scratch_bytes(tokens, static_cast<int32_t>(l.top_k), static_cast<int32_t>(l.experts),

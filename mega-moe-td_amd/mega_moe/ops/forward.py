@@ -485,7 +485,9 @@ class FusedMoEForward(torch.nn.Module):
         ``quantize_blocks`` make them; returns bf16 [T, H]. Sums are fp32; the
         activation (times the routing weight) goes to FC2 in E4M3 with a scale for
         each 128 columns, and the experts' outputs to the sum over the slots in
-        fp32. A NaN scale makes its own token's output NaN (where any slot of the
+        fp32. ``tokens`` and the experts' tensors are aligned to 16 bytes, as new
+        tensors and whole rows or experts of them are; T H and 2 I H are below
+        2^32. A NaN scale makes its own token's output NaN (where any slot of the
         token has an expert) and no other's. Nothing is saved for a backward and
         operands that ask for a gradient are refused; no workspace of the operator
         is used, so calls may run on any stream and captured. No counterpart in
