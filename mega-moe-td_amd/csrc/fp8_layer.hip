@@ -6,7 +6,7 @@
 //   y[i, :]   = act[i, :] W2[e]^T                      (fp32)
 //   out[t, :] = sum_j y[route_to_send[t k + j], :]     (fp32, slot order)
 //
-// Routing tables and tile lists are those of the bf16 layer. The experts' outputs
+// Routing tables and tile lists are those of the bf16 layer (a few rows need none). The experts' outputs
 // stay in fp32 until the slots are summed: in bf16 each would be off by as much
 // as the result is by its own rounding.
 #include <algorithm>
@@ -41,37 +41,62 @@ __device__ __forceinline__ i32x8 load32(const uint8_t* p) {
 // ------------------------------------------------------------------ a few rows in all
 // Where the ring's tiles below would leave most CUs idle: an expert's rows against
 // 16 columns of the activation (the 16 gate and the 16 up channels) or 32 channels
-// of the result. The 4 waves share the blocks of K, 4 of them in flight in each, and
-// join their sums in LDS; weights are the matrix instruction's rows, 16 of the
-// expert's rows its columns. The activation passes in fp32: its 128 columns are in 8
-// workgroups, and each reader makes the same bytes of them in registers.
-// One token, H 2048, 8 experts of I 768: FC1 8.6 us for 25 MB, FC2 5.4 us for 13 MB,
-// which the ring's tiles take 16 and 9 for.
+// of the result. A workgroup belongs to a route and takes all rows of its expert if
+// it is the expert's first: no tables, and a row is its route. The 4 waves share the
+// blocks of K, 4 of them in flight in each, and join their sums in LDS; weights are
+// the matrix instruction's rows, 16 of the expert's rows its columns. The activation
+// passes in fp32: its 128 columns are in 8 workgroups, and each reader makes the same
+// bytes of them in registers.
+// One token, H 2048, 8 experts of I 768: FC1 9 us for 25 MB, FC2 5.5 us for 13 MB,
+// which the ring's tiles take 16 and 9 for, behind 6 us of routing.
+constexpr int kFewRoutes = 256;
+
+struct FewArgs {
+  LayerArgs l;
+  const int32_t* selected;
+  int32_t routes, top_k, experts;
+};
+
 template <bool FC1>
-__global__ __launch_bounds__(256) void fp8_few_kernel(LayerArgs p) {
-  constexpr int W = 4;
+__global__ __launch_bounds__(kFewRoutes) void fp8_few_kernel(FewArgs f) {
+  constexpr int W = kFewRoutes / 64;
   __shared__ f32x4 sums[W - 1][2][64];
+  __shared__ int32_t rows[kFewRoutes], counts[W];
+  const LayerArgs& p = f.l;
   const int groups = FC1 ? p.inter / 16 : p.c / 32;
-  const int tile = blockIdx.x / groups, c0 = blockIdx.x % groups * (FC1 ? 16 : 32);
-  if (tile >= p.tl->count) return;
-  const int4 t = p.tl->tiles[tile];
+  const int route = blockIdx.x / groups, c0 = blockIdx.x % groups * (FC1 ? 16 : 32);
+  const int expert = f.selected[route];
+  if (expert < 0 || expert >= f.experts) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, q = lane >> 4;
+  const bool mine = static_cast<int>(threadIdx.x) < f.routes && f.selected[threadIdx.x] == expert;
+  const uint64_t of_wave = __ballot(mine);
+  if (lane == 0) counts[wave] = __popcll(of_wave);
+  __syncthreads();
+  int before = 0, count = 0;
+#pragma unroll
+  for (int v = 0; v < W; ++v) {
+    before += v < wave ? counts[v] : 0;
+    count += counts[v];
+  }
+  if (mine) rows[before + __popcll(of_wave & ((uint64_t(1) << lane) - 1))] = threadIdx.x;
+  __syncthreads();
+  if (rows[0] != route) return;
   const int kb = p.k / kBlock, c1 = FC1 ? p.inter + c0 : c0 + 16;
-  const uint8_t* const w = p.w + static_cast<int64_t>(t.x) * p.c * p.k;
-  const uint8_t* const ws = p.ws + static_cast<int64_t>(t.x) * (p.c / kBlock) * kb;
+  const uint8_t* const w = p.w + static_cast<int64_t>(expert) * p.c * p.k;
+  const uint8_t* const ws = p.ws + static_cast<int64_t>(expert) * (p.c / kBlock) * kb;
   const uint8_t* const w0 = w + static_cast<int64_t>(c0 + j) * p.k + 16 * q;
   const uint8_t* const w1 = w + static_cast<int64_t>(c1 + j) * p.k + 16 * q;
   const uint8_t* const s0 = ws + static_cast<int64_t>(c0 / kBlock) * kb;
   const uint8_t* const s1 = ws + static_cast<int64_t>(c1 / kBlock) * kb;
-  for (int r = t.y; r < t.z; r += 16) {
-    const int at = min(r + j, t.z - 1);
-    const int64_t row = FC1 ? p.rows[at] : at;
+  for (int r = 0; r < count; r += 16) {
+    const int i = rows[min(r + j, count - 1)];
+    const int64_t row = FC1 ? i / f.top_k : i;
     const uint8_t* const x = p.x + row * p.k + 16 * q;
     const uint8_t* const xs = p.xs + row * kb;
     const float* const a = p.act + row * p.k + 16 * q;
     f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    auto steps = [&](auto count, int b) {
-      constexpr int N = decltype(count)::value;
+    auto steps = [&](auto blocks, int b) {
+      constexpr int N = decltype(blocks)::value;
       i32x8 wv[N][2], xv[N];
       uint32_t sv[N][2], sx[N];
       f32x4 av[N][8];
@@ -128,9 +153,8 @@ __global__ __launch_bounds__(256) void fp8_few_kernel(LayerArgs p) {
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int v = 0; v < W - 1; ++v) acc[g] += sums[v][g][lane];
-      const int i = r + j;
       float* const out = static_cast<float*>(p.out) + static_cast<int64_t>(i) * (FC1 ? p.inter : p.c) + c0 + 4 * q;
-      if (i >= t.z) {
+      if (r + j >= count) {
       } else if constexpr (FC1) {
         const float weight = p.weight[i];
         f32x4 v;
@@ -664,20 +688,26 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(LayerArgs p) {
 }
 
 // out[t, :] = sum of the token's slots in slot order; a thread has 8 columns and
-// loads 4 slots at once. (8 slots one behind another took one token 5.6 us.)
-__global__ __launch_bounds__(256) void fp8_combine_kernel(const float* y, const int32_t* route_to_send, uint32_t tokens,
+// loads 4 slots at once (one token: 2.9 us, and 5.6 with one behind another).
+// Slots name their rows of y (-1: none) or, with ROUTES, their experts: then a
+// slot's row is its route. 4096 tokens of 8 slots, H 7168: 0.2 ms for 1 GB.
+template <bool ROUTES>
+__global__ __launch_bounds__(256) void fp8_combine_kernel(const float* y, const int32_t* slot, int32_t experts, uint32_t tokens,
                                                           int32_t top_k, int32_t hidden, uint16_t* out) {
   const uint32_t chunks = hidden / 8, total = tokens * chunks;  // below 2^29
   for (uint32_t v = blockIdx.x * 256 + threadIdx.x; v < total; v += gridDim.x * 256) {
     const uint32_t token = v / chunks, c = (v - token * chunks) * 8;
-    const int32_t* const rows = route_to_send + static_cast<int64_t>(token) * top_k;
+    const int64_t first = static_cast<int64_t>(token) * top_k;
     float sum[8] = {};
     auto slots = [&](auto count, int j) __attribute__((always_inline)) {
       constexpr int N = decltype(count)::value;
       int32_t row[N];
       f32x4 a[N], b[N];
 #pragma unroll
-      for (int n = 0; n < N; ++n) row[n] = rows[j + n];
+      for (int n = 0; n < N; ++n) {
+        row[n] = slot[first + j + n];
+        if constexpr (ROUTES) row[n] = row[n] >= 0 && row[n] < experts ? static_cast<int32_t>(first) + j + n : -1;
+      }
 #pragma unroll
       for (int n = 0; n < N; ++n) {  // a slot of no expert: a row that is not added
         const f32x4* from = reinterpret_cast<const f32x4*>(y + static_cast<int64_t>(max(row[n], 0)) * hidden + c);
@@ -716,39 +746,42 @@ struct Carver {
 // Bytes of the weights that R rows read at most.
 int64_t weight_bytes(int64_t R, int E, int hidden, int inter) { return std::min<int64_t>(R, E) * 3 * inter * hidden; }
 
-// Up to 16 rows an expert that read up to 512 MB of weights are better off in
-// fp8_few_kernel, whose workgroups are many and short: one token takes 25 us with
-// it and 36 with the ring (38 MB), 4 tokens 46 and 50 (151 MB), 8 tokens 66 and 75
-// (302 MB), and with H 7168 one token 85 and 90 (352 MB), but 2 tokens 140 and 126
-// (705 MB).
+// Up to 256 routes, on average up to 16 an expert, that read up to 512 MB of weights
+// are better off in fp8_few_kernel, whose workgroups are many and short:
+// one token takes 17 us with it and 33 with the ring (38 MB), 4 tokens 40 and 47
+// (151 MB), 8 tokens 63 and 72 (302 MB), and with H 7168 one token 79 and 88 (352
+// MB), but 2 tokens 135 and 123 (705 MB).
 bool few_rows(int64_t R, int E, int hidden, int inter) {
-  return R <= int64_t(16) * E && weight_bytes(R, E, hidden, inter) <= int64_t(512) << 20;
+  return R <= kFewRoutes && R <= int64_t(16) * E && weight_bytes(R, E, hidden, inter) <= int64_t(512) << 20;
 }
 
 struct Scratch {
   int32_t *counts, *offsets, *send_route, *send_token, *route_to_send;
   float* weight_perm;
   void *tiles, *route_ws;
-  uint8_t *act, *act_scale;  // of a few rows in fp32
+  uint8_t *act, *act_scale;  // act of a few rows: fp32
   float* y;
   size_t tiles_bytes, route_ws_bytes, bytes;
 
   Scratch(void* base, int64_t R, int E, int hidden, int inter) {
     Carver c{static_cast<char*>(base)};
     const size_t r = static_cast<size_t>(R);
+    const bool few = few_rows(R, E, hidden, inter);  // which needs no tables
     tiles_bytes = mm_tile_lists_bytes(R, E);
     route_ws_bytes = mm_route_workspace_bytes(R, E);
     y = c.take<float>(r * hidden * 4);
-    act = c.take<uint8_t>(r * inter * (few_rows(R, E, hidden, inter) ? 4 : 1));
-    act_scale = c.take<uint8_t>(r * (inter / kBlock));
-    route_ws = c.take<void>(route_ws_bytes);
-    tiles = c.take<void>(tiles_bytes);
-    counts = c.take<int32_t>(static_cast<size_t>(E) * 4);
-    offsets = c.take<int32_t>(static_cast<size_t>(E + 1) * 4);
-    send_route = c.take<int32_t>(r * 4);
-    send_token = c.take<int32_t>(r * 4);
-    route_to_send = c.take<int32_t>(r * 4);
-    weight_perm = c.take<float>(r * 4);
+    act = c.take<uint8_t>(r * inter * (few ? 4 : 1));
+    if (!few) {
+      act_scale = c.take<uint8_t>(r * (inter / kBlock));
+      route_ws = c.take<void>(route_ws_bytes);
+      tiles = c.take<void>(tiles_bytes);
+      counts = c.take<int32_t>(static_cast<size_t>(E) * 4);
+      offsets = c.take<int32_t>(static_cast<size_t>(E + 1) * 4);
+      send_route = c.take<int32_t>(r * 4);
+      send_token = c.take<int32_t>(r * 4);
+      route_to_send = c.take<int32_t>(r * 4);
+      weight_perm = c.take<float>(r * 4);
+    }
     bytes = c.used;
   }
 };
@@ -764,7 +797,8 @@ bool layer_sizes_ok(int64_t tokens, int32_t top_k, int32_t E, int32_t hidden, in
          int64_t(2) * inter * hidden < most;
 }
 
-int launch(void (*kernel)(LayerArgs), int64_t blocks, int threads, const LayerArgs& p, hipStream_t s) {
+template <class Args>
+int launch(void (*kernel)(Args), int64_t blocks, int threads, const Args& p, hipStream_t s) {
   MM_CHECK_ARG(blocks * threads < (int64_t(1) << 32), "mm_moe_fp8: too many tiles");
   kernel<<<static_cast<uint32_t>(blocks), threads, 0, s>>>(p);
   return mm_check_launch("mm_moe_fp8");
@@ -798,10 +832,25 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
     mm_set_error("mm_moe_fp8: scratch needs %zu bytes", s.bytes);
     return MM_E_WS;
   }
+  const hipStream_t hs = mm_hip_stream(stream);
+  const int64_t groups = std::min<int64_t>((tokens * (hidden / 8) + 255) / 256, 65536);  // of the slots' sums
+  if (few_rows(R, E, hidden, inter)) {
+    float* const act = reinterpret_cast<float*>(s.act);
+    const FewArgs fc1{{x, nullptr, x_scale, nullptr, w1, w1_scale, routing_weights, act, nullptr, nullptr, hidden, 2 * inter, inter,
+                       act_kind, situ_beta, situ_linear_beta, clamp_limit},
+                      selected, static_cast<int32_t>(R), top_k, E};
+    const FewArgs fc2{{nullptr, act, nullptr, nullptr, w2, w2_scale, nullptr, s.y, nullptr, nullptr, inter, hidden, inter, 0, 0, 0, 0},
+                      selected, static_cast<int32_t>(R), top_k, E};
+    int rc = launch(fp8_few_kernel<true>, R * (inter / 16), kFewRoutes, fc1, hs);
+    if (!rc) rc = launch(fp8_few_kernel<false>, R * (hidden / 32), kFewRoutes, fc2, hs);
+    if (rc) return rc;
+    fp8_combine_kernel<true><<<static_cast<uint32_t>(groups), 256, 0, hs>>>(s.y, selected, E, static_cast<uint32_t>(tokens), top_k,
+                                                                            hidden, out);
+    return mm_check_launch("fp8_combine_kernel");
+  }
   int rc = mm_route_tiles(selected, R, top_k, E, routing_weights, s.counts, s.offsets, s.send_route, s.send_token,
                           s.route_to_send, s.weight_perm, s.tiles, s.tiles_bytes, s.route_ws, s.route_ws_bytes, stream);
   if (rc) return rc;
-  const hipStream_t hs = mm_hip_stream(stream);
   // rows an expert on average
   const int64_t mean = (R + E - 1) / E;
   const int height = mean > kStreamRows ? 256 : kStreamRows;
@@ -809,12 +858,9 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
   const int64_t tiles = mm_max_m_tiles(R, E, height), tiles8 = (tiles + 7) / 8 * 8;
   const LayerArgs fc1{x, nullptr, x_scale, s.send_token, w1, w1_scale, s.weight_perm, s.act, s.act_scale, tl, hidden, 2 * inter, inter,
                       act_kind, situ_beta, situ_linear_beta, clamp_limit};
-  const LayerArgs fc2{s.act, reinterpret_cast<const float*>(s.act), s.act_scale, nullptr, w2, w2_scale, nullptr, s.y, nullptr, tl, inter, hidden, inter, 0, 0, 0, 0};
+  const LayerArgs fc2{s.act, nullptr, s.act_scale, nullptr, w2, w2_scale, nullptr, s.y, nullptr, tl, inter, hidden, inter, 0, 0, 0, 0};
   const int64_t fc1_items = tiles8 * (inter / kBlock), fc2_items = tiles8 * ((hidden + 255) / 256);
-  if (few_rows(R, E, hidden, inter)) {
-    rc = launch(fp8_few_kernel<true>, tiles * (inter / 16), 256, fc1, hs);
-    if (!rc) rc = launch(fp8_few_kernel<false>, tiles * (hidden / 32), 256, fc2, hs);
-  } else if (height == 256) {
+  if (height == 256) {
     rc = launch(fp8_rows_kernel<true>, fc1_items, 512, fc1, hs);
     if (!rc) rc = launch(fp8_rows_kernel<false>, fc2_items, 512, fc2, hs);
   } else {
@@ -827,8 +873,7 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
     if (!rc) rc = launch(once ? fp8_ring_kernel<false, true> : fp8_ring_kernel<false, false>, fc2_blocks, 512, fc2, hs);
   }
   if (rc) return rc;
-  const int64_t groups = (tokens * (hidden / 8) + 255) / 256;
-  fp8_combine_kernel<<<static_cast<uint32_t>(groups < 65536 ? groups : 65536), 256, 0, hs>>>(s.y, s.route_to_send, static_cast<uint32_t>(tokens), top_k,
-                                                                                             hidden, out);
+  fp8_combine_kernel<false><<<static_cast<uint32_t>(groups), 256, 0, hs>>>(s.y, s.route_to_send, E, static_cast<uint32_t>(tokens),
+                                                                           top_k, hidden, out);
   return mm_check_launch("fp8_combine_kernel");
 }
