@@ -46,8 +46,10 @@ __device__ __forceinline__ i32x8 load32(const uint8_t* p) {
 // blocks of K, 4 of them in flight in each, and join their sums in LDS; weights are
 // the matrix instruction's rows, 16 of the expert's rows its columns. The activation
 // passes in fp32: its 128 columns are in 8 workgroups, and each reader makes the same
-// bytes of them in registers.
-// One token, H 2048, 8 experts of I 768: FC1 9 us for 25 MB, FC2 5.5 us for 13 MB,
+// bytes of them in registers. FC1 sums in fp32 throughout: an activation that the
+// E4M3 instruction's sums put on the other side of a rounding border, 1 in 10^3 to
+// 10^4, is one of few here (one token: up to 0.005 of the result's norm).
+// One token, H 2048, 8 experts of I 768: FC1 9.5 us for 25 MB, FC2 5.5 us for 13 MB,
 // which the ring's tiles take 16 and 9 for, behind 6 us of routing.
 constexpr int kFewRoutes = 256;
 
@@ -59,6 +61,7 @@ struct FewArgs {
 
 template <bool FC1>
 __global__ __launch_bounds__(kFewRoutes) void fp8_few_kernel(FewArgs f) {
+  using OP = std::conditional_t<FC1, Op16Wide, Op16>;
   constexpr int W = kFewRoutes / 64;
   __shared__ f32x4 sums[W - 1][2][64];
   __shared__ int32_t rows[kFewRoutes], counts[W];
@@ -133,7 +136,7 @@ __global__ __launch_bounds__(kFewRoutes) void fp8_few_kernel(FewArgs f) {
             xv[u][i] = static_cast<int>(s.pack4(av[u][i][0], av[u][i][1], av[u][i][2], av[u][i][3]));
         }
 #pragma unroll
-        for (int g = 0; g < 2; ++g) acc[g] = Op16::mac(wv[u][g], xv[u], acc[g], sv[u][g], sx[u]);
+        for (int g = 0; g < 2; ++g) acc[g] = OP::mac(OP::frag(wv[u][g]), OP::frag(xv[u]), acc[g], sv[u][g], sx[u]);
       }
     };
     int b = wave;
@@ -209,9 +212,11 @@ struct RowPanel {
   __device__ __forceinline__ void put_cut(int8_t*, int, int) const {}
 };
 
+constexpr int kWideRows = 64;
+
 // One tile of 16 MI WM rows of an expert by 256 channels: with FC1 128 columns
 // of the activation, a wave's channels gate and up of the same columns.
-template <bool FC1, int MI, int WM, int WN>
+template <bool FC1, class OP, int MI, int WM, int WN, int PRE>
 __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const int4& t, int cb) {
   constexpr int ROWS = kTile * MI, BM = ROWS * WM, BN = 256, NT = WM * WN * 64, COLS = BN / WN, NI = COLS / kTile;
   constexpr int GATE = NI / 2;  // tiles of gate channels (FC1)
@@ -240,7 +245,7 @@ __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const
   const uint8_t* const sb1 = ws + static_cast<int64_t>(FC1 ? p.inter / kBlock + cb : 0) * kb;
   auto sb = [&](int h, int block) -> uint32_t { return h ? sb1[block] : sb0[block]; };
   f32x4 acc[MI][NI];
-  tile_sums<Op16, BM, BN, WM, WN, 1, 1, FC1 ? 2 : 1>(smem, pa, pb, p.k, sa, sb, acc);
+  tile_sums<OP, BM, BN, WM, WN, 1, PRE, FC1 ? 2 : 1>(smem, pa, pb, p.k, sa, sb, acc);
   __syncthreads();  // the stages are read
 
   if constexpr (FC1) {
@@ -380,7 +385,8 @@ static_assert(kBytes <= 160 * 1024, "fits LDS");
 __device__ __forceinline__ int scale_slot(int r) { return (r >> 3 & 7) * kWaveScales + (r >> 6) * 8 + (r & 7); }
 }  // namespace ring
 
-template <bool FC1, bool ONCE>
+// ONCE: weights that the caches need not keep. WIDE (FC1): sums in fp32 throughout for up to 64 rows.
+template <bool FC1, bool ONCE, bool WIDE>
 struct Ring {
   struct Item {
     const char* w;      // its first channel's weights
@@ -474,6 +480,7 @@ struct Ring {
   template <int MI>
   __device__ __forceinline__ void run() {
     constexpr int NI = 4, ROWS = kTile * MI;
+    constexpr bool EXACT = WIDE && MI <= 2;
     int id = lane;  // kept from the other heights' addresses, which would all be held in registers
     asm volatile("" : "+v"(id));
     const int j = id & 15, q = id >> 4;
@@ -512,6 +519,11 @@ struct Ring {
       const int next_buf = buf + 1 == ring::kDepth ? 0 : buf + 1;
       const int8_t* const now = lds + buf * ring::kStage;
       const int8_t* const nxt = lds + next_buf * ring::kStage;
+      Op16Wide::Frag wide[EXACT ? MI : 1];
+      if constexpr (EXACT) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) wide[i] = Op16Wide::frag(fa[i]);
+      }
 #pragma unroll
       for (int c = 0; c < NI; ++c) {
         const bool tail = c == NI - 1;
@@ -527,16 +539,27 @@ struct Ring {
         if (!(tail && LAST)) fb_next = tail ? bytes_b(nxt, 0) : bytes_b(now, c + 1);
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-          acc[i][c] = Op16::mac(fb, fa[i], acc[i][c], bs[FC1 ? c / 2 : wn / 2], as[i]);
-          if (tail && !LAST) fa[i] = bytes_a(nxt, i);
+          if constexpr (!EXACT) {
+            acc[i][c] = Op16::mac(fb, fa[i], acc[i][c], bs[FC1 ? c / 2 : wn / 2], as[i]);
+            if (tail && !LAST) fa[i] = bytes_a(nxt, i);
+          }
         }
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS read
+        if constexpr (EXACT) {
+          const Op16Wide::Frag fw = Op16Wide::frag(fb);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-          if (tail) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+          for (int i = 0; i < MI; ++i) {
+            acc[i][c] = Op16Wide::mac(fw, wide[i], acc[i][c], bs[c / 2], as[i]);
+            if (tail && !LAST) fa[i] = bytes_a(nxt, i);
+          }
+        } else {
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS read
+#pragma unroll
+          for (int i = 0; i < MI; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+            if (tail) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
         fb = fb_next;
       }
       if constexpr (!LAST) {
@@ -666,25 +689,33 @@ struct Ring {
   }
 };
 
-template <bool FC1, bool ONCE>
+template <bool FC1, bool ONCE, bool WIDE>
 __global__ __launch_bounds__(512) void fp8_ring_kernel(LayerArgs p) {
   __shared__ __attribute__((aligned(1024))) int8_t lds[ring::kBytes];
-  Ring<FC1, ONCE>(p, lds).all();
+  Ring<FC1, ONCE, WIDE>(p, lds).all();
 }
 
 // Experts of many rows, whose weights several tiles of the 256-row list read: tile
 // m runs on XCD m % 8 with all its channels, so that its rows come from one L2.
-template <bool FC1>
+// WIDE (FC1): sums in fp32 throughout, a workgroup for each 64 of a tile's rows.
+template <bool FC1, bool WIDE>
 __global__ __launch_bounds__(512) void fp8_rows_kernel(LayerArgs p) {
-  __shared__ __attribute__((aligned(1024))) int8_t lds[2 * (256 + 256) * BK];
+  __shared__ __attribute__((aligned(1024))) int8_t lds[2 * ((WIDE ? kWideRows : 256) + 256) * BK];
+  constexpr int parts = WIDE ? 256 / kWideRows : 1;
   const int cblocks = FC1 ? p.inter / kBlock : (p.c + 255) / 256;
-  const int slot = blockIdx.x >> 3, tile = slot / cblocks * 8 + (blockIdx.x & 7), cb = slot % cblocks;
+  const int slot = blockIdx.x >> 3, tile = slot / (cblocks * parts) * 8 + (blockIdx.x & 7);
+  const int cb = slot % (cblocks * parts) / parts, part = slot % parts;
   if (tile >= p.tl->count) return;
-  const int4 t = p.tl->tiles[tile];
-  if (t.z - t.y <= 128)
-    rows_tile<FC1, 2, 4, 2>(p, lds, t, cb);
-  else
-    rows_tile<FC1, 4, 4, 2>(p, lds, t, cb);
+  int4 t = p.tl->tiles[tile];
+  if constexpr (WIDE) {
+    t.y += part * kWideRows;
+    t.z = min(t.z, t.y + kWideRows);
+    if (t.y < t.z) rows_tile<FC1, Op16Wide, 2, 2, 4, 2>(p, lds, t, cb);
+  } else if (t.z - t.y <= 128) {
+    rows_tile<FC1, Op16, 2, 4, 2, 1>(p, lds, t, cb);
+  } else {
+    rows_tile<FC1, Op16, 4, 4, 2, 1>(p, lds, t, cb);
+  }
 }
 
 // out[t, :] = sum of the token's slots in slot order; a thread has 8 columns and
@@ -746,13 +777,12 @@ struct Carver {
 // Bytes of the weights that R rows read at most.
 int64_t weight_bytes(int64_t R, int E, int hidden, int inter) { return std::min<int64_t>(R, E) * 3 * inter * hidden; }
 
-// Up to 256 routes, on average up to 16 an expert, that read up to 512 MB of weights
-// are better off in fp8_few_kernel, whose workgroups are many and short:
-// one token takes 17 us with it and 33 with the ring (38 MB), 4 tokens 40 and 47
-// (151 MB), 8 tokens 63 and 72 (302 MB), and with H 7168 one token 79 and 88 (352
-// MB), but 2 tokens 135 and 123 (705 MB).
+// Up to 256 routes, on average up to 16 an expert, are better off in fp8_few_kernel, whose workgroups are many and
+// short, where they are no more than 64 or read no more than 512 MB of weights: H 2048, I 768, E 128 top-8 one token
+// 17.5 us (33 with the ring), 4 tokens 44 (47), 8 tokens 71 (72), 32 tokens (604 MB) 160 (118); H 7168, I 2048, E 64
+// one token 80 (88), 2 tokens 136 (137), 4 tokens 229 (233), 16 tokens (2.8 GB) 500 (431).
 bool few_rows(int64_t R, int E, int hidden, int inter) {
-  return R <= kFewRoutes && R <= int64_t(16) * E && weight_bytes(R, E, hidden, inter) <= int64_t(512) << 20;
+  return R <= kFewRoutes && R <= int64_t(16) * E && (R <= 64 || weight_bytes(R, E, hidden, inter) <= int64_t(512) << 20);
 }
 
 struct Scratch {
@@ -851,29 +881,45 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
   int rc = mm_route_tiles(selected, R, top_k, E, routing_weights, s.counts, s.offsets, s.send_route, s.send_token,
                           s.route_to_send, s.weight_perm, s.tiles, s.tiles_bytes, s.route_ws, s.route_ws_bytes, stream);
   if (rc) return rc;
+  const int64_t mean = (R + E - 1) / E;  // rows an expert
+  const LayerArgs fc1{x, nullptr, x_scale, s.send_token, w1, w1_scale, s.weight_perm, s.act, s.act_scale, nullptr, hidden, 2 * inter,
+                      inter, act_kind, situ_beta, situ_linear_beta, clamp_limit};
+  const LayerArgs fc2{s.act, nullptr, s.act_scale, nullptr, w2, w2_scale, nullptr, s.y, nullptr, nullptr, inter, hidden, inter, 0, 0, 0, 0};
+  // Weights that the last-level cache (256 MB) cannot hold from one call to the
+  // next pass it by: 604 MB of them in 75 us instead of 84 (FC1), 2.8 GB in 277
+  // instead of 306, but 38 MB in 19 instead of 16.
+  const bool once = weight_bytes(R, E, hidden, inter) > int64_t(192) << 20;
+  auto run = [&](void (*ring)(LayerArgs), void (*rows)(LayerArgs), LayerArgs p, int64_t cblocks) {
+    const int height = ring ? kStreamRows : 256;
+    const int64_t items = (mm_max_m_tiles(R, E, height) + 7) / 8 * 8 * cblocks;
+    p.tl = mm_tile_list_of(s.tiles, R, E, height);
+    // the ring takes a CU's items in turn
+    return launch(ring ? ring : rows, ring ? std::min<int64_t>(items, 256) : items, 512, p, hs);
+  };
   // By rows an expert on average: above 128 many have more than the ring's 160 and would stream their weights twice
   // (H 7168, I 2048, E 16: 120 rows 179 us with the ring and 196 in tiles of 256, 150 rows 282 and 219, 200 rows 343
   // and 230, 2000 rows 2.23 and 1.67 ms)
-  const int64_t mean = (R + E - 1) / E;
-  const int height = mean > 128 ? 256 : kStreamRows;
-  const TileList* tl = mm_tile_list_of(s.tiles, R, E, height);
-  const int64_t tiles = mm_max_m_tiles(R, E, height), tiles8 = (tiles + 7) / 8 * 8;
-  const LayerArgs fc1{x, nullptr, x_scale, s.send_token, w1, w1_scale, s.weight_perm, s.act, s.act_scale, tl, hidden, 2 * inter, inter,
-                      act_kind, situ_beta, situ_linear_beta, clamp_limit};
-  const LayerArgs fc2{s.act, nullptr, s.act_scale, nullptr, w2, w2_scale, nullptr, s.y, nullptr, tl, inter, hidden, inter, 0, 0, 0, 0};
-  const int64_t fc1_items = tiles8 * (inter / kBlock), fc2_items = tiles8 * ((hidden + 255) / 256);
-  if (height == 256) {
-    rc = launch(fp8_rows_kernel<true>, fc1_items, 512, fc1, hs);
-    if (!rc) rc = launch(fp8_rows_kernel<false>, fc2_items, 512, fc2, hs);
-  } else {
-    const int64_t fc1_blocks = std::min<int64_t>(fc1_items, 256), fc2_blocks = std::min<int64_t>(fc2_items, 256);
-    // Weights that the last-level cache (256 MB) cannot hold from one call to the
-    // next pass it by: 604 MB of them in 75 us instead of 84 (FC1), 2.8 GB in 277
-    // instead of 306, but 38 MB in 19 instead of 16.
-    const bool once = weight_bytes(R, E, hidden, inter) > int64_t(192) << 20;
-    rc = launch(once ? fp8_ring_kernel<true, true> : fp8_ring_kernel<true, false>, fc1_blocks, 512, fc1, hs);
-    if (!rc) rc = launch(once ? fp8_ring_kernel<false, true> : fp8_ring_kernel<false, false>, fc2_blocks, 512, fc2, hs);
-  }
+  const bool streamed = mean <= 128;
+  // The E4M3 instruction's sums are 1.5e-5 off, which moves 1 of 3000 activations by a step of E4M3, and the scale of 1
+  // of 25000 blocks: among many 0.0017 of the result's norm, as much as bf16 rounds. Among few it can be several times
+  // that (800 rows, I 128: 0.007 once in ten), so few are summed in fp32 throughout: up to 2 million where FC1 waits for
+  // weights anyhow (64 experts of 4 rows, H 7168: 468 us, 450 otherwise), else up to half a million (16 experts of 80
+  // rows, H 1024, I 256: 36 and 37 us, but 8 of 80, H 4096, I 1536: 125 and 78).
+  const bool wide = R * inter <= int64_t(1) << (mean <= 64 ? 21 : 19);
+  const int64_t fc1_cblocks = inter / kBlock, fc2_cblocks = (hidden + 255) / 256;
+  if (wide && mean <= 64)
+    rc = run(once ? fp8_ring_kernel<true, true, true> : fp8_ring_kernel<true, false, true>, nullptr, fc1, fc1_cblocks);
+  else if (wide)
+    rc = run(nullptr, fp8_rows_kernel<true, true>, fc1, fc1_cblocks * (256 / kWideRows));
+  else if (streamed)
+    rc = run(once ? fp8_ring_kernel<true, true, false> : fp8_ring_kernel<true, false, false>, nullptr, fc1, fc1_cblocks);
+  else
+    rc = run(nullptr, fp8_rows_kernel<true, false>, fc1, fc1_cblocks);
+  if (rc) return rc;
+  if (streamed)
+    rc = run(once ? fp8_ring_kernel<false, true, false> : fp8_ring_kernel<false, false, false>, nullptr, fc2, fc2_cblocks);
+  else
+    rc = run(nullptr, fp8_rows_kernel<false, false>, fc2, fc2_cblocks);
   if (rc) return rc;
   fp8_combine_kernel<false><<<static_cast<uint32_t>(groups), 256, 0, hs>>>(s.y, s.route_to_send, E, static_cast<uint32_t>(tokens),
                                                                            top_k, hidden, out);
