@@ -39,8 +39,8 @@ def operator(T, H, k, E, act="swiglu"):
                                     config=mega_moe.MoEForwardConfig(activation=act, **extra))
 
 
-def reference(x, sx, sel, ex, w, act):
-    """(output, bound of the error) in 64 bits on the CPU."""
+def reference(x, sx, sel, ex, w, act, wide=False):
+    """(output, bound of the error) in 64 bits on the CPU. ``wide``: gate and up are summed in fp32 throughout."""
     xv = R.values(x.cpu(), sx.cpu(), 1)
     T, H = xv.shape
     I = ex.down.shape[2]
@@ -54,7 +54,7 @@ def reference(x, sx, sel, ex, w, act):
         w1 = R.values(ex.gate_up[e].cpu(), ex.gate_up_scale[e].cpu(), 128)
         w2 = R.values(ex.down[e].cpu(), ex.down_scale[e].cpu(), 128)
         rows, weight = xv[token], w.cpu().double()[token, slot][:, None]
-        gu, off = rows @ w1.t(), R.sum_error(rows, w1)
+        gu, off = rows @ w1.t(), R.sum_error(rows, w1, wide)
         g, u = gu[:, :I], gu[:, I:]
         a = _act(act, g, u) * weight
         # gate's factor has a slope of at most 1.2 (SiTU-GLU: beta tanh(g / beta) <= g), up's of 1; 16 steps for the function itself

@@ -258,7 +258,10 @@ LAYERS = [  # tokens, hidden, inter, experts, top_k
     (1300, 256, 512, 128, 2),  # 512 tiles of FC1: two for each workgroup
     (800, 128, 128, 40, 1),    # one block of K in either product, a workgroup for a tile
     (1100, 384, 1152, 30, 3),  # 9 and 2 runs of channels, the last one of H half full
-    (640, 512, 896, 130, 4),   # weights past what a cache holds
+    (640, 512, 896, 130, 4),   # 20 rows an expert
+    (640, 512, 1024, 140, 4),  # 220 MB of weights, which pass the caches by
+    (150, 512, 1024, 140, 4),  # the same for few rows
+    (1500, 256, 512, 16, 6),   # 560 rows an expert
     (2000, 256, 256, 12, 1),   # 167 rows an expert: two tiles each
 ]
 
@@ -268,6 +271,22 @@ def test_layer_over_many_tiles(size):
     T, H, I, E, k = size
     ops = make(T, H, I, E, k, seed=T + I, drop=0.05)
     R.near(operator(T, H, k, E).forward_fp8(*ops), *reference(*ops, "swiglu"))
+
+
+FEW = [  # one for each way in which few activations are summed, and one past a tile's part of 64 rows
+    (1, 256, 128, 8, 2), (30, 1024, 384, 16, 4), (16, 640, 256, 2, 2),
+    (300, 384, 256, 60, 4), (900, 256, 384, 24, 2),
+    (200, 384, 256, 6, 4), (420, 512, 128, 3, 1), (700, 256, 256, 2, 2),
+]
+
+
+@pytest.mark.parametrize("size", FEW)
+@pytest.mark.parametrize("act", ["swiglu", "clamp_swiglu", "situglu"])
+def test_few_activations_are_summed_in_32_bits(size, act):
+    """An activation leaves its E4M3 step only where fp32 sums can carry it there."""
+    T, H, I, E, k = size
+    ops = make(T, H, I, E, k, seed=T * I)
+    R.near(operator(T, H, k, E, act).forward_fp8(*ops), *reference(*ops, act, wide=True))
 
 
 def test_layer_of_uneven_experts():
