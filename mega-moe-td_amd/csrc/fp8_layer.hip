@@ -320,8 +320,8 @@ __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const
 // workgroup for each item, alone on its CU by its LDS, the memory idled for 8 us in
 // front of an item, 7 behind it and 8 between workgroups, of 110 (4096 tokens, H
 // 7168, E 256 top-8). There FC1 has 7.5 GB of weights and takes 1.62 ms, 4.6 TB/s,
-// with LDS and the matrix unit each busy for 40% of it; 64 experts of 4 rows take
-// 277 us for 1.9 GB, 6.8 TB/s.
+// with LDS busy for 20% of it and the matrix unit for 31%; 64 experts of 4 rows take
+// 277 us for 1.9 GB, 6.8 TB/s (with WIDE 290).
 //
 // The compiler does not know of the copies, so it waits for none by itself:
 // wait_copies and a barrier stand in front of what reads them. Loads that it knows

@@ -131,7 +131,7 @@ class FusedMoEForward(torch.nn.Module):
         self._routing_generation = 0
         self._forward_stream = None
         self._device = None
-        self._few = None  # the native description of the layer for a few tokens,
+        self._few = None  # the native description of the layer (a few tokens, E4M3),
         self._few_of = None  # and the attributes that it was made of
         # optional runtime.timing.StageTimer: HIP events between stages
         # (MOE_FWD_TIMING=1 attaches one, as the reference's phase stamps are
@@ -485,7 +485,8 @@ class FusedMoEForward(torch.nn.Module):
         ``quantize_blocks`` make them; returns bf16 [T, H]. Sums are fp32; the
         activation (times the routing weight) goes to FC2 in E4M3 with a scale for
         each 128 columns, and the experts' outputs to the sum over the slots in
-        fp32. ``tokens`` and the experts' tensors are aligned to 16 bytes, as new
+        fp32. Few activations are summed in fp32 before they are rounded, many by the
+        E4M3 instruction, which is 1.4e-5 off. ``tokens`` and the experts' tensors are aligned to 16 bytes, as new
         tensors and whole rows or experts of them are; T H and 2 I H are below
         2^32. A NaN scale makes its own token's output NaN (where any slot of the
         token has an expert) and no other's. Nothing is saved for a backward and
