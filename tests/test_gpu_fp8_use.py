@@ -406,3 +406,65 @@ def test_layer_past_32_bits():
     at = torch.arange(T - 64, T) % 64
     R.near(out[-64:], ref[at], bound[at])
     assert torch.equal(out[: 64 * (reps - 1)].view(reps - 1, 64, H), out[:64].expand(reps - 1, 64, H))
+
+
+# ------------------------------------------------------------------ what is not a number, and nothing
+@pytest.mark.parametrize("size", [(6, 256, 128, 4, 2), (400, 384, 256, 16, 2), (640, 512, 896, 130, 4), (200, 256, 128, 4, 2),
+                                  (1500, 256, 512, 16, 6)])
+def test_layer_keeps_bad_tokens_to_themselves(size):
+    """A NaN byte, a NaN scale and infinite weights in a token, on each of the layer's ways."""
+    T, H, I, E, k = size
+    x, sx, sel, ex, w = make(T, H, I, E, k, seed=61)
+    op = operator(T, H, k, E)
+    clean = op.forward_fp8(x, sx, sel, ex, w)
+    x.view(torch.uint8)[1, 77] = 0x7F
+    sx.view(torch.uint8)[2, 1] = 255
+    w[3, 0] = float("nan")
+    w[4, k - 1] = float("inf")
+    out = op.forward_fp8(x, sx, sel, ex, w)
+    assert out[1].isnan().all() and out[2].isnan().all() and out[3].isnan().all() and out[4].isnan().all()
+    rest = [0, *range(5, T)]
+    assert torch.equal(out[rest], clean[rest])
+
+
+def test_layer_keeps_a_bad_expert_to_its_tokens():
+    T, H, I, E, k = 300, 256, 256, 8, 2
+    x, sx, sel, ex, w = make(T, H, I, E, k, seed=62)
+    op = operator(T, H, k, E)
+    clean = op.forward_fp8(x, sx, sel, ex, w)
+    ex.down_scale.view(torch.uint8)[3, 1, 0] = 255  # columns 128-255 of what expert 3 gives
+    out = op.forward_fp8(x, sx, sel, ex, w)
+    hit = (sel == 3).any(1)
+    assert out[hit][:, 128:].isnan().all() and torch.equal(out[hit][:, :128], clean[hit][:, :128])
+    assert torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("m", [5, 40, 400])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_product_of_nan_bytes(m, dtype):
+    gen = torch.Generator().manual_seed(63)
+    a, sa = R.rows_e4m3(gen, m, 300)
+    b, sb = R.blocks_e4m3(gen, 200, 300)
+    clean = mega_moe.fp8_matmul(a, b, sa, sb, out_dtype=dtype)
+    a.view(torch.uint8)[2, 299] = 0xFF
+    b.view(torch.uint8)[7, 0] = 0x7F
+    out = mega_moe.fp8_matmul(a, b, sa, sb, out_dtype=dtype)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[2], bad[:, 7] = True, True
+    assert torch.equal(out.isnan(), bad) and torch.equal(out[~bad], clean[~bad])
+
+
+def test_nothing():
+    """No rows, no columns, no matrices."""
+    empty = lambda *s: torch.empty(*s, dtype=BF, device="cuda")
+    for shape, rows, scales in (((0, 300), 1, (0, 3)), ((5, 0), 1, (5, 0)), ((0, 300), 128, (0, 3)), ((300, 0), 128, (3, 0)),
+                                ((0, 4, 300), 128, (0, 1, 3)), ((2, 0, 7), 1, (2, 0, 1))):
+        q, s = mega_moe.quantize_blocks(empty(*shape), rows)
+        assert q.shape == shape and s.shape == scales and q.dtype == F8 and s.dtype == E8
+    q, s = mega_moe.rms_norm(empty(0, 300), out_dtype=F8, scale_columns=128)
+    assert q.shape == (0, 300) and s.shape == (0, 3)
+    gen = torch.Generator().manual_seed(64)
+    b, sb = R.blocks_e4m3(gen, 200, 300)
+    assert mega_moe.fp8_matmul(q, b, s, sb, out_dtype=F32).shape == (0, 200)
+    assert mega_moe.fp8_linear(empty(0, 300), empty(40, 300)).shape == (0, 40)
+    assert mega_moe.fp8_linear(empty(300), empty(40, 300)).shape == (40,)
