@@ -156,6 +156,7 @@ __device__ __forceinline__ void tile_sums(int8_t (&smem)[2][(BM + BN) * KS * BK]
   // over one by one. (All fragments of a stage read ahead in one go take the
   // registers of a second workgroup: 128 x 128 tiles, 4096^3, 113 us so, 136.)
   static_assert(NI > 1, "moves stand between tiles of channels");
+  static_assert(PRE == 1 || PRE == 2, "a turn of the loop is PRE stages");
   constexpr int SHARE = (MOVES + NI - 2) / (NI - 1);  // moves a step
   typename OP::Frag fa[MI], fb;
   __syncthreads();
