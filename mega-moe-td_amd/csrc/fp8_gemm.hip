@@ -263,24 +263,28 @@ int launch_tiles(const Fp8Args& p, hipStream_t s) {
   return launch(fp8_tile_kernel<OP, BM, BN, WM, WN, KS, PRE, SHIFT>, tiles_of(p, BM, BN), WM * WN * KS * 64, p, s);
 }
 
-// Time of a product in us by its tiles, about 4 us in all and `tile` and `byte` a
+// Time of a product in us by its tiles, about 2.5 us in all and `tile` and `byte` a
 // byte of K for every 256 of them, as measured on full rounds (2048 x 2048 x 1024
-// and 8192 in 128 x 128 tiles, 256 of them: 11.5 and 55 us). Where a CU holds
-// several tiles a part of a round costs what its share is, or 0.42 of a round
-// (968 x 4992 x 6016, 312 such tiles: 58 us, 42 for up to 256).
+// and 8192 in 128 x 128 tiles, 256 of them: 11.6 and 53 us; 1024 x 2048 in 64 x 128
+// tiles 7.6 and 31, whose waves read as much of LDS for a product as those of 128 x
+// 128). Where a CU holds several tiles a part of a round costs what its share is, or
+// 0.42 of a round (968 x 4992 x 6016, 312 tiles of 128 x 128: 58 us, 40 for up to 256).
 struct TileCost {
   int bm, bn, step;  // step: K has to reach one whole stage
   double tile, byte;
   bool several;
 };
 constexpr TileCost kTileCosts[] = {
-    {256, 256, 128, 6.0, 13.2e-3, false}, {128, 128, 128, 1.3, 6.1e-3, true}, {64, 64, 128, 0.2, 2.85e-3, true},
-    {32, 64, 512, 1.0, 1.67e-3, false},   {32, 32, 1024, 1.4, 1.0e-3, false},
+    {256, 256, 128, 5.6, 14.0e-3, false}, {128, 128, 128, 2.8, 5.76e-3, true}, {64, 128, 256, 1.8, 3.26e-3, false},
+    {64, 64, 128, 0.4, 2.75e-3, true},    {32, 64, 512, 1.0, 1.72e-3, false},  {32, 32, 1024, 1.9, 1.07e-3, false},
 };
-// Results in 32 bits (2048 x 2048 x 4096 in 128 x 128 tiles: 62 us; 1024 x 1024 x
-// 4096 in 64 x 64: 24; 64 x 4096 x 7168 in 32 x 64: 22).
-constexpr TileCost kWideCosts[] = {
-    {128, 128, 128, 0.5, 14.1e-3, true}, {64, 64, 128, 0.2, 4.8e-3, true}, {32, 64, 512, 0.5, 2.6e-3, false}};
+// Results in 32 bits (2048 x 2048 x 1024 and 8192 in 128 x 128 tiles 19 and 107 us,
+// in 64 x 128 tiles 17 and 92; 1024 x 1024 x 4096 in 64 x 64: 24; 64 x 4096 x 7168 in
+// 32 x 64: 21).
+constexpr TileCost kWideCosts[] = {{128, 128, 128, 3.8, 12.3e-3, true},
+                                   {64, 128, 128, 1.8, 5.3e-3, true},
+                                   {64, 64, 128, 0.2, 4.8e-3, true},
+                                   {32, 64, 512, 0.5, 2.6e-3, false}};
 
 template <int N>
 int best_tile(const TileCost (&costs)[N], const Fp8Args& p) {
@@ -315,9 +319,13 @@ int launch_best(const Fp8Args& p, hipStream_t s) {
   // 64 x 64: the sum shared by two groups of waves until the chip is full
   const bool shared = p.k >= 2 * BK && tiles_of(p, 64, 64) <= 256;
   if (wide) {
-    switch (best_tile(kWideCosts, p)) {
+    // 128 x 128 where a CU always holds two: a round costs 0.7 of one alone (4096 x 4096 x 8192: 302 us, in 64 x 128 328)
+    switch (tiles_of(p, 128, 128) >= 1024 ? 0 : best_tile(kWideCosts, p)) {
       case 0: return launch_tiles<Op16Wide, 128, 128, 2, 2, 1, 1, false>(p, s);
       case 1:
+        return p.k >= 2 * BK && tiles_of(p, 64, 128) <= 256 ? launch_any<Op16Wide, 64, 128, 2, 2, 2, 1>(p, shift, s)
+                                                            : launch_any<Op16Wide, 64, 128, 2, 2, 1, 1>(p, shift, s);
+      case 2:
         return shared ? launch_any<Op16Wide, 64, 64, 2, 2, 2, 1>(p, shift, s) : launch_any<Op16Wide, 64, 64, 2, 2, 1, 1>(p, shift, s);
       default: return launch_any<Op16Wide, 32, 64, 1, 2, 4, 1>(p, shift, s);
     }
@@ -325,8 +333,9 @@ int launch_best(const Fp8Args& p, hipStream_t s) {
   switch (best_tile(kTileCosts, p)) {
     case 0: return launch_tiles<Op16, 256, 256, 4, 2, 1, 1, false>(p, s);
     case 1: return launch_tiles<Op16, 128, 128, 2, 2, 1, 2, false>(p, s);
-    case 2: return shared ? launch_any<Op16, 64, 64, 2, 2, 2, 2>(p, shift, s) : launch_any<Op16, 64, 64, 2, 2, 1, 2>(p, shift, s);
-    case 3: return launch_any<Op16, 32, 64, 1, 2, 4, 2>(p, shift, s);
+    case 2: return launch_any<Op16, 64, 128, 2, 2, 2, 1>(p, shift, s);
+    case 3: return shared ? launch_any<Op16, 64, 64, 2, 2, 2, 2>(p, shift, s) : launch_any<Op16, 64, 64, 2, 2, 1, 2>(p, shift, s);
+    case 4: return launch_any<Op16, 32, 64, 1, 2, 4, 2>(p, shift, s);
     default: return launch_any<Op16, 32, 32, 1, 1, 8, 1>(p, shift, s);
   }
 }
