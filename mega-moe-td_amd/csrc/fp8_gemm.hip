@@ -26,12 +26,34 @@ struct Fp8Args {
   int32_t m, n, k, kb, out_type, bias_type;
 };
 
+// The bias of columns col .. col + 3 and of those 16 N behind them; past the last
+// one it is repeated. All loads of one type are in flight at once: a branch around
+// each had every one waited for (2.5 us of a tile's end).
+template <class T, int N>
+__device__ __forceinline__ void load_bias_of(const Fp8Args& p, int col, f32x4 (&b)[N]) {
+  const T* const bias = static_cast<const T*>(p.bias);
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) b[j][r] = static_cast<float>(bias[min(col + j * kTile + r, p.n - 1)]);
+}
+template <int N>
+__device__ __forceinline__ void load_bias(const Fp8Args& p, int col, f32x4 (&b)[N]) {
+  if (p.bias_type == MM_T_FP32)
+    load_bias_of<float>(p, col, b);
+  else if (p.bias_type == MM_T_FP16)
+    load_bias_of<_Float16>(p, col, b);
+  else
+    load_bias_of<bf16>(p, col, b);
+}
+
 // Columns col .. col + 3 of a row, from their sums.
 __device__ __forceinline__ void store4(const Fp8Args& p, int row, int col, f32x4 f) {
   const int left = p.n - col;
   if (p.bias) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) f[r] += load_any(p.bias, p.bias_type, min(col + r, p.n - 1));
+    f32x4 b[1];
+    load_bias(p, col, b);
+    f += b[0];
   }
   const int64_t at = row * p.ldo + col;
   if (p.out_type == MM_T_FP32) {
@@ -163,8 +185,8 @@ __global__ __launch_bounds__(W * 64) void fp8_direct_kernel(Fp8Args p) {
 // of a wave at a time go through its own LDS, padded to spread a pass
 // over the banks, so that neighbouring lanes store neighbouring 16 bytes. Large
 // products are bound by the matrix unit's power (8192 x 7168 x 4096: 202-212 us,
-// 2270-2380 TFLOP/s), small ones by the latency of their stages (1021 x 2304 x
-// 1793: 13 us) and the shifting of odd rows (K = 2309: 19 us), 17-64 rows by the
+// 2270-2380 TFLOP/s), small ones by LDS bandwidth (1021 x 2304 x 1793: 11.7 us)
+// and the shifting of odd rows (K = 2309 with a bias: 16.5 us), 17-64 rows by the
 // panels' way from L2 (64 x 7168 x 4096: 10.8 us).
 template <class OP, int BM, int BN, int WM, int WN, int KS, int PRE, bool SHIFT>
 __global__ __launch_bounds__(WM * WN * KS * 64, OP::WAVES) void fp8_tile_kernel(Fp8Args p) {
@@ -218,17 +240,21 @@ __global__ __launch_bounds__(WM * WN * KS * 64, OP::WAVES) void fp8_tile_kernel(
   }
   int8_t* const staged = &smem[0][0] + wave * (R * PITCH);
   const int c0 = n0 + wn * COLS, lane_row = token_of(lane);
+  if (p.bias) {
+    f32x4 b[NI];
+    load_bias(p, c0 + channel_of(lane), b);
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] += b[j];
+  }
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int r0 = m0 + wm * (BM / WM) + i * R;
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int c = j * R + channel_of(lane);
-      f32x4 f = acc[i][j];
-      if (p.bias) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) f[r] += load_any(p.bias, p.bias_type, min(c0 + c + r, p.n - 1));
-      }
+      const f32x4 f = acc[i][j];
       if (p.out_type == MM_T_FP32)
         *reinterpret_cast<f32x4*>(staged + lane_row * PITCH + c * 4) = f;
       else
