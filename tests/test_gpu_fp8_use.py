@@ -468,3 +468,21 @@ def test_nothing():
     assert mega_moe.fp8_matmul(q, b, s, sb, out_dtype=F32).shape == (0, 200)
     assert mega_moe.fp8_linear(empty(0, 300), empty(40, 300)).shape == (0, 40)
     assert mega_moe.fp8_linear(empty(300), empty(40, 300)).shape == (40,)
+
+
+# ------------------------------------------------------------------ products in tiles of 64 x 128
+@pytest.mark.parametrize("m,n,k", [(1000, 1900, 2100), (1000, 1899, 2101), (1793, 2305, 1000), (960, 1920, 257)])
+@pytest.mark.parametrize("dtype,bias", [(BF, None), (torch.float16, F32), (F32, BF)])
+def test_product_of_a_thousand_rows(m, n, k, dtype, bias):
+    gen = torch.Generator().manual_seed(m + k)
+    a, sa = R.rows_e4m3(gen, m, k, low=-8, high=-4)
+    b, sb = R.blocks_e4m3(gen, n, k, low=-8, high=-4)
+    add = None if bias is None else torch.randn(n, generator=gen).to(bias).cuda()
+    av, bv = R.values(a, sa, 1), R.values(b, sb, 128)
+    ref, off = av @ bv.t(), R.sum_error(av, bv, wide=dtype == F32)
+    if bias is not None:
+        ref = ref + add.double()
+        off = off + 2.0 ** -23 * (ref.abs() + off)
+    got = mega_moe.fp8_matmul(a, b, sa, sb, bias=add, out_dtype=dtype)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    R.near(got, ref, off + R.half_step(dtype) * (ref.abs() + off) + tiny)
