@@ -253,28 +253,25 @@ bool sizes_ok(int64_t batch, int64_t rows, int64_t cols) {
   return batch * rows <= most && batch * rows <= most * 2 / kb;
 }
 
-constexpr uint64_t kMaxGroups = (uint64_t(1) << 24) - 1;  // of 256 threads
+int launch(void (*kernel)(QuantArgs), uint64_t groups, uint32_t threads, const QuantArgs& p, hipStream_t s) {
+  MM_CHECK_ARG(groups * threads < uint64_t(1) << 32, "mm_quantize_blocks: too many blocks");  // what a grid holds
+  kernel<<<static_cast<uint32_t>(groups), threads, 0, s>>>(p);
+  return mm_check_launch("mm_quantize_blocks");
+}
 
 template <class T>
 int launch_rows(const QuantArgs& p, hipStream_t s) {
-  const uint64_t groups = (p.units + 63) / 64;
-  MM_CHECK_ARG(groups <= kMaxGroups, "mm_quantize_blocks: too many blocks");
-  quantize_rows_kernel<T><<<static_cast<uint32_t>(groups), 256, 0, s>>>(p);
-  return mm_check_launch("quantize_rows_kernel");
+  return launch(quantize_rows_kernel<T>, (p.units + 63) / 64, 256, p, s);
 }
 
 template <class T, bool BLOCK>
 int launch_tiles(const QuantArgs& p, hipStream_t s) {
   const uint64_t tiles = static_cast<uint64_t>(p.batch) * ((p.rows + 127) / 128) * p.kb;
-  MM_CHECK_ARG(tiles <= kMaxGroups, "mm_quantize_blocks: too many blocks");
   // 1024 threads a tile wait for fewer loads each (1021 x 1793, 120 tiles: 4.8 us, 6.8 with 256; with a scale for
   // each row and column 6.0 and 9.5, and 28 and 30.5 for 2048 tiles); past two tiles a CU, 256 threads overlap more
   // tiles where one scale leaves little to compute (1024 tiles: 13.7 and 12.9)
-  if (!BLOCK || tiles <= 512)
-    quantize_tile_kernel<T, BLOCK, 1024><<<static_cast<uint32_t>(tiles), 1024, 0, s>>>(p);
-  else
-    quantize_tile_kernel<T, BLOCK, 256><<<static_cast<uint32_t>(tiles), 256, 0, s>>>(p);
-  return mm_check_launch("quantize_tile_kernel");
+  if (!BLOCK || tiles <= 512) return launch(quantize_tile_kernel<T, BLOCK, 1024>, tiles, 1024, p, s);
+  return launch(quantize_tile_kernel<T, BLOCK, 256>, tiles, 256, p, s);
 }
 
 }  // namespace
