@@ -177,8 +177,8 @@ __global__ __launch_bounds__(kFewRoutes) void fp8_few_kernel(FewArgs f) {
 // Rows of K bytes, K a multiple of 128: 16-byte vectors of a stage, NT threads.
 template <int ROWS, int NT>
 struct RowPanel {
-  // 32 rows of 8 waves: the upper half of the threads has a vector that the lower one has too
-  static constexpr int PER = (ROWS * 8 + NT - 1) / NT;
+  static constexpr int PER = ROWS * 8 / NT;
+  static_assert(PER * NT == ROWS * 8, "whole vectors");
   static constexpr bool CUTS = false;
   struct Stage {
     i32x4 d[PER];
@@ -190,7 +190,7 @@ struct RowPanel {
   __device__ __forceinline__ RowPanel(const uint8_t* p, int K, const F& row) : base(reinterpret_cast<const char*>(p)) {
 #pragma unroll
     for (int v = 0; v < PER; ++v) {
-      const int c = (v * NT + threadIdx.x) % (ROWS * 8);
+      const int c = v * NT + threadIdx.x;
       off[v] = static_cast<uint32_t>(row(c / 8)) * static_cast<uint32_t>(K) + c % 8 * 16;
     }
   }
@@ -198,7 +198,7 @@ struct RowPanel {
     load_at(r.d[v], base + k, off[v]);
   }
   __device__ __forceinline__ void put_one(int8_t* lds, const Stage& r, int v) const {
-    const int c = (v * NT + threadIdx.x) % (ROWS * 8);
+    const int c = v * NT + threadIdx.x;
     *reinterpret_cast<i32x4*>(lds + slot_of(c / 8, c % 8)) = r.d[v];
   }
   __device__ __forceinline__ void load(Stage& r, int k) const {

@@ -270,8 +270,10 @@ int launch_tiles(const QuantArgs& p, hipStream_t s) {
   // 1024 threads a tile wait for fewer loads each (1021 x 1793, 120 tiles: 4.8 us, 6.8 with 256; with a scale for
   // each row and column 6.0 and 9.5, and 28 and 30.5 for 2048 tiles); past two tiles a CU, 256 threads overlap more
   // tiles where one scale leaves little to compute (1024 tiles: 13.7 and 12.9)
-  if (!BLOCK || tiles <= 512) return launch(quantize_tile_kernel<T, BLOCK, 1024>, tiles, 1024, p, s);
-  return launch(quantize_tile_kernel<T, BLOCK, 256>, tiles, 256, p, s);
+  if constexpr (BLOCK) {
+    if (tiles > 512) return launch(quantize_tile_kernel<T, BLOCK, 256>, tiles, 256, p, s);
+  }
+  return launch(quantize_tile_kernel<T, BLOCK, 1024>, tiles, 1024, p, s);
 }
 
 }  // namespace
