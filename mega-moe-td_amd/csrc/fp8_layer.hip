@@ -385,7 +385,7 @@ static_assert(kBytes <= 160 * 1024, "fits LDS");
 __device__ __forceinline__ int scale_slot(int r) { return (r >> 3 & 7) * kWaveScales + (r >> 6) * 8 + (r & 7); }
 }  // namespace ring
 
-// ONCE: weights that the caches need not keep. WIDE (FC1): sums in fp32 throughout for up to 64 rows.
+// ONCE: weights that the caches need not keep. WIDE (FC1): sums in fp32 throughout.
 template <bool FC1, bool ONCE, bool WIDE>
 struct Ring {
   struct Item {
@@ -480,7 +480,6 @@ struct Ring {
   template <int MI>
   __device__ __forceinline__ void run() {
     constexpr int NI = 4, ROWS = kTile * MI;
-    constexpr bool EXACT = WIDE && MI <= 2;
     int id = lane;  // kept from the other heights' addresses, which would all be held in registers
     asm volatile("" : "+v"(id));
     const int j = id & 15, q = id >> 4;
@@ -509,6 +508,33 @@ struct Ring {
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int c = 0; c < NI; ++c) acc[i][c] = f32x4{0, 0, 0, 0};
+    if constexpr (WIDE && MI > 2) {
+      // The next stage's bytes and this one's in bf16 do not fit the registers together with so many sums: here a
+      // stage is read when it is there, its channels kept in bf16, its rows 16 by 16.
+      for (int s = 0; s < stages; ++s) {
+        const int8_t* const now = lds + buf * ring::kStage;
+        if (s < kb) {
+          scales(now, as, bs);
+          Op16Wide::Frag fw[NI];
+#pragma unroll
+          for (int c = 0; c < NI; ++c) fw[c] = Op16Wide::frag(bytes_b(now, c));
+#pragma unroll
+          for (int i = 0; i < MI; ++i) {
+            const Op16Wide::Frag wide = Op16Wide::frag(bytes_a(now, i));
+#pragma unroll
+            for (int c = 0; c < NI; ++c) acc[i][c] = Op16Wide::mac(fw[c], wide, acc[i][c], bs[c / 2], as[i]);
+          }
+        }
+        wait_copies<(ring::kDepth - 2) * ring::kCopies>();
+        __syncthreads();
+        if (s + 1 < stages) {
+          copy(s + ring::kDepth, buf);
+          buf = buf + 1 == ring::kDepth ? 0 : buf + 1;
+        }
+      }
+      finish<MI>(acc, lds + buf * ring::kStage);
+      return;
+    }
     const int8_t* b = lds + buf * ring::kStage;
 #pragma unroll
     for (int i = 0; i < MI; ++i) fa[i] = bytes_a(b, i);
@@ -519,8 +545,8 @@ struct Ring {
       const int next_buf = buf + 1 == ring::kDepth ? 0 : buf + 1;
       const int8_t* const now = lds + buf * ring::kStage;
       const int8_t* const nxt = lds + next_buf * ring::kStage;
-      Op16Wide::Frag wide[EXACT ? MI : 1];
-      if constexpr (EXACT) {
+      Op16Wide::Frag wide[WIDE ? MI : 1];
+      if constexpr (WIDE) {
 #pragma unroll
         for (int i = 0; i < MI; ++i) wide[i] = Op16Wide::frag(fa[i]);
       }
@@ -539,12 +565,12 @@ struct Ring {
         if (!(tail && LAST)) fb_next = tail ? bytes_b(nxt, 0) : bytes_b(now, c + 1);
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-          if constexpr (!EXACT) {
+          if constexpr (!WIDE) {
             acc[i][c] = Op16::mac(fb, fa[i], acc[i][c], bs[FC1 ? c / 2 : wn / 2], as[i]);
             if (tail && !LAST) fa[i] = bytes_a(nxt, i);
           }
         }
-        if constexpr (EXACT) {
+        if constexpr (WIDE) {
           const Op16Wide::Frag fw = Op16Wide::frag(fb);
 #pragma unroll
           for (int i = 0; i < MI; ++i) {
@@ -908,7 +934,8 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
   // The E4M3 instruction's sums are 1.5e-5 off, which moves 1 of 3000 activations by a step of E4M3, and the scale of 1
   // of 25000 blocks: among many 0.0017 of the result's norm, as much as bf16 rounds. Among few it can be several times
   // that (800 rows, I 128: 0.007 once in ten), so few are summed in fp32 throughout: up to 2 million where FC1 waits for
-  // weights anyhow (64 experts of 4 rows, H 7168: 468 us, 450 otherwise), else up to half a million (16 experts of 80
+  // weights anyhow (64 experts of 4 rows, H 7168: 468 us, 450 otherwise; an item of more than 64 rows takes as long to
+  // multiply as to load: 8 experts of 62 rows, H 7168, 182 and 127), else up to half a million (16 experts of 80
   // rows, H 1024, I 256: 36 and 37 us, but 8 of 80, H 4096, I 1536: 125 and 78).
   const bool wide = R * inter <= int64_t(1) << (mean <= 64 ? 21 : 19);
   const int64_t fc1_cblocks = inter / kBlock, fc2_cblocks = (hidden + 255) / 256;
