@@ -331,7 +331,8 @@ typedef __attribute__((address_space(3))) void lds_void;
 __device__ __forceinline__ uint32_t lds_offset(const int8_t* p) {
   return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)(p))));
 }
-// A wave's copy of 16 bytes a lane, lane l's to `lds` + 16 l.
+// A wave's copy of 16 bytes a lane, lane l's to `lds` + 16 l. (m0 cannot be declared as written: it is the compiler's
+// own, which keeps nothing in it and sets it in front of each of its uses, of which these kernels have none.)
 __device__ __forceinline__ void copy_lines(const char* base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
 }
@@ -339,10 +340,11 @@ __device__ __forceinline__ void copy_lines(const char* base, uint32_t off, uint3
 __device__ __forceinline__ void copy_lines_once(const char* base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "s"(lds) : "memory");
 }
-// Of a byte each in the first 26 lanes, lane l's to the word at `lds` + 4 l; every lane is active around it.
+// Of a byte each in the first 26 lanes, lane l's to the word at `lds` + 4 l.
 __device__ __forceinline__ void copy_scales(const uint8_t* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 exec, 0x3ffffff\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off\n\ts_mov_b64 exec, -1"
-               ::"v"(p), "s"(lds) : "memory");
+  uint64_t lanes;
+  asm volatile("s_and_saveexec_b64 %0, %3\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off\n\ts_mov_b64 exec, %0"
+               : "=&s"(lanes) : "v"(p), "s"(lds), "s"(uint64_t(0x3ffffff)) : "memory", "scc");
 }
 // Of a float a lane.
 __device__ __forceinline__ void copy_float(const float* p, uint32_t lds) {
