@@ -1,11 +1,12 @@
 // The layer on E4M3 rows and E4M3 experts with a power-of-two scale for each
 // block of 128 (fp8.h).
 //
-//   gu[i, :]  = x[token(i), :] W1[e]^T                 (fp32, e = expert of expert-major row i)
+//   gu[i, :]  = x[token(i), :] W1[e]^T                 (held in fp32, e = expert of expert-major row i)
 //   act[i, :] = act_fn(gate, up) * w[i], then E4M3 with a scale for each 128 columns
-//   y[i, :]   = act[i, :] W2[e]^T                      (fp32)
+//   y[i, :]   = act[i, :] W2[e]^T                      (held in fp32)
 //   out[t, :] = sum_j y[route_to_send[t k + j], :]     (fp32, slot order)
 //
+// gu and y are summed as fp8_tile.h says, gu of few activations in fp32 throughout.
 // Routing tables and tile lists are those of the bf16 layer (a few rows need none). The experts' outputs
 // stay in fp32 until the slots are summed: in bf16 each would be off by as much
 // as the result is by its own rounding.
@@ -933,7 +934,7 @@ extern "C" int mm_moe_fp8(const uint8_t* x, const uint8_t* x_scale, const int32_
   // (H 7168, I 2048, E 16: 120 rows 179 us with the ring and 196 in tiles of 256, 150 rows 282 and 219, 200 rows 343
   // and 230, 2000 rows 2.23 and 1.67 ms)
   const bool streamed = mean <= 128;
-  // The E4M3 instruction's sums are 1.5e-5 off, which moves 1 of 3000 activations by a step of E4M3, and the scale of 1
+  // The E4M3 instruction's sums are 1.4e-5 off, which moves 1 of 3000 activations by a step of E4M3, and the scale of 1
   // of 25000 blocks: among many 0.0017 of the result's norm, as much as bf16 rounds. Among few it can be several times
   // that (800 rows, I 128: 0.007 once in ten), so few are summed in fp32 throughout: up to 2 million where FC1 waits for
   // weights anyhow (64 experts of 4 rows, H 7168: 468 us, 450 otherwise; an item of more than 64 rows takes as long to

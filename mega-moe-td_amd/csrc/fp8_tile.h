@@ -7,11 +7,15 @@
 // What the E4M3 instructions sum in: of 8 neighbouring products each is cut 13
 // bits below the largest before they are added (measured: with products of 2^p
 // and 2^q in one such group the smaller is lost from p - q = 14 on, in another
-// group at 24; the same in all three E4M3 instructions), which leaves 1.5e-5 of a
-// sum of normal values whatever its length. Results in 16 bits do not show it
-// (half a step is 2^-9 or 2^-11). Results in 32 bits are summed by the bf16
-// instruction, which holds E4M3 values exactly and adds in fp32, at half the
-// rate.
+// group at 24; the same in all three E4M3 instructions). A sum is off by at most
+// 7 * 2^-13 (8.5e-4) of its groups' largest products, by 1.4e-5 of it (root mean
+// square, no bias) where values are random, whatever its length. Results in 16 bits
+// are summed so by choice: of random values it is little beside their own rounding
+// (half a step is 2^-8 or 2^-11), the operands were rounded by up to 2^-4, and sums
+// in fp32 take twice the matrix time. It shows where large products cancel (448 *
+// 448 - 448 * 448 + 1 is 0), and in fp16 where most of a sum lies in products 2^-13
+// of their neighbour's size. Results in 32 bits are summed by the bf16 instruction,
+// which holds E4M3 values exactly and adds in fp32, at half the rate.
 #pragma once
 
 #include "fp8.h"

@@ -482,13 +482,18 @@ class FusedMoEForward(torch.nn.Module):
 
         ``tokens`` float8_e4m3fn [T, H] with float8_e8m0fnu ``token_scale``
         [T, H / 128], as ``rms_norm`` (``scale_columns=128``) and
-        ``quantize_blocks`` make them; returns bf16 [T, H]. Sums are fp32; the
-        activation (times the routing weight) goes to FC2 in E4M3 with a scale for
+        ``quantize_blocks`` make them; returns bf16 [T, H]. The
+        activation (fp32, times the routing weight) goes to FC2 in E4M3 with a scale for
         each 128 columns, and the experts' outputs to the sum over the slots in
-        fp32. Few activations are summed in fp32 before they are rounded, many by the
-        E4M3 instruction, which is 1.4e-5 off. ``tokens`` and the experts' tensors are aligned to 16 bytes, as new
-        tensors and whole rows or experts of them are; T H and 2 I H are below
-        2^32. A NaN scale makes its own token's output NaN (where any slot of the
+        fp32. FC2 sums as ``fp8_matmul`` does for bf16, products more than 13 bits
+        below their largest neighbour cut (1.4e-5 of a sum of random values). FC1 sums
+        many activations so too, which moves one of about 3000 to the neighbouring
+        E4M3 value, and few in fp32 throughout. Which it is depends on the call's sizes
+        and not on its routing: with R = T top_k routes few are R I up to 2^19, or up
+        to 2^21 where R is up to 64 E, and R up to 64 (and 16 E), or up to 256 that
+        read up to 512 MB of weights. ``tokens`` and the experts' tensors are aligned to
+        16 bytes, as new tensors and whole rows or experts of them are; T H and 2 I H
+        are below 2^32. A NaN scale makes its own token's output NaN (where any slot of the
         token has an expert) and no other's. Nothing is saved for a backward and
         operands that ask for a gradient are refused; no workspace of the operator
         is used, so calls may run on any stream and captured. No counterpart in

@@ -1,8 +1,10 @@
-"""How the E4M3 layer sums few activations: in fp32 throughout, whatever the routing."""
+"""How the E4M3 operators sum: few activations of the layer and results in 32 bits in fp32
+throughout, results in 16 bits within the bound that they are documented with."""
 
 import pytest
 import torch
 
+import mega_moe
 from tests import _fp8 as R
 from tests.test_gpu_fp8_layer import make, operator, reference
 
@@ -85,3 +87,39 @@ def test_few_activations_keep_what_cancels(size, expert):
         size_of += ((sel.cpu() == e) * w.cpu()).sum(1, keepdim=True).double() * 0.78 * down  # silu(1) and half an E4M3 step
     assert ref.abs().max() > 0.1 * size_of.max() / I ** 0.5
     R.near(out, ref, 2.0 ** -8 * ref.abs() + 2.0 ** -10 * size_of)
+
+
+# ------------------------------------------------------------------ products
+PRODUCTS = [(3, 40, 517), (40, 300, 640), (300, 260, 1000), (1000, 1900, 700), (2500, 2500, 300), (4090, 4093, 385)]
+
+
+def _grouped(m, n, k, row, channel):
+    """E4M3 operands whose rows repeat ``row`` and ``channel``, all scales 1."""
+    make_rows = lambda r, c: torch.tensor(c, device="cuda").repeat(R.ceil(k, len(c)))[:k].expand(r, k).contiguous().to(R.F8)
+    scale = lambda *s: torch.full(s, 127, dtype=torch.uint8, device="cuda").view(R.E8)
+    kb = R.ceil(k, 128)
+    return make_rows(m, row), make_rows(n, channel), scale(m, kb), scale(R.ceil(n, 128), kb)
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_products_to_32_bits_keep_what_cancels(m, n, k):
+    """Every group of 8 holds 448 * 448 - 448 * 448 + 1: sums of whole numbers below 2^24, exact in fp32."""
+    a, b, sa, sb = _grouped(m, n, k, [448.0, 448.0, 1.0, 0, 0, 0, 0, 0], [448.0, -448.0, 1.0, 0, 0, 0, 0, 0])
+    want = (a[0].double() * b[0].double()).sum().item()
+    assert want < 448 * 448 + 1000
+    out = mega_moe.fp8_matmul(a, b, sa, sb, out_dtype=torch.float32)
+    assert (out == want).all()
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("small", [3.75, 4.0, 14.0])
+def test_products_to_16_bits_are_as_far_off_as_documented(m, n, k, dtype, small):
+    """Seven of eight products next to the border at which they are cut: within 7 * 2^-13 of the largest."""
+    a, b, sa, sb = _grouped(m, n, k, [448.0] + [small] * 7, [448.0] + [small] * 7)
+    sa.view(torch.uint8).sub_(14)  # into fp16's range
+    exact = (a[0].double() * b[0].double()).sum() * 2.0 ** -14
+    largest = R.ceil(k, 8) * 448.0 * 448.0 * 2.0 ** -14
+    out = mega_moe.fp8_matmul(a, b, sa, sb, out_dtype=dtype).double()
+    off = 7 * 2.0 ** -13 * largest + (128 + R.ceil(k, 128) + 16) * 2.0 ** -23 * exact
+    assert (out - exact).abs().max() <= off + R.half_step(dtype) * (exact + off)
