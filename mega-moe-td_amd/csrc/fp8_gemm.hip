@@ -186,10 +186,13 @@ __global__ __launch_bounds__(W * 64) void fp8_direct_kernel(Fp8Args p) {
 // BM x BN tile of tile_sums; the KS groups' sums are joined in order, and 16 rows
 // of a wave at a time go through its own LDS, padded to spread a pass
 // over the banks, so that neighbouring lanes store neighbouring 16 bytes. Large
-// products are bound by the matrix unit's power (8192 x 7168 x 4096: 202-212 us,
-// 2270-2380 TFLOP/s), small ones by LDS bandwidth (1021 x 2304 x 1793: 11.7 us)
-// and the shifting of odd rows (K = 2309 with a bias: 16.5 us), 17-64 rows by the
-// panels' way from L2 (64 x 7168 x 4096: 10.8 us).
+// products are bound by the matrix unit's power (8192 x 7168 x 4096: 194-212 us,
+// 2270-2480 TFLOP/s), small ones by a stage's chain of load, LDS, barrier and
+// fragments with one workgroup a CU (1021 x 2304 x 1793: 11.7 us, LDS busy 35% of
+// them, matrix units 20%) and the shifting of odd rows (K = 2309 with a bias: 16.5
+// us), 17-64 rows by the panels' way from L2 (64 x 7168 x 4096: 10.8 us), results
+// in 32 bits by their conversion beside the matrix unit (4096 x 4096 x 4096: 162-187
+// us, vector units busy 57%, matrix units 37%).
 template <class OP, int BM, int BN, int WM, int WN, int KS, int PRE, bool SHIFT>
 __global__ __launch_bounds__(WM * WN * KS * 64, OP::WAVES) void fp8_tile_kernel(Fp8Args p) {
   constexpr int NT = WM * WN * KS * 64, STEP = KS * BK, R = kTile, MI = BM / WM / R, NI = BN / WN / R;

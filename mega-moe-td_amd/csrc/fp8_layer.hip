@@ -324,10 +324,12 @@ __device__ __forceinline__ void rows_tile(const LayerArgs& p, int8_t* lds, const
 // with LDS busy for 20% of it and the matrix unit for 31%; 64 experts of 4 rows take
 // 277 us for 1.9 GB, 6.8 TB/s (with WIDE 290).
 //
-// The compiler does not know of the copies, so it waits for none by itself:
-// wait_copies and a barrier stand in front of what reads them. Loads that it knows
-// would wait for all of them: row numbers and tiles come through the scalar cache,
-// routing weights by a copy.
+// The compiler does not know of the copies: wait_copies and a barrier stand in front
+// of what reads them. A load that it knows waits for all of them: row numbers and
+// tiles come through the scalar cache, routing weights by a copy. What is left are
+// registers that it spills and loads again: in FC2 in front of every item and in the
+// last stage of those of more than 128 rows, in FC1 (not WIDE) behind the last stage
+// of those; there the ring is empty for a moment.
 typedef __attribute__((address_space(3))) void lds_void;
 __device__ __forceinline__ uint32_t lds_offset(const int8_t* p) {
   return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)(p))));
