@@ -44,7 +44,8 @@ def test_few_activations_of_uneven_experts_are_summed_in_32_bits(size, shares, a
     R.near(operator(T, H, k, E, act).forward_fp8(*ops), *reference(*ops, act, wide=True))
 
 
-@pytest.mark.parametrize("size", [(640, 1024, 256, 20, 1), (900, 512, 1024, 140, 2)])
+@pytest.mark.parametrize("size", [(640, 1024, 256, 20, 1), (900, 512, 1024, 140, 2),
+                                  (2000, 512, 1280, 40, 1), (1500, 256, 512, 16, 6)])  # the last two: many activations
 def test_a_token_does_not_see_where_the_others_go(size):
     """In a call of the same sizes: 8 tokens alone on their expert, and with 40, 100, 150 and 300 more beside them."""
     T, H, I, E, k = size
